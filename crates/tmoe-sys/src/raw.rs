@@ -13,6 +13,8 @@ pub const TMOE_E_UNSUPPORTED: c_int = -4;
 pub const TMOE_E_DEVICE: c_int = -5;
 pub const TMOE_E_COMM: c_int = -6;
 pub const TMOE_E_NOTFOUND: c_int = -7;
+pub const TMOE_TYPE_F32: c_int = 0;
+pub const TMOE_TYPE_BF16: c_int = 30;
 pub const TMOE_TYPE_Q4_K: c_int = 12;
 pub const TMOE_TYPE_Q6_K: c_int = 14;
 pub const TMOE_TYPE_Q6_K_R8: c_int = 270;
@@ -53,6 +55,39 @@ pub struct tmoe_config {
     pub max_tokens: i32,
     pub device: i32,
     pub rms_eps: f32,
+}
+
+/// The four planes of a 4-bit KV cache (`tmoe_kv4_cache`): caller-owned device memory.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct tmoe_kv4_cache {
+    pub k_codes: *mut c_void,
+    pub k_scales: *mut c_void,
+    pub v_codes: *mut c_void,
+    pub v_scales: *mut c_void,
+    pub n_seq: i32,
+    pub n_kv: i32,
+    pub head_dim: i32,
+    pub n_ctx: i32,
+}
+
+/// The tensors and options of an attention call over a 4-bit KV cache (`tmoe_kv4_attn`).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct tmoe_kv4_attn {
+    pub q: *const c_void,
+    pub k: *const c_void,
+    pub v: *const c_void,
+    pub out: *mut c_void,
+    pub scratch: *mut c_void,
+    pub q_ld: i64,
+    pub kv_ld: i64,
+    pub out_ld: i64,
+    pub ty: i32,
+    pub n_head: i32,
+    pub window: i32,
+    pub n_sink: i32,
+    pub scale: f32,
 }
 
 /// Stacked or slot expert tensors: device pointers into caller-owned ggml buffers.
@@ -447,6 +482,52 @@ extern "C" {
         rows: i64,
         n: i64,
         out: *mut i32,
+    ) -> c_int;
+    pub fn tmoe_kv4_store(
+        h: *mut tmoe_handle,
+        stream: *mut c_void,
+        cache: *const tmoe_kv4_cache,
+        ty: i32,
+        k: *const c_void,
+        v: *const c_void,
+        ld: i64,
+        seq: *const i32,
+        seq0: i32,
+        pos: *const i32,
+        pos0: i32,
+        n: i64,
+    ) -> c_int;
+    pub fn tmoe_kv4_load(
+        h: *mut tmoe_handle,
+        stream: *mut c_void,
+        cache: *const tmoe_kv4_cache,
+        ty: i32,
+        k: *mut c_void,
+        v: *mut c_void,
+        ld: i64,
+        seq: *const i32,
+        seq0: i32,
+        pos: *const i32,
+        pos0: i32,
+        n: i64,
+    ) -> c_int;
+    pub fn tmoe_kv4_attn_scratch_bytes(h: *mut tmoe_handle) -> i64;
+    pub fn tmoe_kv4_attn_decode(
+        h: *mut tmoe_handle,
+        stream: *mut c_void,
+        cache: *const tmoe_kv4_cache,
+        attn: *const tmoe_kv4_attn,
+        pos: *const i32,
+        B: i32,
+    ) -> c_int;
+    pub fn tmoe_kv4_attn_prefill(
+        h: *mut tmoe_handle,
+        stream: *mut c_void,
+        cache: *const tmoe_kv4_cache,
+        attn: *const tmoe_kv4_attn,
+        seq: i32,
+        pos0: i32,
+        S: i32,
     ) -> c_int;
     pub fn tmoe_gguf_open(path: *const c_char, out: *mut *mut tmoe_gguf) -> c_int;
     pub fn tmoe_gguf_close(g: *mut tmoe_gguf);

@@ -68,6 +68,9 @@ extern "C" {
 #define TMOE_E_COMM -6      /* NCCL failure */
 #define TMOE_E_NOTFOUND -7  /* a GGUF key or tensor that the file does not have */
 
+/* element types of the 4-bit cache's activations (ggml's ids) */
+#define TMOE_TYPE_F32 0
+#define TMOE_TYPE_BF16 30
 #define TMOE_TYPE_Q4_K 12
 #define TMOE_TYPE_Q6_K 14
 /* Q6_K in this library's 8-row fragment order, made from Q6_K matrices by tmoe_prepack (not a
@@ -360,6 +363,76 @@ TMOE_API int tmoe_attn_prefill(tmoe_handle *h, void *stream, const float *q, con
                                int32_t n_head, int32_t n_kv, int32_t head_dim, int32_t n_ctx, float scale, float *out);
 TMOE_API int tmoe_add(tmoe_handle *h, void *stream, const float *a, const float *b, float *out, int64_t n);
 TMOE_API int tmoe_argmax(tmoe_handle *h, void *stream, const float *x, int64_t rows, int64_t n, int32_t *out);
+
+/* A KV cache held in 4 bits and the attention over it (no counterpart in the reference's own crates,
+ * whose caches are F16; the values are those of ggml's Q4_0).  A row (sequence, KV head, position) of
+ * K or of V is head_dim values (64 or 128) in blocks of 32; a block holds d * (c - 8), d one F16 scale
+ * and c a 4-bit code.  Per block, in f32 arithmetic, each operation rounded:
+ *     m = the value of the largest magnitude (the positive one of a pair);  d = m / -8 within +-65504
+ *     c = floor(x * (1 / d) + 8.5) within 0 .. 15;  d is kept as F16, and as 0 all values read as 0
+ * A NaN is stored as 0 and an infinity as the largest float: the cache holds finite values only.
+ * The caller owns four planes of device memory, 16-byte aligned:
+ *     codes  [n_seq][n_kv][n_ctx][head_dim / 2] bytes, value 2j of a block in the low half of its byte j;
+ *            block b's 16 bytes at slot b ^ ((position >> 1) & 3) of the row (head_dim 128) or
+ *            b ^ ((position >> 2) & 1) (head_dim 64)
+ *     scales [n_seq][n_kv][n_ctx][head_dim / 32] F16
+ * with n_ctx, the positions held per sequence and head, a multiple of 64.
+ *   tmoe_kv4_store        rows k, v [n][n_kv][head_dim] of `type` (TMOE_TYPE_F32 or TMOE_TYPE_BF16), ld
+ *                         elements apart, into the cache: row i at position pos[i] (pos NULL: pos0 + i)
+ *                         of sequence seq[i] (seq NULL: seq0, or sequence i where seq0 is negative).
+ *                         A negative position: no row.  The places of a call's rows are distinct
+ *   tmoe_kv4_load         the same rows back as values (zeros where there is no row)
+ *   tmoe_kv4_attn_decode  one new token for each of B sequences: its row k, v is stored at pos[b] of
+ *                         sequence b (k and v NULL: it is there already) and its query attends to the
+ *                         positions that it sees, the new one included, as the cache holds them.
+ *                         pos[b] negative: sequence b has no token; nothing is stored, zeros come out
+ *   tmoe_kv4_attn_prefill S tokens of sequence `seq` at pos0 .. pos0 + S - 1: their rows are stored
+ *                         (k and v NULL: they are there already), then every query attends
+ * A query at position t sees position p if p <= t and (window is 0, or t - p < window, or p < n_sink):
+ * full causal attention, or a sliding window with the first n_sink positions always in sight.
+ * Out = softmax(scale * q . K) V per head; query head h reads KV head h / (n_head / n_kv).  Statistics and
+ * sums are f32.  Decoding with f32 activations computes to f32 precision; with bf16, P is rounded to 16
+ * bits once.  The prefill takes Q, K, P and V to the tensor cores as F16 with either type, as
+ * tmoe_attn_prefill does.
+ * scratch: tmoe_kv4_attn_scratch_bytes bytes, 16-byte aligned, zeroed once before its first use; every
+ * call leaves it ready for the next.  Calls that may run at the same time need a scratch each.
+ * A sequence or position outside the cache is skipped (its output zero) and latches the device error
+ * (tmoe_check).  q, k, v, out and their ld in bytes are multiples of 16. */
+typedef struct {
+    void *k_codes;
+    void *k_scales;
+    void *v_codes;
+    void *v_scales;
+    int32_t n_seq;
+    int32_t n_kv;
+    int32_t head_dim;
+    int32_t n_ctx;
+} tmoe_kv4_cache;
+typedef struct {
+    const void *q;   /* [tokens][n_head][head_dim], q_ld elements from token to token */
+    const void *k;   /* [tokens][n_kv][head_dim], kv_ld; NULL (with v): the rows are in the cache */
+    const void *v;
+    void *out;       /* [tokens][n_head][head_dim], out_ld */
+    void *scratch;
+    int64_t q_ld;
+    int64_t kv_ld;
+    int64_t out_ld;
+    int32_t type;    /* of q, k, v and out: TMOE_TYPE_F32 or TMOE_TYPE_BF16 */
+    int32_t n_head;  /* a multiple of the cache's n_kv */
+    int32_t window;  /* 0: none */
+    int32_t n_sink;
+    float scale;
+} tmoe_kv4_attn;
+TMOE_API int tmoe_kv4_store(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cache, int32_t type, const void *k,
+                            const void *v, int64_t ld, const int32_t *seq, int32_t seq0, const int32_t *pos,
+                            int32_t pos0, int64_t n);
+TMOE_API int tmoe_kv4_load(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cache, int32_t type, void *k, void *v,
+                           int64_t ld, const int32_t *seq, int32_t seq0, const int32_t *pos, int32_t pos0, int64_t n);
+TMOE_API int64_t tmoe_kv4_attn_scratch_bytes(tmoe_handle *h);
+TMOE_API int tmoe_kv4_attn_decode(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cache, const tmoe_kv4_attn *attn,
+                                  const int32_t *pos, int32_t B);
+TMOE_API int tmoe_kv4_attn_prefill(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cache, const tmoe_kv4_attn *attn,
+                                   int32_t seq, int32_t pos0, int32_t S);
 
 /* GGUF model files (crates/model/src/gguf.rs; the loader of load_weights, qwen3moe.rs:2498-2584).
  *   tmoe_gguf_open        <- Gguf::open (gguf.rs:236-296): the header, metadata and tensor index of a

@@ -14,6 +14,7 @@ TMOE_OK = 0
 ERRORS = {-1: "TMOE_E_INVALID", -2: "TMOE_E_CUDA", -3: "TMOE_E_NOMEM", -4: "TMOE_E_UNSUPPORTED",
           -5: "TMOE_E_DEVICE", -6: "TMOE_E_COMM", -7: "TMOE_E_NOTFOUND"}
 TMOE_E_INVALID, TMOE_E_UNSUPPORTED, TMOE_E_NOTFOUND = -1, -4, -7
+TYPE_F32, TYPE_BF16 = 0, 30  # element types of the 4-bit cache's activations
 TYPE_Q4_K, TYPE_Q6_K = 12, 14
 TYPE_Q6_K_R8 = 270  # Q6_K in 8-row fragment order (tmoe_prepack)
 
@@ -37,6 +38,19 @@ class ExpertTensors(C.Structure):
                 ("up_nb1", C.c_size_t), ("up_nb2", C.c_size_t),
                 ("down_nb1", C.c_size_t), ("down_nb2", C.c_size_t),
                 ("n_slots", C.c_int32)]
+
+
+class Kv4CacheStruct(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p),
+                ("v_scales", C.c_void_p), ("n_seq", C.c_int32), ("n_kv", C.c_int32),
+                ("head_dim", C.c_int32), ("n_ctx", C.c_int32)]
+
+
+class Kv4AttnStruct(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+                ("scratch", C.c_void_p), ("q_ld", C.c_int64), ("kv_ld", C.c_int64), ("out_ld", C.c_int64),
+                ("type", C.c_int32), ("n_head", C.c_int32), ("window", C.c_int32), ("n_sink", C.c_int32),
+                ("scale", C.c_float)]
 
 
 P = C.c_void_p
@@ -99,6 +113,11 @@ SIGNATURES = {
     "tmoe_attn_decode_scratch_bytes": ([P, I32, I32, I32, I32, I32], I64),
     "tmoe_attn_decode": ([P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, C.c_float, P, P], C.c_int),
     "tmoe_attn_prefill": ([P, P, P, P, P, P, P, I32, I32, I32, I32, I32, I32, I32, I32, C.c_float, P], C.c_int),
+    "tmoe_kv4_store": ([P, P, P, I32, P, P, I64, P, I32, P, I32, I64], C.c_int),
+    "tmoe_kv4_load": ([P, P, P, I32, P, P, I64, P, I32, P, I32, I64], C.c_int),
+    "tmoe_kv4_attn_scratch_bytes": ([P], I64),
+    "tmoe_kv4_attn_decode": ([P, P, P, P, P, I32], C.c_int),
+    "tmoe_kv4_attn_prefill": ([P, P, P, P, I32, I32, I32], C.c_int),
     "tmoe_add": ([P, P, P, P, P, I64], C.c_int),
     "tmoe_argmax": ([P, P, P, I64, I64, P], C.c_int),
     "tmoe_trace_open": ([C.c_char_p, C.POINTER(C.c_void_p)], C.c_int),

@@ -35,6 +35,7 @@ __host__ __device__ __forceinline__ int q6r_offset(int g, int off) {
 #define TMOE_DEV_ERR_TIMEOUT 1
 #define TMOE_DEV_ERR_BADID 2
 #define TMOE_DEV_ERR_NOSLOT 3  // every expert slot is pinned: a miss has nowhere to go
+#define TMOE_DEV_ERR_BADPOS 4  // a row's sequence or position lies outside its 4-bit cache
 
 // A bounded wait gives up after this many nanoseconds of %globaltimer.
 #define TMOE_WAIT_LIMIT_NS 1000000000ull

@@ -278,4 +278,23 @@ cudaError_t launch_slot_unstage(const SlotsDev &s, int chunk, const SlotCopy &cp
 int gemv_rows_per_item(int wt, int K, int N);
 cudaError_t launch_gemv(int wt, bool gateup, const GemvArgs &a, int max_items, int sm_count, cudaStream_t st);
 
+// kv4.cu, kv4_prefill.cu: the 4-bit KV cache and the attention over it
+struct Kv4Planes;
+// rows (seq[i] or seq0, or i where seq0 < 0; pos[i] or pos0 + i) from k, v into the cache, or back
+cudaError_t launch_kv4_rows(bool store, bool f32, int head_dim, void *k, void *v, int64_t ld, const int32_t *seq,
+                            int seq0, const int32_t *pos, int pos0, int64_t n, const Kv4Planes &c, int *err,
+                            cudaStream_t st);
+struct Kv4Attn {
+    const void *q, *k, *v;  // k, v nullptr: the new rows are in the cache already
+    void *out;
+    int64_t q_ld, kv_ld, out_ld;
+    const int32_t *pos;  // nullptr: token t at pos0 + t
+    int pos0, seq0;      // seq0 < 0: token t is of sequence t
+    int n_tok, n_head, window, n_sink;
+    float scale;
+};
+size_t kv4_attn_scratch_bytes(int sm_count);
+cudaError_t launch_kv4_attn(bool f32, int head_dim, Kv4Attn &x, const Kv4Planes &c, void *scratch, int sm_count,
+                            int *err, cudaStream_t st);
+
 }  // namespace tmoe

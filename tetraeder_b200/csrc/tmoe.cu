@@ -13,6 +13,7 @@
 #include "../../include/tmoe.h"
 #include "common.cuh"
 #include "kernels.cuh"
+#include "kv4.cuh"
 
 namespace {
 
@@ -686,6 +687,8 @@ int tmoe_check(tmoe_handle *h, void *stream) {
         cudaMemset(h->err, 0, sizeof(int));
         if (flag == TMOE_DEV_ERR_BADID) return fail(h, TMOE_E_INVALID, "an expert id was >= n_slots");
         if (flag == TMOE_DEV_ERR_NOSLOT) return fail(h, TMOE_E_INVALID, "no free expert slot (all pinned)");
+        if (flag == TMOE_DEV_ERR_BADPOS)
+            return fail(h, TMOE_E_INVALID, "a sequence or position lay outside the 4-bit cache");
         return fail(h, TMOE_E_DEVICE, "a kernel gave up on a bounded wait (code %d)", flag);
     }
     return TMOE_OK;
@@ -1405,6 +1408,162 @@ int tmoe_attn_prefill(tmoe_handle *h, void *stream, const float *q, const float 
     const cudaError_t e = tmoe::launch_attn_prefill(q, k, v, (__half *)k_cache, (__half *)v_cache, seq, pos0, S, n_head,
                                                     n_kv, head_dim, n_ctx, scale, out, (cudaStream_t)stream);
     return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "prefill attention");
+}
+
+// ---------------------------------------------------------------- the 4-bit KV cache
+namespace {
+
+constexpr int kKv4MaxCtx = 1 << 28;
+
+int check_kv4_cache(tmoe_handle *h, const tmoe_kv4_cache *c) {
+    if (!c) return fail(h, TMOE_E_INVALID, "null cache");
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return fail(h, TMOE_E_UNSUPPORTED, "4-bit cache of %d-wide heads (64 or 128)", c->head_dim);
+    if (c->n_seq <= 0 || c->n_kv <= 0 || c->n_kv > 32767 || c->n_ctx <= 0 || c->n_ctx % 64 || c->n_ctx > kKv4MaxCtx)
+        return fail(h, TMOE_E_INVALID, "4-bit cache of %d sequences, %d KV heads, %d positions (a multiple of 64)",
+                    c->n_seq, c->n_kv, c->n_ctx);
+    if (!c->k_codes || !c->k_scales || !c->v_codes || !c->v_scales) return fail(h, TMOE_E_INVALID, "null plane");
+    if (!aligned16(c->k_codes) || !aligned16(c->k_scales) || !aligned16(c->v_codes) || !aligned16(c->v_scales))
+        return fail(h, TMOE_E_INVALID, "the planes must be 16-byte aligned");
+    return TMOE_OK;
+}
+
+tmoe::Kv4Planes kv4_planes(const tmoe_kv4_cache *c) {
+    return {(uint8_t *)c->k_codes, (__half *)c->k_scales, (uint8_t *)c->v_codes, (__half *)c->v_scales,
+            c->n_seq, c->n_kv, c->n_ctx};
+}
+
+// Activation rows `ld` elements of `type` apart, each of `width` elements.
+int check_kv4_rows(tmoe_handle *h, const char *what, int type, const void *p, int64_t ld, int64_t width) {
+    const int64_t size = type == TMOE_TYPE_F32 ? 4 : 2;
+    if (!p) return fail(h, TMOE_E_INVALID, "null %s", what);
+    if (ld < width) return fail(h, TMOE_E_INVALID, "%s: rows of %lld elements, %lld apart", what, (long long)width, (long long)ld);
+    if (!aligned16(p) || (ld * size) % 16) return fail(h, TMOE_E_INVALID, "%s: rows must be 16-byte aligned", what);
+    return TMOE_OK;
+}
+
+int kv4_rows(tmoe_handle *h, void *stream, const tmoe_kv4_cache *c, bool store, int type, void *k, void *v, int64_t ld,
+             const int32_t *seq, int32_t seq0, const int32_t *pos, int32_t pos0, int64_t n) {
+    if (!h) return TMOE_E_INVALID;
+    int rc = check_kv4_cache(h, c);
+    if (rc != TMOE_OK) return rc;
+    if (type != TMOE_TYPE_F32 && type != TMOE_TYPE_BF16) return fail(h, TMOE_E_UNSUPPORTED, "4-bit cache rows of type %d", type);
+    if (n < 0 || n > (1ll << 30)) return fail(h, TMOE_E_INVALID, "%lld rows", (long long)n);
+    if (!seq && (seq0 >= c->n_seq || (seq0 < 0 && n > c->n_seq)))
+        return fail(h, TMOE_E_INVALID, "%lld rows from sequence %d: the cache holds %d", (long long)n, seq0, c->n_seq);
+    if (!pos && (pos0 < 0 || pos0 + n > c->n_ctx))
+        return fail(h, TMOE_E_INVALID, "%lld rows at position %d: the cache holds %d", (long long)n, pos0, c->n_ctx);
+    if (n == 0) return TMOE_OK;
+    const int64_t width = (int64_t)c->n_kv * c->head_dim;
+    if ((rc = check_kv4_rows(h, "k", type, k, ld, width)) != TMOE_OK) return rc;
+    if ((rc = check_kv4_rows(h, "v", type, v, ld, width)) != TMOE_OK) return rc;
+    DeviceGuard dg(h->cfg.device);
+    tmoe::PdlScope pdl(!h->prof.on);  // overlap with the kernel before (programmatic launch)
+    const cudaError_t e = tmoe::launch_kv4_rows(store, type == TMOE_TYPE_F32, c->head_dim, k, v, ld, seq, seq0, pos, pos0,
+                                                n, kv4_planes(c), h->err, (cudaStream_t)stream);
+    return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, store ? "kv4 store" : "kv4 load");
+}
+
+int check_kv4_attn(tmoe_handle *h, const tmoe_kv4_cache *c, const tmoe_kv4_attn *a) {
+    const int rc = check_kv4_cache(h, c);
+    if (rc != TMOE_OK) return rc;
+    if (!a) return fail(h, TMOE_E_INVALID, "null attention arguments");
+    if (a->type != TMOE_TYPE_F32 && a->type != TMOE_TYPE_BF16)
+        return fail(h, TMOE_E_UNSUPPORTED, "4-bit cache attention of type %d", a->type);
+    if (a->n_head <= 0 || a->n_head % c->n_kv || a->n_head > 65535)
+        return fail(h, TMOE_E_INVALID, "%d heads over %d KV heads", a->n_head, c->n_kv);
+    if (a->window < 0 || a->n_sink < 0) return fail(h, TMOE_E_INVALID, "window %d, %d sinks", a->window, a->n_sink);
+    if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return fail(h, TMOE_E_INVALID, "scale %g", (double)a->scale);
+    return TMOE_OK;
+}
+
+int check_kv4_tensors(tmoe_handle *h, const tmoe_kv4_cache *c, const tmoe_kv4_attn *a) {
+    int rc;
+    const int64_t qw = (int64_t)a->n_head * c->head_dim, kw = (int64_t)c->n_kv * c->head_dim;
+    if ((rc = check_kv4_rows(h, "q", a->type, a->q, a->q_ld, qw)) != TMOE_OK) return rc;
+    if ((rc = check_kv4_rows(h, "out", a->type, a->out, a->out_ld, qw)) != TMOE_OK) return rc;
+    if (a->k || a->v) {
+        if ((rc = check_kv4_rows(h, "k", a->type, a->k, a->kv_ld, kw)) != TMOE_OK) return rc;
+        if ((rc = check_kv4_rows(h, "v", a->type, a->v, a->kv_ld, kw)) != TMOE_OK) return rc;
+    }
+    if (!a->scratch || !aligned16(a->scratch)) return fail(h, TMOE_E_INVALID, "scratch must be 16-byte aligned memory");
+    return TMOE_OK;
+}
+
+tmoe::Kv4Attn kv4_attn(const tmoe_kv4_cache *c, const tmoe_kv4_attn *a) {
+    tmoe::Kv4Attn x;
+    x.q = a->q, x.k = a->k, x.v = a->v, x.out = a->out;
+    x.q_ld = a->q_ld, x.kv_ld = a->kv_ld, x.out_ld = a->out_ld;
+    x.pos = nullptr, x.pos0 = 0, x.seq0 = -1, x.n_tok = 0;
+    x.n_head = a->n_head;
+    x.window = a->window >= c->n_ctx ? 0 : a->window;  // a window over everything is none
+    x.n_sink = a->n_sink < c->n_ctx ? a->n_sink : c->n_ctx;
+    x.scale = a->scale;
+    return x;
+}
+
+}  // namespace
+
+int tmoe_kv4_store(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cache, int32_t type, const void *k,
+                   const void *v, int64_t ld, const int32_t *seq, int32_t seq0, const int32_t *pos, int32_t pos0,
+                   int64_t n) {
+    return kv4_rows(h, stream, cache, true, type, (void *)k, (void *)v, ld, seq, seq0, pos, pos0, n);
+}
+
+int tmoe_kv4_load(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cache, int32_t type, void *k, void *v,
+                  int64_t ld, const int32_t *seq, int32_t seq0, const int32_t *pos, int32_t pos0, int64_t n) {
+    return kv4_rows(h, stream, cache, false, type, k, v, ld, seq, seq0, pos, pos0, n);
+}
+
+int64_t tmoe_kv4_attn_scratch_bytes(tmoe_handle *h) {
+    if (!h) return TMOE_E_INVALID;
+    return (int64_t)tmoe::kv4_attn_scratch_bytes(h->sm_count);
+}
+
+int tmoe_kv4_attn_decode(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cache, const tmoe_kv4_attn *attn,
+                         const int32_t *pos, int32_t B) {
+    if (!h) return TMOE_E_INVALID;
+    int rc = check_kv4_attn(h, cache, attn);
+    if (rc != TMOE_OK) return rc;
+    if (B < 0 || B > cache->n_seq)
+        return fail(h, TMOE_E_INVALID, "%d tokens for a cache of %d sequences", B, cache->n_seq);
+    if (B == 0) return TMOE_OK;
+    if (!pos) return fail(h, TMOE_E_INVALID, "null pos");
+    if ((rc = check_kv4_tensors(h, cache, attn)) != TMOE_OK) return rc;
+    tmoe::Kv4Attn x = kv4_attn(cache, attn);
+    x.pos = pos, x.n_tok = B;
+    DeviceGuard dg(h->cfg.device);
+    tmoe::PdlScope pdl(!h->prof.on);  // overlap with the kernel before (programmatic launch)
+    const cudaError_t e = tmoe::launch_kv4_attn(attn->type == TMOE_TYPE_F32, cache->head_dim, x, kv4_planes(cache),
+                                                attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
+    return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "kv4 decode attention");
+}
+
+int tmoe_kv4_attn_prefill(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cache, const tmoe_kv4_attn *attn,
+                          int32_t seq, int32_t pos0, int32_t S) {
+    if (!h) return TMOE_E_INVALID;
+    int rc = check_kv4_attn(h, cache, attn);
+    if (rc != TMOE_OK) return rc;
+    if (S < 0 || seq < 0 || seq >= cache->n_seq || pos0 < 0 || (int64_t)pos0 + S > cache->n_ctx)
+        return fail(h, TMOE_E_INVALID, "prefill of %d tokens at position %d of sequence %d: the cache holds %d sequences "
+                                       "of %d positions", S, pos0, seq, cache->n_seq, cache->n_ctx);
+    if (S == 0) return TMOE_OK;
+    if ((rc = check_kv4_tensors(h, cache, attn)) != TMOE_OK) return rc;
+    tmoe::Kv4Attn x = kv4_attn(cache, attn);
+    x.pos0 = pos0, x.seq0 = seq, x.n_tok = S;
+    const bool f32 = attn->type == TMOE_TYPE_F32;
+    const tmoe::Kv4Planes planes = kv4_planes(cache);
+    DeviceGuard dg(h->cfg.device);
+    tmoe::PdlScope pdl(!h->prof.on);  // overlap with the kernel before (programmatic launch)
+    cudaError_t e = cudaSuccess;
+    if (x.k) {
+        e = tmoe::launch_kv4_rows(true, f32, cache->head_dim, (void *)x.k, (void *)x.v, x.kv_ld, nullptr, seq, nullptr,
+                                  pos0, S, planes, h->err, (cudaStream_t)stream);
+        if (e != cudaSuccess) return cuda_fail(h, e, "kv4 store");
+        x.k = x.v = nullptr;
+    }
+    e = tmoe::launch_kv4_attn(f32, cache->head_dim, x, planes, attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
+    return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "kv4 prefill attention");
 }
 
 int tmoe_add(tmoe_handle *h, void *stream, const float *a, const float *b, float *out, int64_t n) {

@@ -1,0 +1,203 @@
+"""The 4-bit KV cache and the attention over it (tmoe_kv4_* of include/tmoe.h, where the format and the
+rules stand): K and V rows are quantised as they are written, 4.5 bits a value against F16's 16, and the
+decode and prefill attention read them as they are.
+
+    cache = Kv4Cache(n_seq=8, n_kv=4, head_dim=128, n_ctx=32768)
+    out = cache.prefill(q, k, v, seq=0, pos0=0)            # [S, n_head, 128] queries of one sequence
+    out = cache.decode(q, k, v, pos, window=4096, n_sink=4)  # [B, n_head, 128], one token per sequence
+
+Activations are float32 or bfloat16 CUDA tensors; a token's heads are contiguous, tokens may be apart
+(views into a fused projection's output work)."""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16}
+_layers: dict = {}  # device ordinal -> a small handle, for caches made without one
+
+
+def _default_layer(device: int):
+    from .moe import MoeLayer
+    if device not in _layers:
+        _layers[device] = MoeLayer(512, 256, 8, 2, gate_type=_lib.TYPE_Q4_K, up_type=_lib.TYPE_Q4_K,
+                                   down_type=_lib.TYPE_Q4_K, max_tokens=4, device=device)
+    return _layers[device]
+
+
+class Kv4Cache:
+    """Planes k_codes, v_codes uint8 [n_seq, n_kv, capacity, head_dim / 2] and k_scales, v_scales float16
+    [n_seq, n_kv, capacity, head_dim / 32]; capacity is n_ctx rounded up to a multiple of 64.  `layer` (a
+    MoeLayer) gives the handle whose device error flag the calls use; without one, caches of a device
+    share a small handle.  One scratch per cache: its attention calls run on one stream, or ordered ones."""
+
+    def __init__(self, n_seq: int, n_kv: int, head_dim: int, n_ctx: int, device: int | None = None, layer=None):
+        if not torch.cuda.is_available():
+            raise RuntimeError("tetraeder_b200 needs a CUDA device (there is no CPU path)")
+        if n_seq <= 0 or n_kv <= 0 or n_ctx <= 0 or head_dim not in (64, 128):
+            raise ValueError(f"a 4-bit cache of {n_seq} sequences, {n_kv} KV heads of {head_dim} (64 or 128), "
+                             f"{n_ctx} positions")
+        if device is None:
+            device = torch.cuda.current_device() if layer is None else layer.device.index
+        dev = torch.device("cuda", device)
+        cap = -(-n_ctx // 64) * 64
+        planes = []
+        for _ in range(2):
+            planes.append(torch.zeros((n_seq, n_kv, cap, head_dim // 2), dtype=torch.uint8, device=dev))
+            planes.append(torch.zeros((n_seq, n_kv, cap, head_dim // 32), dtype=torch.float16, device=dev))
+        self._set(planes, layer)
+
+    @classmethod
+    def from_planes(cls, k_codes, k_scales, v_codes, v_scales, layer=None) -> "Kv4Cache":
+        """A cache over planes that the caller holds (contiguous, of the class's shapes)."""
+        self = cls.__new__(cls)
+        self._set([k_codes, k_scales, v_codes, v_scales], layer)
+        return self
+
+    def _set(self, planes, layer):
+        codes, scales = planes[0], planes[1]
+        if codes.dim() != 4 or scales.dim() != 4:
+            raise ValueError("planes are [n_seq, n_kv, positions, bytes or scales]")
+        n_seq, n_kv, cap, half = codes.shape
+        for i, t in enumerate(planes):
+            want = (n_seq, n_kv, cap, half if i % 2 == 0 else half // 16)
+            if tuple(t.shape) != want or t.dtype != (torch.float16 if i % 2 else torch.uint8):
+                raise ValueError(f"plane {i} is {t.dtype} {tuple(t.shape)}, not {want}")
+            if not t.is_cuda or t.device != codes.device or not t.is_contiguous():
+                raise ValueError("planes are contiguous CUDA tensors of one device")
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = planes
+        self.n_seq, self.n_kv, self.head_dim, self.n_ctx = n_seq, n_kv, 2 * half, cap
+        self.device = codes.device
+        self.layer = _default_layer(codes.device.index) if layer is None else layer
+        if self.layer.device != self.device:
+            raise ValueError("the layer's handle is of another device")
+        self.lib, self.h = self.layer.lib, self.layer.h
+        self._c = _lib.Kv4CacheStruct(*(t.data_ptr() for t in planes), n_seq, n_kv, self.head_dim, cap)
+        self._cp = C.addressof(self._c)
+        n = self.lib.tmoe_kv4_attn_scratch_bytes(self.h)
+        _lib.check(n if n < 0 else 0, self.h)
+        self._scratch = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        self._a = _lib.Kv4AttnStruct()
+        self._a.scratch = self._scratch.data_ptr()
+        self._ap = C.addressof(self._a)
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales))
+
+    # -- arguments -------------------------------------------------------------------------
+    def _heads(self, name, t, n, dtype, n_head=None):
+        """Elements from token to token of t [n, heads, head_dim] (a token's heads contiguous)."""
+        hd = self.head_dim
+        if t.dim() != 3 or t.shape[0] != n or t.shape[2] != hd or (n_head is not None and t.shape[1] != n_head):
+            raise ValueError(f"{name} is {tuple(t.shape)}, not [{n}, {'heads' if n_head is None else n_head}, {hd}]")
+        if t.dtype != dtype or t.device != self.device:
+            raise ValueError(f"{name} is {t.dtype} on {t.device}, not {dtype} on {self.device}")
+        ld, sh, sd = t.stride()
+        if sd != 1 or (sh != hd and t.shape[1] != 1):
+            raise ValueError(f"{name}: a token's heads must be contiguous")
+        return ld if n > 1 else t.shape[1] * hd
+
+    def _index(self, name, t, n):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != self.device or not t.is_contiguous():
+            raise ValueError(f"{name} is a contiguous int32 tensor [{n}] on {self.device}")
+        return t.data_ptr()
+
+    def _place(self, n, pos, seq):
+        """(seq, seq0, pos, pos0) of the C calls."""
+        p, pos0 = (self._index("pos", pos, n), 0) if torch.is_tensor(pos) else (None, int(pos))
+        if torch.is_tensor(seq):
+            return self._index("seq", seq, n), 0, p, pos0
+        if seq is None and p is None:
+            raise ValueError("a run of positions needs its sequence")
+        if seq is not None and not 0 <= seq < self.n_seq:
+            raise ValueError(f"sequence {seq} of {self.n_seq}")
+        return None, -1 if seq is None else int(seq), p, pos0
+
+    def _stream(self, stream):
+        return torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream.cuda_stream
+
+    def _type(self, t):
+        if t.dtype not in _TYPES:
+            raise ValueError(f"activations are float32 or bfloat16, not {t.dtype}")
+        return _TYPES[t.dtype]
+
+    # -- rows ------------------------------------------------------------------------------
+    def store(self, k, v, pos, seq=None, stream=None):
+        """Quantises rows k, v [n, n_kv, head_dim] into the cache: row i at position pos[i] of sequence
+        seq[i] (an int: that one; None: sequence i), or at pos + i of one sequence, where pos is an int.  A negative pos[i]: no row."""
+        n, ty = k.shape[0], self._type(k)
+        ld = self._heads("k", k, n, k.dtype, self.n_kv)
+        if self._heads("v", v, n, k.dtype, self.n_kv) != ld:
+            raise ValueError("k and v rows are different distances apart")
+        s, s0, p, p0 = self._place(n, pos, seq)
+        _lib.check(self.lib.tmoe_kv4_store(self.h, self._stream(stream), self._cp, ty, k.data_ptr(), v.data_ptr(), ld,
+                                           s, s0, p, p0, n), self.h)
+
+    def load(self, pos, n: int | None = None, seq=None, dtype=torch.float32, stream=None):
+        """The rows as values, (k, v) [n, n_kv, head_dim]: placed as in store (n: how many,
+        where pos is an int).  Zeros where pos[i] is negative."""
+        n = pos.shape[0] if torch.is_tensor(pos) else n
+        if n is None:
+            raise ValueError("load from an int position needs n")
+        if dtype not in _TYPES:
+            raise ValueError(f"rows come as float32 or bfloat16, not {dtype}")
+        s, s0, p, p0 = self._place(n, pos, seq)
+        k, v = torch.empty((2, n, self.n_kv, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+        _lib.check(self.lib.tmoe_kv4_load(self.h, self._stream(stream), self._cp, _TYPES[dtype], k.data_ptr(),
+                                          v.data_ptr(), self.n_kv * self.head_dim, s, s0, p, p0, n), self.h)
+        return k, v
+
+    # -- attention -------------------------------------------------------------------------
+    def _attn(self, q, k, v, window, n_sink, scale, out):
+        n, dt = q.shape[0], q.dtype
+        a = self._a
+        a.type = self._type(q)
+        a.q_ld = self._heads("q", q, n, dt)
+        a.n_head = n_head = q.shape[1]
+        if out is None:
+            out = torch.empty((n, n_head, self.head_dim), dtype=dt, device=self.device)
+            a.out_ld = n_head * self.head_dim
+        else:
+            a.out_ld = self._heads("out", out, n, dt, n_head)
+        if (k is None) != (v is None):
+            raise ValueError("k and v come together")
+        if k is None:
+            a.k = a.v = None
+        else:
+            a.kv_ld = self._heads("k", k, n, dt, self.n_kv)
+            if self._heads("v", v, n, dt, self.n_kv) != a.kv_ld:
+                raise ValueError("k and v rows are different distances apart")
+            a.k, a.v = k.data_ptr(), v.data_ptr()
+        a.q, a.out = q.data_ptr(), out.data_ptr()
+        a.window, a.n_sink = window, n_sink
+        a.scale = self.head_dim ** -0.5 if scale is None else scale
+        return out
+
+    def decode(self, q, k, v, pos, window: int = 0, n_sink: int = 0, scale: float | None = None, out=None, stream=None):
+        """One new token for each of B <= n_seq sequences: q [B, n_head, head_dim], its row k, v [B, n_kv, head_dim]
+        (None: stored already) at pos[b] (int32 CUDA [B]; negative: no token, zeros come out).  Each query
+        attends to positions 0..pos[b] of its sequence, with window > 0 to the last `window` of them and the
+        first n_sink.  Returns out [B, n_head, head_dim]."""
+        out = self._attn(q, k, v, window, n_sink, scale, out)
+        B = q.shape[0]
+        _lib.check(self.lib.tmoe_kv4_attn_decode(self.h, self._stream(stream), self._cp, self._ap,
+                                                 self._index("pos", pos, B), B), self.h)
+        return out
+
+    def prefill(self, q, k, v, seq: int = 0, pos0: int = 0, window: int = 0, n_sink: int = 0,
+                scale: float | None = None, out=None, stream=None):
+        """S new tokens of sequence `seq` at positions pos0 .. pos0 + S - 1: rows k, v [S, n_kv, head_dim] are stored
+        (None: stored already), then query i of q [S, n_head, head_dim] attends to positions 0 .. pos0 + i (or
+        its window and sinks).  Returns out [S, n_head, head_dim]."""
+        out = self._attn(q, k, v, window, n_sink, scale, out)
+        _lib.check(self.lib.tmoe_kv4_attn_prefill(self.h, self._stream(stream), self._cp, self._ap, seq, pos0,
+                                                  q.shape[0]), self.h)
+        return out
+
+    def check(self):
+        """Synchronises the current stream and raises if a kernel latched an error."""
+        _lib.check(self.lib.tmoe_check(self.h, self._stream(None)), self.h)
