@@ -294,6 +294,9 @@ struct Kv4Attn {
     float scale;
 };
 size_t kv4_attn_scratch_bytes(int sm_count);
+size_t kv4_prefill_part_bytes(int sm_count);
+cudaError_t launch_kv4_prefill(bool f32, int head_dim, const Kv4Attn &x, const Kv4Planes &c, void *scratch,
+                               int sm_count, int *err, cudaStream_t st);
 cudaError_t launch_kv4_attn(bool f32, int head_dim, Kv4Attn &x, const Kv4Planes &c, void *scratch, int sm_count,
                             int *err, cudaStream_t st);
 

@@ -178,12 +178,6 @@ __device__ __forceinline__ void ka_mma(float (&d)[PREC ? 4 : 2], const float (&c
             : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(0.0f), "f"(0.0f));
     }
 }
-__device__ __forceinline__ uint32_t ka_half2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    uint32_t u;
-    memcpy(&u, &h, 4);
-    return u;
-}
 __device__ __forceinline__ float2 ka_float2(uint32_t u) {
     __half2 h;
     memcpy(&h, &u, 4);
@@ -191,12 +185,10 @@ __device__ __forceinline__ float2 ka_float2(uint32_t u) {
 }
 // hi = f16(a, b), lo = f16 of what that leaves
 __device__ __forceinline__ void ka_split(float a, float b, uint32_t &hi, uint32_t &lo) {
-    hi = ka_half2(a, b);
+    hi = kv4_half2(a, b);
     const float2 f = ka_float2(hi);
-    lo = ka_half2(a - f.x, b - f.y);
+    lo = kv4_half2(a - f.x, b - f.y);
 }
-// 2^e, e in [-126, 127]
-__device__ __forceinline__ float ka_pow2(int e) { return __int_as_float((127 + e) << 23); }
 // (u & mask | 1024) - off as f16 pairs
 __device__ __forceinline__ uint32_t ka_codes(uint32_t u, uint32_t mask, __half2 off) {
     uint32_t r;
@@ -346,8 +338,8 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             // 2^e * top in [2^13, 2^14); two factors, as 2^e alone may not be a float
             const int e = top > 0.0f && top <= FLT_MAX ? 13 - ilogbf(top) : 0;
             const int e1 = e / 2, e2 = e - e1;
-            const float up1 = ka_pow2(e1), up2 = ka_pow2(e2);
-            to_log2 = a.scale * 1.4426950408889634f * ka_pow2(12 - e1) * ka_pow2(12 - e2);
+            const float up1 = kv4_pow2(e1), up2 = kv4_pow2(e2);
+            to_log2 = a.scale * 1.4426950408889634f * kv4_pow2(12 - e1) * kv4_pow2(12 - e2);
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 float z[8], sh = 0.0f, sl = 0.0f;
@@ -361,7 +353,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                         f = ka_float2(ql[b][i]);
                         sl += f.x + f.y;
                     } else {
-                        qh[b][i] = ka_half2(z[i], z[i + 4]);
+                        qh[b][i] = kv4_half2(z[i], z[i + 4]);
                     }
                     f = ka_float2(qh[b][i]);
                     sh += f.x + f.y;
@@ -565,7 +557,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                             if constexpr (PREC)
                                 ka_split(x, y, ph[b][e], pl[b][e]);
                             else
-                                ph[b][e] = ka_half2(x, y);
+                                ph[b][e] = kv4_half2(x, y);
                         }
                     }
                     uint32_t x0[NB], x1[NB];  // positions 0..7 and 8..15 of the step
@@ -722,8 +714,9 @@ cudaError_t launch_kv4_rows(bool store, bool f32, int head_dim, void *k, void *v
 }
 
 size_t kv4_attn_scratch_bytes(int sm_count) {
-    const size_t grid = 2 * (size_t)sm_count;
-    return grid * 4 + 2 * grid * KA_HEADS * (128 + 2) * 4;
+    const size_t grid = 2 * (size_t)sm_count, decode = 2 * grid * KA_HEADS * (128 + 2) * 4;
+    const size_t prefill = kv4_prefill_part_bytes(sm_count);
+    return kv4_counter_bytes(sm_count) + (decode > prefill ? decode : prefill);
 }
 
 template <int HD, typename T>
@@ -750,7 +743,7 @@ static cudaError_t attn_launch(Kv4Attn &x, const Kv4Planes &c, void *scratch, in
     a.pos = x.pos, a.pos0 = x.pos0, a.seq0 = x.seq0;
     a.n_tok = x.n_tok, a.n_head = x.n_head, a.window = x.window, a.n_sink = x.n_sink, a.scale = x.scale;
     a.arrived = (int *)scratch;
-    a.part = (float *)scratch + 2 * sm_count;
+    a.part = kv4_scratch_parts(scratch, sm_count);
     a.err = err;
     return launch_k(kv4_attn_kernel<HD, T>, dim3((unsigned)(want < cap ? want : cap)), dim3(KA_THREADS),
                     (size_t)Cfg::SMEM, st, a, c);

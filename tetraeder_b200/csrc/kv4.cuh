@@ -100,10 +100,24 @@ __device__ __forceinline__ void kv4_store_row(__nv_bfloat16 *p, const float (&v)
                                                        kv4_pack_bf2(v[i + 4], v[i + 5]), kv4_pack_bf2(v[i + 6], v[i + 7]));
 }
 
+__device__ __forceinline__ uint32_t kv4_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    uint32_t u;
+    memcpy(&u, &h, 4);
+    return u;
+}
+// 2^e, e in [-126, 127]
+__device__ __forceinline__ float kv4_pow2(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ float kv4_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// The attention calls' scratch: 2 counters per SM (zero between calls), then the parts of split work.
+inline size_t kv4_counter_bytes(int sm_count) { return ((size_t)sm_count * 8 + 15) / 16 * 16; }
+inline float *kv4_scratch_parts(void *scratch, int sm_count) {
+    return reinterpret_cast<float *>(static_cast<char *>(scratch) + kv4_counter_bytes(sm_count));
 }
 
 // Which positions a query at position `last` sees: those up to it, of them (window > 0) the last

@@ -1556,13 +1556,18 @@ int tmoe_kv4_attn_prefill(tmoe_handle *h, void *stream, const tmoe_kv4_cache *ca
     DeviceGuard dg(h->cfg.device);
     tmoe::PdlScope pdl(!h->prof.on);  // overlap with the kernel before (programmatic launch)
     cudaError_t e = cudaSuccess;
+    if (S == 1) {
+        // a decode step of one sequence
+        e = tmoe::launch_kv4_attn(f32, cache->head_dim, x, planes, attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
+        return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "kv4 decode attention");
+    }
     if (x.k) {
         e = tmoe::launch_kv4_rows(true, f32, cache->head_dim, (void *)x.k, (void *)x.v, x.kv_ld, nullptr, seq, nullptr,
                                   pos0, S, planes, h->err, (cudaStream_t)stream);
         if (e != cudaSuccess) return cuda_fail(h, e, "kv4 store");
         x.k = x.v = nullptr;
     }
-    e = tmoe::launch_kv4_attn(f32, cache->head_dim, x, planes, attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
+    e = tmoe::launch_kv4_prefill(f32, cache->head_dim, x, planes, attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
     return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "kv4 prefill attention");
 }
 

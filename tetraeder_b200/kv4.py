@@ -32,7 +32,8 @@ class Kv4Cache:
     """Planes k_codes, v_codes uint8 [n_seq, n_kv, capacity, head_dim / 2] and k_scales, v_scales float16
     [n_seq, n_kv, capacity, head_dim / 32]; capacity is n_ctx rounded up to a multiple of 64.  `layer` (a
     MoeLayer) gives the handle whose device error flag the calls use; without one, caches of a device
-    share a small handle.  One scratch per cache: its attention calls run on one stream, or ordered ones."""
+    share a small handle.  The caches of a handle share its attention scratch: like a handle's other calls,
+    theirs run on one stream, or on ordered ones."""
 
     def __init__(self, n_seq: int, n_kv: int, head_dim: int, n_ctx: int, device: int | None = None, layer=None):
         if not torch.cuda.is_available():
@@ -77,9 +78,11 @@ class Kv4Cache:
         self.lib, self.h = self.layer.lib, self.layer.h
         self._c = _lib.Kv4CacheStruct(*(t.data_ptr() for t in planes), n_seq, n_kv, self.head_dim, cap)
         self._cp = C.addressof(self._c)
-        n = self.lib.tmoe_kv4_attn_scratch_bytes(self.h)
-        _lib.check(n if n < 0 else 0, self.h)
-        self._scratch = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        self._scratch = getattr(self.layer, "_kv4_scratch", None)
+        if self._scratch is None:
+            n = self.lib.tmoe_kv4_attn_scratch_bytes(self.h)
+            _lib.check(n if n < 0 else 0, self.h)
+            self._scratch = self.layer._kv4_scratch = torch.zeros(n, dtype=torch.uint8, device=self.device)
         self._a = _lib.Kv4AttnStruct()
         self._a.scratch = self._scratch.data_ptr()
         self._ap = C.addressof(self._a)
