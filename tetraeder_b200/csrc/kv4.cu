@@ -101,23 +101,23 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(T *__restrict__ k, T *__r
 // heads together (more are further passes over the same rows, from L2).
 //
 // Bound: HBM (a cached position is read once, 4.5 bits a value).  At that rate an SM has about 195
-// clocks for a 32-position tile of 128-wide K and V, 780 issue slots; the kernel needs about 500 of
-// them (f32 queries: 620), so the work per value has to stay small:
-//   - Codes meet the tensor cores as they are.  S = Q K^T runs on mma.sync m16n8k16 (f16 operands, f32
-//     sums) with the heads as rows: a 4-bit code under a mask is the f16 subnormal c * 2^-24 (or 16 times
-//     that), so a word of 8 codes becomes four operand registers with four ANDs and one shift.  The
-//     factor 16 is undone in Q, the -8 is the accumulator's start value -8 * sum(q), and the scale of
-//     a block multiplies its own accumulator in f32: K enters exactly.
-//   - O += P V takes V the same way, as 1024 + c minus 1032 in f16 (here the -8 has to go before the
-//     product: averaged over many positions, sum(P c) - 8 sum(P) would cancel), its scale on P.
-//   - No transposes: K's words through ldmatrix are the B operand for two steps of 16 dimensions; V's 16-bit
-//     units (4 codes) through ldmatrix.trans are, mask by mask, the B operand of four output blocks,
-//     and S's accumulators are P's A operand.
+// clocks for a 32-position tile of 128-wide K and V, 780 issue slots, so the work per value has to be
+// small:
+//   - Codes meet the tensor cores as they are, as the 16-row operand of mma.sync m16n8k16 (f16 operands, f32
+//     sums); the 8 heads are the 8 columns.  S^T = K Q^T: a 4-bit code under a mask is the f16 subnormal
+//     c * 2^-24 (or 16 times that), so a word of 8 codes becomes four operand registers with four ANDs and one
+//     shift.  The factor 16 is undone in Q.  A block's scale multiplies its own accumulator in f32: K
+//     enters exactly.  The codes' -8 is a product of its own, scales x (-8 sum of q per block), on m16n8k8.
+//   - O^T += V^T P takes V as 1024 + c minus 1032 in f16 (here the -8 has to go before the product:
+//     averaged over many positions, sum(P c) - 8 sum(P) would cancel), its scale on P.
+//   - K's words through ldmatrix are the operand of two steps of 16 dimensions; V's 16-bit units (4 codes)
+//     through ldmatrix.trans are, mask by mask, the operand's rows.  P takes one movmatrix per 8 positions.
+//   - A head's reference moves only when a score exceeds it by more than 2^8, so that no tile waits for a
+//     reduction over the warp.
 // Precision: Q is scaled by a power of two per head into f16's upper range; bf16 queries then are exact.
-// f32 queries are split as high + low f16 parts, the low ones in rows 8..15 of the operand, which the
-// 8 heads leave free; P likewise.  P times the V scale is held relative to the running maximum and the
-// largest V scale seen, so that small scales do not end in f16's subnormals; for bf16 it is one f16
-// (2^-12 relative, below the output's own 2^-9).
+// f32 queries, and P with them, are split into high + low f16 parts, in two products.  P times the V scale is
+// held relative to the reference and to the largest V scale seen, so that small scales do not end in
+// f16's subnormals; for bf16 it is f16 (2^-12 relative, below the output's own 2^-9).
 //
 // Work: the tiles of all (token, KV head, pass) are one list, cut into equal runs, one per CTA: ragged
 // lengths, few sequences or many all load every SM the same.  A warp takes every 8th tile of a run,
@@ -127,6 +127,8 @@ constexpr int KA_TILE = 32;
 constexpr int KA_WARPS = 8;
 constexpr int KA_THREADS = 32 * KA_WARPS;
 constexpr int KA_HEADS = 8;
+constexpr float KA_ROOM = 8.0f;  // how far (log2) a score may exceed its head's reference
+constexpr float KA_BIAS = 6.0f;  // P times the V scale is held below 2^(KA_BIAS + KA_ROOM)
 
 struct Kv4AttnArgs {
     const void *q, *k, *v;  // k == nullptr: the new rows are in the cache already
@@ -145,44 +147,53 @@ template <int HD, bool PREC>
 struct Kv4AttnCfg {
     static constexpr int NB = HD / 32;
     static constexpr int CODES = KA_TILE * HD / 2, SCALES = KA_TILE * NB * 2;
-    static constexpr int STAGE = 2 * (CODES + SCALES);
-    static constexpr int STAGES = (PREC ? 6 : 3) * (128 / HD);
-    static constexpr int CTAS = PREC ? 1 : 2;  // per SM
+    static constexpr int STAGE = 2 * (CODES + SCALES);  // K codes, V codes, K scales, V scales
+    static constexpr int VCODES = CODES, KSCALES = 2 * CODES, VSCALES = 2 * CODES + SCALES;
+    static constexpr int STAGES = 3 * (128 / HD);
+    static constexpr int CTAS = 2;  // per SM
     static constexpr int RING = KA_WARPS * STAGES * STAGE;
     static constexpr int SMEM = RING + KA_WARPS * STAGES * 8 + 128;
     static_assert(KA_WARPS * KA_HEADS * (HD + 2) * 4 <= RING, "the warps' sums are joined in the ring's space");
 };
 
-__device__ __forceinline__ void ka_ldsm(uint32_t addr, uint32_t (&r)[4]) {
+__device__ __forceinline__ void ka_ldsm(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
                  : "r"(addr));
 }
-__device__ __forceinline__ void ka_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+__device__ __forceinline__ void ka_ldsm_t(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
                  : "r"(addr));
 }
-// d = a b + c; without PREC rows 8..15 of a are zero and their results are dropped.
-template <bool PREC>
-__device__ __forceinline__ void ka_mma(float (&d)[PREC ? 4 : 2], const float (&c)[PREC ? 4 : 2], uint32_t a0, uint32_t a1,
-                                       uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (PREC) {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
-    } else {
-        float x, y;
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-            : "=f"(d[0]), "=f"(d[1]), "=f"(x), "=f"(y)
-            : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(0.0f), "f"(0.0f));
-    }
+__device__ __forceinline__ uint32_t ka_transpose(uint32_t u) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(u));
+    return r;
 }
-__device__ __forceinline__ float2 ka_float2(uint32_t u) {
+// d += a b
+__device__ __forceinline__ void ka_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ka_mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(b0));
+}
+__device__ __forceinline__ __half2 ka_h2(uint32_t u) {
     __half2 h;
     memcpy(&h, &u, 4);
-    return __half22float2(h);
+    return h;
 }
+__device__ __forceinline__ uint32_t ka_u(__half2 h) {
+    uint32_t u;
+    memcpy(&u, &h, 4);
+    return u;
+}
+__device__ __forceinline__ float2 ka_float2(uint32_t u) { return __half22float2(ka_h2(u)); }
 // hi = f16(a, b), lo = f16 of what that leaves
 __device__ __forceinline__ void ka_split(float a, float b, uint32_t &hi, uint32_t &lo) {
     hi = kv4_half2(a, b);
@@ -193,11 +204,7 @@ __device__ __forceinline__ void ka_split(float a, float b, uint32_t &hi, uint32_
 __device__ __forceinline__ uint32_t ka_codes(uint32_t u, uint32_t mask, __half2 off) {
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(u), "r"(mask), "r"(0x64006400u));  // (u & mask) | magic
-    __half2 h;
-    memcpy(&h, &r, 4);
-    h = __hsub2(h, off);
-    memcpy(&r, &h, 4);
-    return r;
+    return ka_u(__hsub2(ka_h2(r), off));
 }
 
 template <int HD, typename T>
@@ -205,15 +212,15 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
     kv4_attn_kernel(const Kv4AttnArgs a, const Kv4Planes c) {
     constexpr bool PREC = sizeof(T) == 4;
     using Cfg = Kv4AttnCfg<HD, PREC>;
-    constexpr int NB = Cfg::NB, AC = PREC ? 4 : 2, ST = Cfg::STAGES;
+    constexpr int NB = Cfg::NB, ST = Cfg::STAGES, RW = HD + 2;
+    constexpr uint32_t M1 = 0x000f000fu, M16 = 0x00f000f0u;
     extern __shared__ __align__(128) uint8_t ka_smem[];
     uint64_t *bars = reinterpret_cast<uint64_t *>(ka_smem + Cfg::RING);
-    __shared__ long long sh_sum[KA_WARPS];
-    __shared__ long long sh_start[2];  // token and the list position of its first tile
+    __shared__ int sh_sum[KA_WARPS];
+    __shared__ int sh_start[2];  // token and the list position of its first tile
     __shared__ int sh_last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t4 = lane & 3;
     const int G = a.n_head / c.n_kv, passes = (G + KA_HEADS - 1) / KA_HEADS, H = c.n_kv * passes;
-    uint8_t *ring = ka_smem + warp * ST * Cfg::STAGE;
     uint64_t *bar = bars + warp * ST;
     if (lane == 0)
         for (int s = 0; s < ST; s++) mbar_init(&bar[s], 1);
@@ -221,23 +228,20 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
     pdl_wait();
     pdl_trigger();
 
-    auto pos_of = [&](int t) -> int {  // -1: no query
+    auto pos_of = [&](int t) -> int {  // -1: no query, -2: a place outside the cache
         const int64_t p = a.pos ? a.pos[t] : (int64_t)a.pos0 + t;
         if (p >= c.n_ctx) return -2;
         return p < 0 ? -1 : (int)p;
     };
-    auto tiles_of = [&](int t) -> int {
-        if (t >= a.n_tok) return 0;
-        const int p = pos_of(t);
-        return p < 0 ? 0 : Kv4Seen::of<KA_TILE>(p, a.window, a.n_sink).tiles;
-    };
-    // the list: token t's tiles, H times (once per KV head and pass), t ascending.  Its length, and
-    // where this CTA's run starts
-    auto scan = [&](int base, long long &before, long long &sum) -> int {  // over 256 tokens; a CTA barrier inside
-        const int n = tiles_of(base + threadIdx.x);
-        long long inc = n;
+    // the list: token t's tiles, H times (once per KV head and pass), t ascending (below 2^31 entries, by the
+    // host's check).  Its length, and where this CTA's run starts
+    auto scan = [&](int base, int &before, int &sum) -> int {  // over 256 tokens; CTA barriers inside
+        const int t = base + threadIdx.x;
+        const int p = t < a.n_tok ? pos_of(t) : -1;
+        const int n = p < 0 ? 0 : Kv4Seen::of<KA_TILE>(p, a.window, a.n_sink).tiles;
+        int inc = n;
         for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+            const int up = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += up;
         }
         if (lane == 31) sh_sum[warp] = inc;
@@ -250,16 +254,15 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         __syncthreads();
         return n;
     };
-    long long total = 0, before = 0, sum = 0;
-    int n_mine = 0;
+    int total = 0, before = 0, sum = 0, n_mine = 0;
     for (int base = 0; base < a.n_tok; base += KA_THREADS) {
         n_mine = scan(base, before, sum);
         total += sum;
     }
     total *= H;
-    const long long even = (total + gridDim.x - 1) / gridDim.x;
-    const long long per = even > KA_WARPS ? even : KA_WARPS;  // a tile for each warp before another CTA joins in
-    const long long start = blockIdx.x * per, end = start + per < total ? start + per : total;
+    const int even = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int per = even > KA_WARPS ? even : KA_WARPS;  // a tile for each warp before another CTA joins in
+    const int start = min((int)blockIdx.x * per, total), end = min(start + per, total);
     // tokens without a query: zeros
     for (int t = blockIdx.x; t < a.n_tok; t += gridDim.x) {
         const int p = pos_of(t);
@@ -270,18 +273,28 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         for (int i = threadIdx.x; i < a.n_head * HD / 8; i += KA_THREADS) kv4_store_row(o + 8 * i, z);
     }
     if (start >= end) return;
-    long long run = 0;
+    int run = 0;
     for (int base = 0; base < a.n_tok; base += KA_THREADS) {
         if (a.n_tok > KA_THREADS) n_mine = scan(base, before, sum);
-        const long long s0 = (run + before) * H;
-        if (n_mine && s0 <= start && start < s0 + (long long)n_mine * H) sh_start[0] = base + threadIdx.x, sh_start[1] = s0;
+        const int s0 = (run + before) * H;
+        if (n_mine && s0 <= start && start < s0 + n_mine * H) sh_start[0] = base + threadIdx.x, sh_start[1] = s0;
         run += sum;
     }
     __syncthreads();
-    int tok = (int)sh_start[0];
-    long long tok0 = sh_start[1];  // list position of the token's first tile
-    long long at = start;
-    int fills = 0;  // of this warp's ring, over all parts of the run
+    int tok = sh_start[0];
+    int tok0 = sh_start[1];  // list position of the token's first tile
+    int at = start;
+    // the ring: the next stage to fill and to read, and the phase of the latter
+    int st_fill = 0, st_read = 0;
+    uint32_t phase = 0;
+    const uint32_t ring = smem_u32(ka_smem) + warp * ST * Cfg::STAGE;
+    // where a lane reads in a stage: K and V rows as ldmatrix operands, scales of rows gr (K) and 2 t4 (V)
+    uint32_t at_codes;
+    if constexpr (HD == 128)  // 8 rows, a block per 8 lanes
+        at_codes = (lane & 7) * 64 + 16 * ((lane >> 3) ^ kv4_turn<128>(lane & 7));
+    else  // 16 rows: lanes 0..15 rows 0..7 of blocks 0, 1; lanes 16..31 rows 8..15
+        at_codes = ((lane & 7) + 8 * (lane >> 4)) * 32 + 16 * (((lane >> 3) & 1) ^ kv4_turn<64>(lane & 7));
+    const __half2 off1 = __float2half2_rn(1032.0f), off16 = __float2half2_rn(1152.0f);
 
     while (at < end) {
         const int p_new = pos_of(tok);
@@ -290,36 +303,42 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             continue;
         }
         const Kv4Seen seen = Kv4Seen::of<KA_TILE>(p_new, a.window, a.n_sink);
-        const int hc = (int)((at - tok0) / seen.tiles), first = (int)((at - tok0) % seen.tiles);
-        const long long seg0 = tok0 + (long long)hc * seen.tiles;  // the list position of this head's tiles
-        const int n_part = (int)(end - at < seen.tiles - first ? end - at : seen.tiles - first);
+        const int hc = (at - tok0) / seen.tiles, first = (at - tok0) % seen.tiles;
+        const int n_part = min(end - at, seen.tiles - first);
         const int g = hc / passes, h0 = (hc % passes) * KA_HEADS;
-        const int heads = G - h0 < KA_HEADS ? G - h0 : KA_HEADS;
-        const int sq = a.seq0 >= 0 ? a.seq0 : tok;
-        const int64_t row0 = ((int64_t)sq * c.n_kv + g) * c.n_ctx;
+        const int heads = min(G - h0, KA_HEADS);
+        const int64_t row0 = ((int64_t)(a.seq0 >= 0 ? a.seq0 : tok) * c.n_kv + g) * c.n_ctx;
 
-        // ---- this warp's tiles: first + warp, first + warp + 8, ...
+        // ---- this warp's tiles: first + warp, first + warp + 8, ...  Lanes 0..3 copy a plane's piece each
         const int mine = n_part > warp ? (n_part - warp + KA_WARPS - 1) / KA_WARPS : 0;
+        const uint8_t *src;
+        uint32_t piece, dst;
+        {
+            const bool is_v = lane & 1, is_scale = lane & 2;
+            piece = is_scale ? Cfg::SCALES : Cfg::CODES;
+            dst = ring + (is_scale ? Cfg::KSCALES : 0) + (is_v ? piece : 0);
+            src = (is_scale ? reinterpret_cast<const uint8_t *>(is_v ? c.vs : c.ks) : is_v ? c.vc : c.kc) +
+                  row0 * (piece / KA_TILE);
+        }
         auto fill = [&](int j) {
-            if (lane == 0) {
-                const int s = (fills + j) % ST;
-                const int64_t r = row0 + (int64_t)seen.tile(first + warp + j * KA_WARPS) * KA_TILE;
-                uint8_t *d = ring + s * Cfg::STAGE;
-                mbar_arrive_expect_tx(&bar[s], Cfg::STAGE);
-                bulk_g2s(d, c.kc + r * (HD / 2), Cfg::CODES, &bar[s]);
-                bulk_g2s(d + Cfg::CODES, c.ks + r * NB, Cfg::SCALES, &bar[s]);
-                bulk_g2s(d + Cfg::CODES + Cfg::SCALES, c.vc + r * (HD / 2), Cfg::CODES, &bar[s]);
-                bulk_g2s(d + 2 * Cfg::CODES + Cfg::SCALES, c.vs + r * NB, Cfg::SCALES, &bar[s]);
-            }
+            uint64_t *b = &bar[st_fill];
+            if (lane == 0) mbar_arrive_expect_tx(b, Cfg::STAGE);
+            if (lane < 4)
+                asm volatile(
+                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                        dst + st_fill * Cfg::STAGE),
+                    "l"(src + (int64_t)seen.tile(first + warp + j * KA_WARPS) * piece), "r"(piece), "r"(smem_u32(b))
+                    : "memory");
+            st_fill = st_fill + 1 == ST ? 0 : st_fill + 1;
         };
         int filled = 0;
         for (; filled < mine && filled < ST; filled++) fill(filled);
 
-        // ---- Q operand: head gr of the pass; of block b the thread has dims 32 b + 8 t4 + 0..7, as
+        // ---- Q operand: column gr is head gr of the pass; of block b the thread has dims 32 b + 8 t4 + 0..7, as
         // pairs (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16, matching the codes' order in a word
         uint32_t qh[NB][4], ql[PREC ? NB : 1][4];
-        float start_acc[NB][AC];
-        float to_log2;
+        uint32_t q_sums;      // -8 * 2^-24 * sum of q of blocks 2 (t4 & 1), 2 (t4 & 1) + 1; t4 < 2 high parts, else low
+        float to_log2[2];     // of heads 2 t4, 2 t4 + 1: log2 score of an accumulator's 1
         {
             float x[NB][8];
             float top = 0.0f;
@@ -339,248 +358,268 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             const int e = top > 0.0f && top <= FLT_MAX ? 13 - ilogbf(top) : 0;
             const int e1 = e / 2, e2 = e - e1;
             const float up1 = kv4_pow2(e1), up2 = kv4_pow2(e2);
-            to_log2 = a.scale * 1.4426950408889634f * kv4_pow2(12 - e1) * kv4_pow2(12 - e2);
+            // never 0: masked scores are -inf times it
+            const float c_gr = fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(12 - e1) * kv4_pow2(12 - e2), FLT_MIN);
+            to_log2[0] = __shfl_sync(0xffffffffu, c_gr, 8 * t4);
+            to_log2[1] = __shfl_sync(0xffffffffu, c_gr, 8 * t4 + 4);
+            uint32_t sums[2] = {0, 0};  // [low]: of this lane's two blocks
+            float pair = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                float z[8], sh = 0.0f, sl = 0.0f;
+                float z[8], sq = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) z[i] = x[b][i] * up1 * up2;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
+                    const __half2 r = __float2half2_rn(i & 1 ? 0.0625f : 1.0f);
                     float2 f;
                     if constexpr (PREC) {
                         ka_split(z[i], z[i + 4], qh[b][i], ql[b][i]);
                         f = ka_float2(ql[b][i]);
-                        sl += f.x + f.y;
+                        sq += f.x + f.y;
+                        ql[b][i] = ka_u(__hmul2(ka_h2(ql[b][i]), r));
                     } else {
                         qh[b][i] = kv4_half2(z[i], z[i + 4]);
                     }
                     f = ka_float2(qh[b][i]);
-                    sh += f.x + f.y;
-                    if (i & 1) {
-                        const __half2 r = __float2half2_rn(0.0625f);
-                        __half2 h;
-                        memcpy(&h, &qh[b][i], 4);
-                        h = __hmul2(h, r);
-                        memcpy(&qh[b][i], &h, 4);
-                        if constexpr (PREC) {
-                            memcpy(&h, &ql[b][i], 4);
-                            h = __hmul2(h, r);
-                            memcpy(&ql[b][i], &h, 4);
-                        }
-                    }
+                    sq += f.x + f.y;
+                    qh[b][i] = ka_u(__hmul2(ka_h2(qh[b][i]), r));
                 }
-                sh += __shfl_xor_sync(0xffffffffu, sh, 1);
-                sh += __shfl_xor_sync(0xffffffffu, sh, 2);
-                start_acc[b][0] = start_acc[b][1] = -8.0f * 0x1p-24f * sh;
-                if constexpr (PREC) {
-                    sl += __shfl_xor_sync(0xffffffffu, sl, 1);
-                    sl += __shfl_xor_sync(0xffffffffu, sl, 2);
-                    start_acc[b][2] = start_acc[b][3] = -8.0f * 0x1p-24f * sl;
+                sq += __shfl_xor_sync(0xffffffffu, sq, 1);
+                sq += __shfl_xor_sync(0xffffffffu, sq, 2);
+                sq *= -0x1p-21f;
+                if (b & 1) {
+                    if ((t4 & 1) == b / 2) ka_split(pair, sq, sums[0], sums[1]);
+                } else {
+                    pair = sq;
                 }
             }
+            q_sums = t4 < 2 ? sums[0] : sums[1];
         }
-        float o[NB][4][AC];
+        float o[NB][2][4];  // [block][values 0, 1 or 2, 3 of 4 gr ..]: rows (value, head 2 t4 + {0, 1})
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < AC; j++) o[b][i][j] = 0.0f;
-        // of head gr: the running maximum; what exponents are taken against (the maximum, lowered by the
-        // room that P times the largest V scale leaves below 2^14); the sum, over this thread's positions
-        float top = -INFINITY, ref = -INFINITY, l = 0.0f;
-        uint32_t v_top = 0;     // the largest V scale seen, as f16 bits
-        int v_exp = 0;          // V scales are below 2^v_exp
-        const __half2 off1 = __float2half2_rn(1032.0f), off16 = __float2half2_rn(1152.0f);
+            for (int i = 0; i < 2; i++) o[b][i][0] = o[b][i][1] = o[b][i][2] = o[b][i][3] = 0.0f;
+        // of heads 2 t4 + {0, 1}: the reference, the sum over this thread's positions
+        float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        uint32_t v_top = 0;  // the largest V scale seen, as f16 bits; V scales are below 2^v_exp
+        int v_exp = 0;
         bool dead = false;
 
         for (int j = 0; j < filled; j++) {
-            const int s = (fills + j) % ST;
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bar[s], ((fills + j) / ST) & 1))) {
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bar[st_read], phase))) {
                 if (lane == 0) latch_error(a.err, TMOE_DEV_ERR_TIMEOUT);
                 dead = true;  // no more fills; the loop goes on to wait for those in flight
             }
-            uint8_t *kcodes = ring + s * Cfg::STAGE, *kscales = kcodes + Cfg::CODES, *vcodes = kscales + Cfg::SCALES,
-                    *vscales = vcodes + Cfg::CODES;
-            const int tile = seen.tile(first + warp + j * KA_WARPS), p0 = tile * KA_TILE;
-            const bool whole = seen.whole(p0, KA_TILE, a.n_sink);
+            const uint32_t stage = ring + st_read * Cfg::STAGE;
+            uint8_t *const stage_p = ka_smem + (stage - smem_u32(ka_smem));
+            st_read++;
+            if (st_read == ST) st_read = 0, phase ^= 1;
+            const int p0 = seen.tile(first + warp + j * KA_WARPS) * KA_TILE;
+            const bool whole = seen.whole(p0, KA_TILE, a.n_sink), newest = p0 + KA_TILE > p_new;
             if (!dead) {
-                if (a.k && tile == p_new / KA_TILE) {
-                    // the new row: quantised into the tile, and (one pass only) into the cache
-                    constexpr int LANES = HD / 4;
-                    const int r = p_new % KA_TILE, b = lane >> 3;
+                if (!whole || newest) {
+                    uint8_t *ks = stage_p + Cfg::KSCALES, *vs = stage_p + Cfg::VSCALES;
+                    if (a.k && newest) {
+                        // the new row: quantised into the tile, and (one pass only) into the cache
+                        constexpr int LANES = HD / 4;
+                        const int r = p_new % KA_TILE, b = lane >> 3;
+#pragma unroll 1
+                        for (int kv = 0; kv < 2; kv++) {
+                            float x[4] = {0, 0, 0, 0};
+                            if (lane < LANES)
+                                kv4_load_row(reinterpret_cast<const T *>(kv ? a.v : a.k) + (int64_t)tok * a.kv_ld +
+                                                 g * HD + 4 * lane, x);
+                            float hi = -FLT_MAX, lo = FLT_MAX;
 #pragma unroll
-                    for (int kv = 0; kv < 2; kv++) {
-                        float x[4] = {0, 0, 0, 0};
-                        if (lane < LANES)
-                            kv4_load_row(reinterpret_cast<const T *>(kv ? a.v : a.k) + (int64_t)tok * a.kv_ld + g * HD +
-                                             4 * lane, x);
-                        float hi = -FLT_MAX, lo = FLT_MAX;
+                            for (int i = 0; i < 4; i++)
+                                x[i] = kv4_finite(x[i]), hi = fmaxf(hi, x[i]), lo = fminf(lo, x[i]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) x[i] = kv4_finite(x[i]), hi = fmaxf(hi, x[i]), lo = fminf(lo, x[i]);
+                            for (int m = 1; m <= 4; m <<= 1) {
+                                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+                                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
+                            }
+                            __half d;
+                            float inv;
+                            kv4_scale(hi, lo, d, inv);
+                            uint32_t w = 0;
 #pragma unroll
-                        for (int m = 1; m <= 4; m <<= 1) {
-                            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
-                            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-                        }
-                        __half d;
-                        float inv;
-                        kv4_scale(hi, lo, d, inv);
-                        uint32_t w = 0;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) w |= kv4_code(x[i], inv) << (4 * i);
-                        if (lane < LANES) {
-                            const int byte = 16 * (b ^ kv4_turn<HD>(p_new)) + 2 * (lane & 7);
-                            uint8_t *sc = kv ? vcodes : kcodes;
-                            __half *ss = reinterpret_cast<__half *>(kv ? vscales : kscales);
-                            *reinterpret_cast<uint16_t *>(sc + r * (HD / 2) + byte) = (uint16_t)w;
-                            if ((lane & 7) == 0) ss[r * NB + b] = d;
-                            if (h0 == 0) {
-                                const int64_t row = row0 + p_new;
-                                *reinterpret_cast<uint16_t *>((kv ? c.vc : c.kc) + row * (HD / 2) + byte) = (uint16_t)w;
-                                if ((lane & 7) == 0) (kv ? c.vs : c.ks)[row * NB + b] = d;
+                            for (int i = 0; i < 4; i++) w |= kv4_code(x[i], inv) << (4 * i);
+                            if (lane < LANES) {
+                                const int byte = 16 * (b ^ kv4_turn<HD>(p_new)) + 2 * (lane & 7);
+                                *reinterpret_cast<uint16_t *>(stage_p + (kv ? Cfg::VCODES : 0) + r * (HD / 2) + byte) =
+                                    (uint16_t)w;
+                                if ((lane & 7) == 0) reinterpret_cast<__half *>(kv ? vs : ks)[r * NB + b] = d;
+                                if (h0 == 0) {
+                                    const int64_t row = row0 + p_new;
+                                    *reinterpret_cast<uint16_t *>((kv ? c.vc : c.kc) + row * (HD / 2) + byte) = (uint16_t)w;
+                                    if ((lane & 7) == 0) (kv ? c.vs : c.ks)[row * NB + b] = d;
+                                }
                             }
                         }
+                        __syncwarp();
                     }
+                    if (!seen.sees(p0 + lane, a.n_sink)) {
+                        // rows that are not seen may hold anything: their scales become zero
+#pragma unroll
+                        for (int b = 0; b < NB; b += 2) {
+                            *reinterpret_cast<uint32_t *>(ks + (lane * NB + b) * 2) = 0u;
+                            *reinterpret_cast<uint32_t *>(vs + (lane * NB + b) * 2) = 0u;
+                        }
+                    }
+                    // shared memory that a later bulk copy fills again
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
-                if (!whole && !seen.sees(p0 + lane, a.n_sink)) {
-                    // rows that are not seen may hold anything: their scales become zero
-#pragma unroll
-                    for (int b = 0; b < NB; b += 2) {
-                        *reinterpret_cast<uint32_t *>(kscales + (lane * NB + b) * 2) = 0u;
-                        *reinterpret_cast<uint32_t *>(vscales + (lane * NB + b) * 2) = 0u;
-                    }
-                }
-                // both wrote shared memory that a later bulk copy fills again
-                if (!whole || tile == p_new / KA_TILE) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
 
-                // ---- S: 8 heads x 32 positions; this thread: head gr, positions 8 nb + 2 t4 + {0, 1}
-                float sc[4][2];
-                const uint32_t k_at = smem_u32(kcodes), v_at = smem_u32(vcodes);
+                // ---- S^T: rows positions 16 hb + gr + {0, 8}, columns heads 2 t4 + {0, 1}
+                float s[2][4];
 #pragma unroll
-                for (int nb = 0; nb < 4; nb++) {
-                    uint32_t w[4];
-                    uint32_t ds[NB];  // scales of the two positions, [position][block]
+                for (int hb = 0; hb < 2; hb++) {
+                    uint32_t w0[NB], w1[NB];  // words t4 of rows gr, gr + 8
+                    uint32_t d0[NB / 2], d1[NB / 2];
+                    const uint8_t *ks = stage_p + Cfg::KSCALES + (16 * hb + gr) * NB * 2;
                     if constexpr (HD == 128) {
-                        const int r = 8 * nb + (lane & 7), b = lane >> 3;
-                        ka_ldsm(k_at + r * 64 + 16 * (b ^ kv4_turn<128>(r)), w);
-                        const uint4 d4 = *reinterpret_cast<const uint4 *>(kscales + (8 * nb + 2 * t4) * 8);
-                        ds[0] = d4.x, ds[1] = d4.y, ds[2] = d4.z, ds[3] = d4.w;
+                        ka_ldsm(stage + at_codes + hb * 1024, w0[0], w0[1], w0[2], w0[3]);
+                        ka_ldsm(stage + at_codes + hb * 1024 + 512, w1[0], w1[1], w1[2], w1[3]);
+                        const uint2 u0 = *reinterpret_cast<const uint2 *>(ks), u1 = *reinterpret_cast<const uint2 *>(ks + 64);
+                        d0[0] = u0.x, d0[1] = u0.y, d1[0] = u1.x, d1[1] = u1.y;
                     } else {
-                        const int r = 8 * nb + (lane & 7), b = (lane >> 3) & 1;  // lanes 16..31: the same again
-                        ka_ldsm(k_at + r * 32 + 16 * (b ^ kv4_turn<64>(r)), w);
-                        const uint2 d2 = *reinterpret_cast<const uint2 *>(kscales + (8 * nb + 2 * t4) * 4);
-                        ds[0] = d2.x, ds[1] = d2.y;
+                        ka_ldsm(stage + at_codes + hb * 512, w0[0], w0[1], w1[0], w1[1]);
+                        d0[0] = *reinterpret_cast<const uint32_t *>(ks), d1[0] = *reinterpret_cast<const uint32_t *>(ks + 32);
                     }
-                    float s0 = 0.0f, s1 = 0.0f;
+                    s[hb][0] = s[hb][1] = s[hb][2] = s[hb][3] = 0.0f;
+                    if constexpr (HD == 128)
+                        ka_mma8(s[hb], t4 & 1 ? d0[1] : d0[0], t4 & 1 ? d1[1] : d1[0], q_sums);
+                    else  // two blocks: lanes t4 = 0 (high) and 2 (low)
+                        ka_mma8(s[hb], t4 & 1 ? 0u : d0[0], t4 & 1 ? 0u : d1[0], q_sums);
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
-                        float acc[AC], acc2[AC];
-                        const uint32_t w8 = w[b] >> 8;
-                        constexpr uint32_t M1 = 0x000f000fu, M16 = 0x00f000f0u;
-                        ka_mma<PREC>(acc, start_acc[b], qh[b][0], PREC ? ql[PREC ? b : 0][0] : 0, qh[b][1],
-                                     PREC ? ql[PREC ? b : 0][1] : 0, w[b] & M1, w[b] & M16);
-                        ka_mma<PREC>(acc2, acc, qh[b][2], PREC ? ql[PREC ? b : 0][2] : 0, qh[b][3],
-                                     PREC ? ql[PREC ? b : 0][3] : 0, w8 & M1, w8 & M16);
-                        if constexpr (PREC) acc2[0] += acc2[AC - 2], acc2[1] += acc2[AC - 1];
-                        const float2 d0 = ka_float2(ds[b / 2]), d1 = ka_float2(ds[NB / 2 + b / 2]);
-                        s0 = fmaf(b & 1 ? d0.y : d0.x, acc2[0], s0);
-                        s1 = fmaf(b & 1 ? d1.y : d1.x, acc2[1], s1);
+                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        const uint32_t x0 = w0[b] >> 8, x1 = w1[b] >> 8;
+                        ka_mma(acc, w0[b] & M1, w1[b] & M1, w0[b] & M16, w1[b] & M16, qh[b][0], qh[b][1]);
+                        ka_mma(acc, x0 & M1, x1 & M1, x0 & M16, x1 & M16, qh[b][2], qh[b][3]);
+                        if constexpr (PREC) {
+                            ka_mma(acc, w0[b] & M1, w1[b] & M1, w0[b] & M16, w1[b] & M16, ql[b][0], ql[b][1]);
+                            ka_mma(acc, x0 & M1, x1 & M1, x0 & M16, x1 & M16, ql[b][2], ql[b][3]);
+                        }
+                        const float2 f0 = ka_float2(d0[b / 2]), f1 = ka_float2(d1[b / 2]);
+                        const float e0 = b & 1 ? f0.y : f0.x, e1 = b & 1 ? f1.y : f1.x;
+                        s[hb][0] = fmaf(e0, acc[0], s[hb][0]), s[hb][1] = fmaf(e0, acc[1], s[hb][1]);
+                        s[hb][2] = fmaf(e1, acc[2], s[hb][2]), s[hb][3] = fmaf(e1, acc[3], s[hb][3]);
                     }
-                    sc[nb][0] = s0 * to_log2, sc[nb][1] = s1 * to_log2;
                 }
                 if (!whole) {
 #pragma unroll
-                    for (int nb = 0; nb < 4; nb++)
+                    for (int hb = 0; hb < 2; hb++)
 #pragma unroll
                         for (int i = 0; i < 2; i++)
-                            if (!seen.sees(p0 + 8 * nb + 2 * t4 + i, a.n_sink)) sc[nb][i] = -INFINITY;
+                            if (!seen.sees(p0 + 16 * hb + gr + 8 * i, a.n_sink)) s[hb][2 * i] = s[hb][2 * i + 1] = -INFINITY;
                 }
-                // ---- the running maximum and the largest V scale; both seldom grow
-                float mx = sc[0][0];
-#pragma unroll
-                for (int nb = 0; nb < 4; nb++) mx = fmaxf(mx, fmaxf(sc[nb][0], sc[nb][1]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                // ---- the references and the largest V scale, which seldom grow
+                float mx[2];
+                mx[0] = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])) * to_log2[0];
+                mx[1] = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3])) * to_log2[1];
                 uint32_t dm;  // this lane's position: its largest V scale
                 if constexpr (HD == 128) {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(vscales + lane * 8);
+                    const uint2 u = *reinterpret_cast<const uint2 *>(stage_p + Cfg::VSCALES + lane * 8);
                     dm = __vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu);
                 } else {
-                    dm = *reinterpret_cast<const uint32_t *>(vscales + lane * 4) & 0x7fff7fffu;
+                    dm = *reinterpret_cast<const uint32_t *>(stage_p + Cfg::VSCALES + lane * 4) & 0x7fff7fffu;
                 }
                 dm = max(dm & 0xffffu, dm >> 16);
-                if (__any_sync(0xffffffffu, mx > top || dm > v_top)) {
-                    top = fmaxf(top, mx);
+                if (__any_sync(0xffffffffu, mx[0] > ref[0] + KA_ROOM || mx[1] > ref[1] + KA_ROOM || dm > v_top)) {
+                    float f[2];
                     v_top = max(v_top, __reduce_max_sync(0xffffffffu, dm));
-                    // f16 bits e, m: the value is below 2^(e - 14); subnormals below 2^-14
-                    v_exp = (int)(v_top >> 10) - 14;
-                    const float ref_new = top + (float)(v_exp - 14);
-                    const float f = ref == -INFINITY ? 0.0f : kv4_exp2(ref - ref_new);
-                    ref = ref_new;
-                    l *= f;
+                    const int v_old = v_exp;
+                    v_exp = (int)(v_top >> 10) - 14;  // f16 bits e, m: the value is below 2^(e - 14)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+#pragma unroll
+                        for (int m = 4; m <= 16; m <<= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], m));
+                        const float next = fmaxf(ref[i], mx[i]);
+                        f[i] = ref[i] == -INFINITY ? 0.0f : kv4_exp2(ref[i] - next);
+                        ref[i] = next;
+                        l[i] *= f[i];
+                        f[i] *= kv4_pow2(v_old - v_exp);  // O is held times 2^-v_exp
+                    }
 #pragma unroll
                     for (int b = 0; b < NB; b++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            o[b][i][0] *= f, o[b][i][1] *= f;
-                            if constexpr (PREC) o[b][i][AC - 2] *= f, o[b][i][AC - 1] *= f;
+                        for (int i = 0; i < 2; i++) {
+                            o[b][i][0] *= f[0], o[b][i][1] *= f[1];
+                            o[b][i][2] *= f[0], o[b][i][3] *= f[1];
                         }
                 }
+                // ---- P (rows positions, columns heads); f32: exact exponents, else 2^KA_BIAS at the reference
+                float nr[2];
 #pragma unroll
-                for (int nb = 0; nb < 4; nb++) {
-                    sc[nb][0] = kv4_exp2(sc[nb][0] - ref), sc[nb][1] = kv4_exp2(sc[nb][1] - ref);
-                    l += sc[nb][0] + sc[nb][1];
-                }
-                // ---- O += (P d) (c - 8), 16 positions a step
+                for (int i = 0; i < 2; i++) nr[i] = (PREC ? 0.0f : KA_BIAS) - (ref[i] == -INFINITY ? 0.0f : ref[i]);
 #pragma unroll
-                for (int ks = 0; ks < 2; ks++) {
-                    uint32_t ph[NB][2], pl[PREC ? NB : 1][2];
+                for (int hb = 0; hb < 2; hb++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int nb = 2 * ks + e;
-                        uint32_t ds[NB];
-                        if constexpr (HD == 128) {
-                            const uint4 d4 = *reinterpret_cast<const uint4 *>(vscales + (8 * nb + 2 * t4) * 8);
-                            ds[0] = d4.x, ds[1] = d4.y, ds[2] = d4.z, ds[3] = d4.w;
-                        } else {
-                            const uint2 d2 = *reinterpret_cast<const uint2 *>(vscales + (8 * nb + 2 * t4) * 4);
-                            ds[0] = d2.x, ds[1] = d2.y;
-                        }
-#pragma unroll
-                        for (int b = 0; b < NB; b++) {
-                            const float2 d0 = ka_float2(ds[b / 2]), d1 = ka_float2(ds[NB / 2 + b / 2]);
-                            const float x = sc[nb][0] * (b & 1 ? d0.y : d0.x), y = sc[nb][1] * (b & 1 ? d1.y : d1.x);
-                            if constexpr (PREC)
-                                ka_split(x, y, ph[b][e], pl[b][e]);
-                            else
-                                ph[b][e] = kv4_half2(x, y);
-                        }
+                    for (int i = 0; i < 4; i++) {
+                        s[hb][i] = kv4_exp2(fmaf(s[hb][i], to_log2[i & 1], nr[i & 1]));
+                        l[i & 1] += s[hb][i];
                     }
-                    uint32_t x0[NB], x1[NB];  // positions 0..7 and 8..15 of the step
-                    if constexpr (HD == 128) {
-                        const int r = 16 * ks + (lane & 7), b = lane >> 3;
-                        ka_ldsm_t(v_at + r * 64 + 16 * (b ^ kv4_turn<128>(r)), x0);
-                        ka_ldsm_t(v_at + (r + 8) * 64 + 16 * (b ^ kv4_turn<128>(r + 8)), x1);
+                // ---- O^T += (V^T - 8) (P d): 16 positions a step
+                const float room = kv4_pow2(-v_exp);
+                const __half2 room2 = __float2half2_rn(room);
+#pragma unroll
+                for (int hb = 0; hb < 2; hb++) {
+                    uint32_t ph[NB][2], pl[PREC ? NB : 1][2];  // positions 2 t4 + {0, 1} and + 8, column head gr
+                    if constexpr (PREC) {
+                        const uint8_t *vs = stage_p + Cfg::VSCALES + (16 * hb + gr) * NB * 2;
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const float x = s[hb][2 * i] * (room * 64.0f), y = s[hb][2 * i + 1] * (room * 64.0f);
+#pragma unroll
+                            for (int b = 0; b < NB; b += 2) {
+                                const float2 d = ka_float2(*reinterpret_cast<const uint32_t *>(vs + (8 * i * NB + b) * 2));
+                                uint32_t u, v;
+                                ka_split(x * d.x, y * d.x, u, v);
+                                ph[b][i] = ka_transpose(u), pl[b][i] = ka_transpose(v);
+                                ka_split(x * d.y, y * d.y, u, v);
+                                ph[b + 1][i] = ka_transpose(u), pl[b + 1][i] = ka_transpose(v);
+                            }
+                        }
                     } else {
-                        const int r = 16 * ks + (lane & 7) + 8 * (lane >> 4), b = (lane >> 3) & 1;
-                        uint32_t x[4];
-                        ka_ldsm_t(v_at + r * 32 + 16 * (b ^ kv4_turn<64>(r)), x);
-                        x0[0] = x[0], x0[1] = x[1], x1[0] = x[2], x1[1] = x[3];
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const __half2 p = ka_h2(ka_transpose(kv4_half2(s[hb][2 * i], s[hb][2 * i + 1])));
+                            const uint8_t *vs = stage_p + Cfg::VSCALES + (16 * hb + 8 * i + 2 * t4) * NB * 2;
+                            uint32_t d[NB];  // [position][pair of blocks]
+                            if constexpr (HD == 128) {
+                                const uint4 u = *reinterpret_cast<const uint4 *>(vs);
+                                d[0] = u.x, d[1] = u.y, d[2] = u.z, d[3] = u.w;
+                            } else {
+                                const uint2 u = *reinterpret_cast<const uint2 *>(vs);
+                                d[0] = u.x, d[1] = u.y;
+                            }
+#pragma unroll
+                            for (int b = 0; b < NB; b++) {
+                                const uint32_t dd = __byte_perm(d[b / 2], d[NB / 2 + b / 2], b & 1 ? 0x7632 : 0x5410);
+                                ph[b][i] = ka_u(__hmul2(p, __hmul2(ka_h2(dd), room2)));
+                            }
+                        }
+                    }
+                    uint32_t x0[NB], x1[NB];  // positions 2 t4 + {0, 1} and + 8, 16-bit unit gr of each block
+                    if constexpr (HD == 128) {
+                        ka_ldsm_t(stage + Cfg::VCODES + at_codes + hb * 1024, x0[0], x0[1], x0[2], x0[3]);
+                        ka_ldsm_t(stage + Cfg::VCODES + at_codes + hb * 1024 + 512, x1[0], x1[1], x1[2], x1[3]);
+                    } else {
+                        ka_ldsm_t(stage + Cfg::VCODES + at_codes + hb * 512, x0[0], x0[1], x1[0], x1[1]);
                     }
 #pragma unroll
                     for (int b = 0; b < NB; b++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {  // dims 32 b + 4 (column) + i; odd i: 16 times the value
-                            const uint32_t mask = i & 1 ? 0x00f000f0u : 0x000f000fu;
-                            const __half2 off = i & 1 ? off16 : off1;
-                            const uint32_t b0 = ka_codes(i & 2 ? x0[b] >> 8 : x0[b], mask, off);
-                            const uint32_t b1 = ka_codes(i & 2 ? x1[b] >> 8 : x1[b], mask, off);
-                            ka_mma<PREC>(o[b][i], o[b][i], ph[b][0], PREC ? pl[PREC ? b : 0][0] : 0, ph[b][1],
-                                         PREC ? pl[PREC ? b : 0][1] : 0, b0, b1);
+                        for (int i = 0; i < 2; i++) {  // rows: values 4 gr + 2 i, and 4 gr + 2 i + 1 (16 times)
+                            const uint32_t y0 = i ? x0[b] >> 8 : x0[b], y1 = i ? x1[b] >> 8 : x1[b];
+                            const uint32_t a0 = ka_codes(y0, M1, off1), a1 = ka_codes(y0, M16, off16);
+                            const uint32_t a2 = ka_codes(y1, M1, off1), a3 = ka_codes(y1, M16, off16);
+                            ka_mma(o[b][i], a0, a1, a2, a3, ph[b][0], ph[b][1]);
+                            if constexpr (PREC) ka_mma(o[b][i], a0, a1, a2, a3, pl[b][0], pl[b][1]);
                         }
                 }
             }
@@ -590,30 +629,30 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                 filled++;
             }
         }
-        fills += filled;
 
         // ---- join the warps: [warp][head][ref, l, o...]
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int m = 4; m <= 16; m <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], m);
         __syncthreads();  // the ring is idle
-        constexpr int RW = HD + 2;
         float *sums = reinterpret_cast<float *>(ka_smem);
-        {
-            float *r = sums + (warp * KA_HEADS + gr) * RW;
-            if (t4 == 0) r[0] = ref, r[1] = l;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float *r = sums + (warp * KA_HEADS + 2 * t4 + i) * RW;
+            const float f = (PREC ? 0.015625f : 1.0f) * kv4_pow2(v_exp);
+            if (gr == 0) r[0] = ref[i], r[1] = l[i];
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float x = o[b][i][e];
-                        if constexpr (PREC) x += o[b][i][AC - 2 + e];
-                        r[2 + 32 * b + 8 * t4 + 4 * e + i] = i & 1 ? x * 0.0625f : x;
-                    }
+                for (int e = 0; e < 2; e++) {
+                    *reinterpret_cast<float2 *>(r + 2 + 32 * b + 4 * gr + 2 * e) =
+                        make_float2(o[b][e][i] * f, o[b][e][2 + i] * (f * 0.0625f));
+                }
         }
         __syncthreads();
-        const long long first_cta = seg0 / per, last_cta = (seg0 + seen.tiles - 1) / per;
+        const int seg0 = tok0 + hc * seen.tiles;  // the list position of this head's tiles
+        const int first_cta = seg0 / per, last_cta = (seg0 + seen.tiles - 1) / per;
         const bool split = first_cta != last_cta;
         float *mine_out = a.part + ((int64_t)blockIdx.x * 2 + (at == start ? 0 : 1)) * KA_HEADS * RW;
         T *out = reinterpret_cast<T *>(a.out) + (int64_t)tok * a.out_ld + (int64_t)(g * G + h0) * HD;
@@ -648,7 +687,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         if (split) {
             __threadfence();
             __syncthreads();
-            const int expect = (int)(last_cta - first_cta + 1);
+            const int expect = last_cta - first_cta + 1;
             if (threadIdx.x == 0) {
                 const int n = atomicAdd(a.arrived + first_cta, 1);
                 sh_last = n == expect - 1;
@@ -663,10 +702,10 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                     const int h = i / (HD / 8), d = 8 * (i % (HD / 8));
                     float top_ref = -INFINITY;
                     for (int w = 0; w < expect; w++)
-                        top_ref = fmaxf(top_ref, __ldcg(a.part + (((first_cta + w) * 2 + (w ? 0 : slot0)) * KA_HEADS + h) * RW));
+                        top_ref = fmaxf(top_ref, __ldcg(a.part + (((int64_t)(first_cta + w) * 2 + (w ? 0 : slot0)) * KA_HEADS + h) * RW));
                     float L = 0.0f, x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
                     for (int w = 0; w < expect; w++) {
-                        const float *r = a.part + (((first_cta + w) * 2 + (w ? 0 : slot0)) * KA_HEADS + h) * RW;
+                        const float *r = a.part + (((int64_t)(first_cta + w) * 2 + (w ? 0 : slot0)) * KA_HEADS + h) * RW;
                         const float2 rl = __ldcg(reinterpret_cast<const float2 *>(r));
                         const float f = rl.y == 0.0f ? 0.0f : rl.x == -INFINITY ? 1.0f : kv4_exp2(rl.x - top_ref);
                         L += f * rl.y;
@@ -686,7 +725,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         __syncthreads();  // the sums are read; the ring may be filled again
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         at += n_part;
-        if (at == tok0 + (long long)H * seen.tiles) tok0 = at, tok++;
+        if (at == tok0 + H * seen.tiles) tok0 = at, tok++;
     }
 }
 
@@ -736,6 +775,7 @@ static cudaError_t attn_launch(Kv4Attn &x, const Kv4Planes &c, void *scratch, in
     const int G = x.n_head / c.n_kv, passes = (G + KA_HEADS - 1) / KA_HEADS;
     const int most = x.window > 0 && x.window < c.n_ctx ? x.window + 2 * KA_TILE + x.n_sink : c.n_ctx;
     const int64_t tiles = (int64_t)x.n_tok * c.n_kv * passes * (((most < c.n_ctx ? most : c.n_ctx) + KA_TILE - 1) / KA_TILE);
+    if (tiles > (1ll << 30)) return cudaErrorInvalidValue;  // list positions are 32-bit
     const int64_t want = (tiles + KA_WARPS - 1) / KA_WARPS, cap = (int64_t)Cfg::CTAS * sm_count;
     Kv4AttnArgs a;
     a.q = x.q, a.k = x.k, a.v = x.v, a.out = x.out;

@@ -181,7 +181,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 uint8_t *dst = smem + Cfg::Q + m * Cfg::TILE + (ch >> 3) * Cfg::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
                 *reinterpret_cast<uint4 *>(dst) = make_uint4(kv4_half2(x[0], x[4]), kv4_half2(x[1], x[5]),
                                                              kv4_half2(x[2], x[6]), kv4_half2(x[3], x[7]));
-                if (ch == 0) row_c[m * KP_M + r] = a.scale * 1.4426950408889634f * kv4_pow2(-e1) * kv4_pow2(-e2);
+                if (ch == 0)  // never 0: masked scores are -inf times it
+                    row_c[m * KP_M + r] = fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(-e1) * kv4_pow2(-e2), FLT_MIN);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
