@@ -120,13 +120,17 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(T *__restrict__ k, T *__r
 // f16's subnormals; for bf16 it is f16 (2^-12 relative, below the output's own 2^-9).
 //
 // Work: the tiles of all (token, KV head, pass) are one list, cut into equal runs, one per CTA: ragged
-// lengths, few sequences or many all load every SM the same.  A warp takes every 8th tile of a run,
-// fetched by bulk copies into its own ring.  Runs that end inside a token's list leave partial sums in
-// scratch; the CTA that arrives last there joins them, in run order (same sums every call).
+// lengths, few sequences or many all load every SM the same.  A segment (one token, KV head and pass)
+// costs a CTA about KA_PART tiles' time to begin and to join, so that a segment counts that much more in
+// the list; where the segments are few against the CTAs, each is instead padded to whole runs, and no
+// CTA has more than one (the cheaper of the two by its longest run).  A warp takes every 8th tile of a
+// run, fetched by bulk copies into its own ring.  Runs that hold less than a segment leave partial sums in
+// scratch; the CTA that arrives last there joins them, in run order (the same sums every call).
 constexpr int KA_TILE = 32;
 constexpr int KA_WARPS = 8;
 constexpr int KA_THREADS = 32 * KA_WARPS;
 constexpr int KA_HEADS = 8;
+constexpr int KA_PART = 16;
 constexpr float KA_ROOM = 8.0f;  // how far (log2) a score may exceed its head's reference
 constexpr float KA_BIAS = 6.0f;  // P times the V scale is held below 2^(KA_BIAS + KA_ROOM)
 
@@ -138,8 +142,8 @@ struct Kv4AttnArgs {
     int pos0, seq0;      // seq0 >= 0: every token is of that sequence; else token t of sequence t
     int n_tok, n_head, window, n_sink;
     float scale;
-    int *arrived;  // [grid] zero between calls
-    float *part;   // [2 * grid][KA_HEADS][HD + 2]
+    int *arrived;  // [grid] parts of the segment that starts in a run; zero between calls
+    float *part;   // [grid][2][KA_HEADS][HD + 2]
     int *err;
 };
 
@@ -233,13 +237,16 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         if (p >= c.n_ctx) return -2;
         return p < 0 ? -1 : (int)p;
     };
-    // the list: token t's tiles, H times (once per KV head and pass), t ascending (below 2^31 entries, by the
-    // host's check).  Its length, and where this CTA's run starts
-    auto scan = [&](int base, int &before, int &sum) -> int {  // over 256 tokens; CTA barriers inside
-        const int t = base + threadIdx.x;
+    // the list: token t's segments, H of them (KV heads times passes), t ascending; below 2^31 entries by the
+    // host's check.  A segment of n tiles takes ka_length(n, per) entries
+    auto tiles_of = [&](int t) -> int {
         const int p = t < a.n_tok ? pos_of(t) : -1;
-        const int n = p < 0 ? 0 : Kv4Seen::of<KA_TILE>(p, a.window, a.n_sink).tiles;
+        return p < 0 ? 0 : Kv4Seen::of<KA_TILE>(p, a.window, a.n_sink).tiles;
+    };
+    // over 256 tokens' values: the sum before this thread's, and of all; CTA barriers inside
+    auto scan = [&](int n, int &before, int &sum) {
         int inc = n;
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
             const int up = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += up;
@@ -252,17 +259,34 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             sum += sh_sum[w];
         }
         __syncthreads();
-        return n;
     };
-    int total = 0, before = 0, sum = 0, n_mine = 0;
+    int total = 0, live = 0, n_mine = 0;  // tiles and tokens with a query
+#pragma unroll 1
     for (int base = 0; base < a.n_tok; base += KA_THREADS) {
-        n_mine = scan(base, before, sum);
+        int before, sum;
+        n_mine = tiles_of(base + threadIdx.x);
+        scan(n_mine, before, sum);
         total += sum;
+        live += __syncthreads_count(n_mine > 0);
     }
-    total *= H;
-    const int even = (total + (int)gridDim.x - 1) / (int)gridDim.x;
-    const int per = even > KA_WARPS ? even : KA_WARPS;  // a tile for each warp before another CTA joins in
-    const int start = min((int)blockIdx.x * per, total), end = min(start + per, total);
+    total *= H, live *= H;
+    const int grid = gridDim.x;
+    // runs of whole segments' pieces, a tile a warp at least; or runs over the list as it comes
+    const int alone = live < grid ? max((total + grid - live - 1) / (grid - live), KA_WARPS) : 0x7fffffff;
+    const int across = (int)(((int64_t)total + (int64_t)live * KA_PART + grid - 1) / grid);
+    const bool pad = alone <= across;
+    const int per = max(pad ? alone : across, 1);
+    auto length = [&](int n) { return pad ? (n + per - 1) / per * per : n + KA_PART; };
+    // this thread's token (of the last 256) in the list, and the list's length
+    int before = 0, entries = 0, all = 0;
+#pragma unroll 1
+    for (int base = 0; base < a.n_tok; base += KA_THREADS) {
+        if (a.n_tok > KA_THREADS) n_mine = tiles_of(base + threadIdx.x);
+        entries = n_mine ? H * length(n_mine) : 0;
+        int sum;
+        scan(entries, before, sum);
+        all += sum;
+    }
     // tokens without a query: zeros
     for (int t = blockIdx.x; t < a.n_tok; t += gridDim.x) {
         const int p = pos_of(t);
@@ -272,18 +296,6 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         const float z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         for (int i = threadIdx.x; i < a.n_head * HD / 8; i += KA_THREADS) kv4_store_row(o + 8 * i, z);
     }
-    if (start >= end) return;
-    int run = 0;
-    for (int base = 0; base < a.n_tok; base += KA_THREADS) {
-        if (a.n_tok > KA_THREADS) n_mine = scan(base, before, sum);
-        const int s0 = (run + before) * H;
-        if (n_mine && s0 <= start && start < s0 + n_mine * H) sh_start[0] = base + threadIdx.x, sh_start[1] = s0;
-        run += sum;
-    }
-    __syncthreads();
-    int tok = sh_start[0];
-    int tok0 = sh_start[1];  // list position of the token's first tile
-    int at = start;
     // the ring: the next stage to fill and to read, and the phase of the latter
     int st_fill = 0, st_read = 0;
     uint32_t phase = 0;
@@ -296,6 +308,28 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         at_codes = ((lane & 7) + 8 * (lane >> 4)) * 32 + 16 * (((lane >> 3) & 1) ^ kv4_turn<64>(lane & 7));
     const __half2 off1 = __float2half2_rn(1032.0f), off16 = __float2half2_rn(1152.0f);
 
+    const int run = blockIdx.x, start = run * per, end = min(start + per, all);
+    // the token whose entries hold `start`
+    if (threadIdx.x == 0) sh_start[0] = -1;
+    __syncthreads();
+    if (a.n_tok <= KA_THREADS) {
+        if (before <= start && start < before + entries) sh_start[0] = threadIdx.x, sh_start[1] = before;
+    } else {
+        int done = 0;
+#pragma unroll 1
+        for (int base = 0; base < a.n_tok; base += KA_THREADS) {
+            int b4, sum;
+            const int n = tiles_of(base + threadIdx.x), len = n ? H * length(n) : 0;
+            scan(len, b4, sum);
+            b4 += done, done += sum;
+            if (b4 <= start && start < b4 + len) sh_start[0] = base + threadIdx.x, sh_start[1] = b4;
+        }
+    }
+    __syncthreads();
+    int tok = sh_start[0];
+    if (tok < 0) return;  // the list is shorter
+    int tok0 = sh_start[1];  // where the token's first segment starts
+    int at = start;
     while (at < end) {
         const int p_new = pos_of(tok);
         if (p_new < 0) {
@@ -303,11 +337,28 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             continue;
         }
         const Kv4Seen seen = Kv4Seen::of<KA_TILE>(p_new, a.window, a.n_sink);
-        const int hc = (at - tok0) / seen.tiles, first = (at - tok0) % seen.tiles;
-        const int n_part = min(end - at, seen.tiles - first);
+        const int len = length(seen.tiles), hc = (at - tok0) / len;
+        const int seg0 = tok0 + hc * len, upto = min(end, seg0 + len);
+        // the segment's tiles first .. first + n_part - 1, and whose runs hold the others
+        int first, n_part, first_run, parts;
+        if (pad) {
+            parts = len / per, first_run = seg0 / per;
+            const int i = run - first_run;
+            first = (int)((int64_t)seen.tiles * i / parts);
+            n_part = (int)((int64_t)seen.tiles * (i + 1) / parts) - first;
+        } else {
+            // its tiles are the entries from seg0 + KA_PART on
+            first = max(at - seg0 - KA_PART, 0);
+            n_part = upto - seg0 - KA_PART - first;
+            first_run = (seg0 + KA_PART) / per, parts = (seg0 + len - 1) / per - first_run + 1;
+        }
+        at = upto;
+        if (at == tok0 + H * len) tok0 = at, tok++;
+        if (n_part <= 0) continue;
+        const int t = at == tok0 ? tok - 1 : tok;
         const int g = hc / passes, h0 = (hc % passes) * KA_HEADS;
         const int heads = min(G - h0, KA_HEADS);
-        const int64_t row0 = ((int64_t)(a.seq0 >= 0 ? a.seq0 : tok) * c.n_kv + g) * c.n_ctx;
+        const int64_t row0 = ((int64_t)(a.seq0 >= 0 ? a.seq0 : t) * c.n_kv + g) * c.n_ctx;
 
         // ---- this warp's tiles: first + warp, first + warp + 8, ...  Lanes 0..3 copy a plane's piece each
         const int mine = n_part > warp ? (n_part - warp + KA_WARPS - 1) / KA_WARPS : 0;
@@ -332,6 +383,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             st_fill = st_fill + 1 == ST ? 0 : st_fill + 1;
         };
         int filled = 0;
+#pragma unroll 1
         for (; filled < mine && filled < ST; filled++) fill(filled);
 
         // ---- Q operand: column gr is head gr of the pass; of block b the thread has dims 32 b + 8 t4 + 0..7, as
@@ -347,7 +399,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[b][i] = 0.0f;
                 if (gr < heads)
-                    kv4_load_row(reinterpret_cast<const T *>(a.q) + (int64_t)tok * a.q_ld +
+                    kv4_load_row(reinterpret_cast<const T *>(a.q) + (int64_t)t * a.q_ld +
                                      (int64_t)(g * G + h0 + gr) * HD + 32 * b + 8 * t4, x[b]);
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[b][i]));
@@ -429,7 +481,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                         for (int kv = 0; kv < 2; kv++) {
                             float x[4] = {0, 0, 0, 0};
                             if (lane < LANES)
-                                kv4_load_row(reinterpret_cast<const T *>(kv ? a.v : a.k) + (int64_t)tok * a.kv_ld +
+                                kv4_load_row(reinterpret_cast<const T *>(kv ? a.v : a.k) + (int64_t)t * a.kv_ld +
                                                  g * HD + 4 * lane, x);
                             float hi = -FLT_MAX, lo = FLT_MAX;
 #pragma unroll
@@ -651,81 +703,82 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                 }
         }
         __syncthreads();
-        const int seg0 = tok0 + hc * seen.tiles;  // the list position of this head's tiles
-        const int first_cta = seg0 / per, last_cta = (seg0 + seen.tiles - 1) / per;
-        const bool split = first_cta != last_cta;
-        float *mine_out = a.part + ((int64_t)blockIdx.x * 2 + (at == start ? 0 : 1)) * KA_HEADS * RW;
-        T *out = reinterpret_cast<T *>(a.out) + (int64_t)tok * a.out_ld + (int64_t)(g * G + h0) * HD;
-        // A sum whose reference is still -inf counts only if it is not zero (a NaN, which must come out)
-        for (int i = threadIdx.x; i < heads * (HD / 8); i += KA_THREADS) {
-            const int h = i / (HD / 8), d = 8 * (i % (HD / 8));
-            float top_ref = -INFINITY;
+        const bool split = parts > 1;
+        // A run's part of a segment that started in an earlier run is in its slot 0, else in slot 1
+        float *mine_out = a.part + ((int64_t)run * 2 + (run == first_run)) * KA_HEADS * RW;
+        T *out = reinterpret_cast<T *>(a.out) + (int64_t)t * a.out_ld + (int64_t)(g * G + h0) * HD;
+        // A thread joins 4 values of a head.  A sum whose reference is still -inf counts only if it is not zero
+        // (a NaN, which must come out)
+        static_assert(KA_HEADS * HD / 4 <= KA_THREADS, "a thread each");
+        const int h = threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
+        float top_ref = -INFINITY, L = 0.0f, x[4] = {0, 0, 0, 0};
+        auto add = [&](float r, float l_, float2 y0, float2 y1, float top) {
+            if (l_ == 0.0f) return;
+            const float f = r == -INFINITY ? 1.0f : kv4_exp2(r - top);
+            L += f * l_;
+            x[0] += f * y0.x, x[1] += f * y0.y, x[2] += f * y1.x, x[3] += f * y1.y;
+        };
+        auto finish = [&]() {
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            T *p = out + h * HD + d;
+            if constexpr (PREC)
+                *reinterpret_cast<float4 *>(p) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+            else
+                *reinterpret_cast<uint2 *>(p) = make_uint2(kv4_pack_bf2(x[0] * inv, x[1] * inv), kv4_pack_bf2(x[2] * inv, x[3] * inv));
+        };
+        if (h < heads) {
 #pragma unroll
             for (int w = 0; w < KA_WARPS; w++) top_ref = fmaxf(top_ref, sums[(w * KA_HEADS + h) * RW]);
-            float L = 0.0f, x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
             for (int w = 0; w < KA_WARPS; w++) {
                 const float *r = sums + (w * KA_HEADS + h) * RW;
-                if (r[1] == 0.0f) continue;
-                const float f = r[0] == -INFINITY ? 1.0f : kv4_exp2(r[0] - top_ref);
-                L += f * r[1];
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[e] += f * r[2 + d + e];
+                add(r[0], r[1], *reinterpret_cast<const float2 *>(r + 2 + d), *reinterpret_cast<const float2 *>(r + 4 + d), top_ref);
             }
             if (split) {
-                float *r = mine_out + h * RW;
-                if (d == 0) r[0] = top_ref, r[1] = L;
-#pragma unroll
-                for (int e = 0; e < 8; e++) r[2 + d + e] = x[e];
+                float2 *r = reinterpret_cast<float2 *>(mine_out + h * RW);
+                if (d == 0) r[0] = make_float2(top_ref, L);
+                r[1 + d / 2] = make_float2(x[0], x[1]), r[2 + d / 2] = make_float2(x[2], x[3]);
             } else {
-                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[e] *= inv;
-                kv4_store_row(out + h * HD + d, x);
+                finish();
             }
         }
         if (split) {
-            __threadfence();
             __syncthreads();
-            const int expect = last_cta - first_cta + 1;
             if (threadIdx.x == 0) {
-                const int n = atomicAdd(a.arrived + first_cta, 1);
-                sh_last = n == expect - 1;
-                if (sh_last) a.arrived[first_cta] = 0;
+                int n;  // release this CTA's part, acquire the others'
+                asm volatile("fence.acq_rel.gpu; atom.add.acq_rel.gpu.s32 %0, [%1], 1;" : "=r"(n) : "l"(a.arrived + first_run) : "memory");
+                sh_last = n == parts - 1;
+                if (sh_last) a.arrived[first_run] = 0;
             }
             __syncthreads();
-            if (sh_last) {
-                __threadfence();
-                // run first_cta starts this list at its own start or later (slot 0 or 1); the others at their start
-                const int slot0 = seg0 == first_cta * per ? 0 : 1;
-                for (int i = threadIdx.x; i < heads * (HD / 8); i += KA_THREADS) {
-                    const int h = i / (HD / 8), d = 8 * (i % (HD / 8));
-                    float top_ref = -INFINITY;
-                    for (int w = 0; w < expect; w++)
-                        top_ref = fmaxf(top_ref, __ldcg(a.part + (((int64_t)(first_cta + w) * 2 + (w ? 0 : slot0)) * KA_HEADS + h) * RW));
-                    float L = 0.0f, x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                    for (int w = 0; w < expect; w++) {
-                        const float *r = a.part + (((int64_t)(first_cta + w) * 2 + (w ? 0 : slot0)) * KA_HEADS + h) * RW;
-                        const float2 rl = __ldcg(reinterpret_cast<const float2 *>(r));
-                        const float f = rl.y == 0.0f ? 0.0f : rl.x == -INFINITY ? 1.0f : kv4_exp2(rl.x - top_ref);
-                        L += f * rl.y;
+            if (sh_last && h < heads) {
+                const float *p = a.part + ((int64_t)first_run * 2 * KA_HEADS + h) * RW;
+                top_ref = -INFINITY, L = 0.0f, x[0] = x[1] = x[2] = x[3] = 0.0f;
+#pragma unroll 1
+                for (int w0 = 0; w0 < parts; w0 += 8) {
+                    float2 rl[8], y0[8], y1[8];
+                    float top = top_ref;
 #pragma unroll
-                        for (int e = 0; e < 8; e += 2) {
-                            const float2 y = __ldcg(reinterpret_cast<const float2 *>(r + 2 + d + e));
-                            x[e] += f * y.x, x[e + 1] += f * y.y;
+                    for (int w = 0; w < 8; w++) {
+                        rl[w] = make_float2(-INFINITY, 0.0f), y0[w] = y1[w] = make_float2(0.0f, 0.0f);
+                        if (w0 + w < parts) {
+                            const float2 *r = reinterpret_cast<const float2 *>(p + ((w0 + w) * 2 + (w0 + w == 0)) * (KA_HEADS * RW));
+                            rl[w] = __ldcg(r), y0[w] = __ldcg(r + 1 + d / 2), y1[w] = __ldcg(r + 2 + d / 2);
                         }
                     }
-                    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] *= inv;
-                    kv4_store_row(out + h * HD + d, x);
+                    for (int w = 0; w < 8; w++) top = fmaxf(top, rl[w].x);
+                    const float f = top_ref == -INFINITY ? 1.0f : kv4_exp2(top_ref - top);
+                    L *= f, x[0] *= f, x[1] *= f, x[2] *= f, x[3] *= f;
+                    top_ref = top;
+#pragma unroll
+                    for (int w = 0; w < 8; w++) add(rl[w].x, rl[w].y, y0[w], y1[w], top);
                 }
+                finish();
             }
         }
         __syncthreads();  // the sums are read; the ring may be filled again
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        at += n_part;
-        if (at == tok0 + H * seen.tiles) tok0 = at, tok++;
     }
 }
 
@@ -753,7 +806,7 @@ cudaError_t launch_kv4_rows(bool store, bool f32, int head_dim, void *k, void *v
 }
 
 size_t kv4_attn_scratch_bytes(int sm_count) {
-    const size_t grid = 2 * (size_t)sm_count, decode = 2 * grid * KA_HEADS * (128 + 2) * 4;
+    const size_t runs = 2 * (size_t)sm_count, decode = runs * 2 * KA_HEADS * (128 + 2) * 4;
     const size_t prefill = kv4_prefill_part_bytes(sm_count);
     return kv4_counter_bytes(sm_count) + (decode > prefill ? decode : prefill);
 }
@@ -774,9 +827,10 @@ static cudaError_t attn_launch(Kv4Attn &x, const Kv4Planes &c, void *scratch, in
     // as many CTAs as the most tiles that the cache allows need, at a tile a warp, and at most what is resident
     const int G = x.n_head / c.n_kv, passes = (G + KA_HEADS - 1) / KA_HEADS;
     const int most = x.window > 0 && x.window < c.n_ctx ? x.window + 2 * KA_TILE + x.n_sink : c.n_ctx;
-    const int64_t tiles = (int64_t)x.n_tok * c.n_kv * passes * (((most < c.n_ctx ? most : c.n_ctx) + KA_TILE - 1) / KA_TILE);
-    if (tiles > (1ll << 30)) return cudaErrorInvalidValue;  // list positions are 32-bit
-    const int64_t want = (tiles + KA_WARPS - 1) / KA_WARPS, cap = (int64_t)Cfg::CTAS * sm_count;
+    const int64_t segments = (int64_t)x.n_tok * c.n_kv * passes;
+    const int64_t tiles = segments * (((most < c.n_ctx ? most : c.n_ctx) + KA_TILE - 1) / KA_TILE);
+    if (tiles + KA_PART * segments > (1ll << 30)) return cudaErrorInvalidValue;  // list positions are 32-bit
+    const int64_t want = segments + (tiles + KA_WARPS - 1) / KA_WARPS, cap = (int64_t)Cfg::CTAS * sm_count;
     Kv4AttnArgs a;
     a.q = x.q, a.k = x.k, a.v = x.v, a.out = x.out;
     a.q_ld = x.q_ld, a.kv_ld = x.kv_ld, a.out_ld = x.out_ld;

@@ -114,7 +114,7 @@ __device__ __forceinline__ float kv4_exp2(float x) {
     return y;
 }
 
-// The attention calls' scratch: 2 counters per SM (zero between calls), then the parts of split work.
+// The attention calls' scratch: counters (zero between calls), then the parts of split work.
 inline size_t kv4_counter_bytes(int sm_count) { return ((size_t)sm_count * 8 + 15) / 16 * 16; }
 inline float *kv4_scratch_parts(void *scratch, int sm_count) {
     return reinterpret_cast<float *>(static_cast<char *>(scratch) + kv4_counter_bytes(sm_count));

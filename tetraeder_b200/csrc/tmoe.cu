@@ -147,7 +147,10 @@ struct DeviceGuard {
     bool ok = true;
     explicit DeviceGuard(int dev) {
         if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
+        if (prev != dev)
+            ok = cudaSetDevice(dev) == cudaSuccess;
+        else
+            prev = -1;  // nothing to put back
     }
     ~DeviceGuard() {
         if (prev >= 0) cudaSetDevice(prev);

@@ -17,6 +17,9 @@ import torch
 from . import _lib
 
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16}
+# the current stream's handle by device ordinal, without the Stream object where torch has the call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 _layers: dict = {}  # device ordinal -> a small handle, for caches made without one
 
 
@@ -86,12 +89,17 @@ class Kv4Cache:
         self._a = _lib.Kv4AttnStruct()
         self._a.scratch = self._scratch.data_ptr()
         self._ap = C.addressof(self._a)
+        self._dev, self._scale = self.device.index, self.head_dim ** -0.5
+        self._q_sig = self._kv_sig = None
+        self._kv_ld = 0
 
     @property
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales))
 
     # -- arguments -------------------------------------------------------------------------
+    # A serving loop makes the same calls step after step, so the checks of a call's shapes, strides and types
+    # are remembered for the last ones seen (never addresses or values).
     def _heads(self, name, t, n, dtype, n_head=None):
         """Elements from token to token of t [n, heads, head_dim] (a token's heads contiguous)."""
         hd = self.head_dim
@@ -105,7 +113,7 @@ class Kv4Cache:
         return ld if n > 1 else t.shape[1] * hd
 
     def _index(self, name, t, n):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != self.device or not t.is_contiguous():
+        if t.dtype != torch.int32 or t.shape != (n,) or t.get_device() != self._dev or (n > 1 and t.stride(0) != 1):
             raise ValueError(f"{name} is a contiguous int32 tensor [{n}] on {self.device}")
         return t.data_ptr()
 
@@ -121,24 +129,35 @@ class Kv4Cache:
         return None, -1 if seq is None else int(seq), p, pos0
 
     def _stream(self, stream):
-        return torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream.cuda_stream
+        return _raw_stream(self._dev) if stream is None else stream.cuda_stream
 
-    def _type(self, t):
+    @staticmethod
+    def _type(t):
         if t.dtype not in _TYPES:
             raise ValueError(f"activations are float32 or bfloat16, not {t.dtype}")
         return _TYPES[t.dtype]
+
+    def _kv_rows(self, k, v, n, dtype):
+        """Elements from token to token of rows k, v [n, n_kv, head_dim]."""
+        sig = (n, dtype, k.dtype, v.dtype, k.shape, v.shape, k.stride(), v.stride(), k.get_device(), v.get_device())
+        if sig != self._kv_sig:
+            ld = self._heads("k", k, n, dtype, self.n_kv)
+            if self._heads("v", v, n, dtype, self.n_kv) != ld:
+                raise ValueError("k and v rows are different distances apart")
+            self._kv_sig, self._kv_ld = sig, ld
+        return self._kv_ld
 
     # -- rows ------------------------------------------------------------------------------
     def store(self, k, v, pos, seq=None, stream=None):
         """Quantises rows k, v [n, n_kv, head_dim] into the cache: row i at position pos[i] of sequence
         seq[i] (an int: that one; None: sequence i), or at pos + i of one sequence, where pos is an int.  A negative pos[i]: no row."""
         n, ty = k.shape[0], self._type(k)
-        ld = self._heads("k", k, n, k.dtype, self.n_kv)
-        if self._heads("v", v, n, k.dtype, self.n_kv) != ld:
-            raise ValueError("k and v rows are different distances apart")
+        ld = self._kv_rows(k, v, n, k.dtype)
         s, s0, p, p0 = self._place(n, pos, seq)
-        _lib.check(self.lib.tmoe_kv4_store(self.h, self._stream(stream), self._cp, ty, k.data_ptr(), v.data_ptr(), ld,
-                                           s, s0, p, p0, n), self.h)
+        rc = self.lib.tmoe_kv4_store(self.h, self._stream(stream), self._cp, ty, k.data_ptr(), v.data_ptr(), ld,
+                                     s, s0, p, p0, n)
+        if rc:
+            _lib.check(rc, self.h)
 
     def load(self, pos, n: int | None = None, seq=None, dtype=torch.float32, stream=None):
         """The rows as values, (k, v) [n, n_kv, head_dim]: placed as in store (n: how many,
@@ -146,38 +165,41 @@ class Kv4Cache:
         n = pos.shape[0] if torch.is_tensor(pos) else n
         if n is None:
             raise ValueError("load from an int position needs n")
-        if dtype not in _TYPES:
+        ty = _TYPES.get(dtype)
+        if ty is None:
             raise ValueError(f"rows come as float32 or bfloat16, not {dtype}")
         s, s0, p, p0 = self._place(n, pos, seq)
-        k, v = torch.empty((2, n, self.n_kv, self.head_dim), dtype=dtype, device=self.device).unbind(0)
-        _lib.check(self.lib.tmoe_kv4_load(self.h, self._stream(stream), self._cp, _TYPES[dtype], k.data_ptr(),
-                                          v.data_ptr(), self.n_kv * self.head_dim, s, s0, p, p0, n), self.h)
+        k = torch.empty((n, self.n_kv, self.head_dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        rc = self.lib.tmoe_kv4_load(self.h, self._stream(stream), self._cp, ty, k.data_ptr(), v.data_ptr(),
+                                    self.n_kv * self.head_dim, s, s0, p, p0, n)
+        if rc:
+            _lib.check(rc, self.h)
         return k, v
 
     # -- attention -------------------------------------------------------------------------
     def _attn(self, q, k, v, window, n_sink, scale, out):
-        n, dt = q.shape[0], q.dtype
-        a = self._a
-        a.type = self._type(q)
-        a.q_ld = self._heads("q", q, n, dt)
-        a.n_head = n_head = q.shape[1]
+        a, n, dt = self._a, q.shape[0], q.dtype
+        sig = (dt, q.shape, q.stride(), q.get_device())
+        if sig != self._q_sig:
+            a.type = self._type(q)
+            a.q_ld, a.n_head = self._heads("q", q, n, dt), q.shape[1]
+            self._q_sig = sig
         if out is None:
-            out = torch.empty((n, n_head, self.head_dim), dtype=dt, device=self.device)
-            a.out_ld = n_head * self.head_dim
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=self.device)
+            a.out_ld = q.shape[1] * self.head_dim
         else:
-            a.out_ld = self._heads("out", out, n, dt, n_head)
-        if (k is None) != (v is None):
-            raise ValueError("k and v come together")
-        if k is None:
+            a.out_ld = self._heads("out", out, n, dt, q.shape[1])
+        if k is not None and v is not None:
+            a.kv_ld = self._kv_rows(k, v, n, dt)
+            a.k, a.v = k.data_ptr(), v.data_ptr()
+        elif k is None and v is None:
             a.k = a.v = None
         else:
-            a.kv_ld = self._heads("k", k, n, dt, self.n_kv)
-            if self._heads("v", v, n, dt, self.n_kv) != a.kv_ld:
-                raise ValueError("k and v rows are different distances apart")
-            a.k, a.v = k.data_ptr(), v.data_ptr()
+            raise ValueError("k and v come together")
         a.q, a.out = q.data_ptr(), out.data_ptr()
         a.window, a.n_sink = window, n_sink
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
+        a.scale = self._scale if scale is None else scale
         return out
 
     def decode(self, q, k, v, pos, window: int = 0, n_sink: int = 0, scale: float | None = None, out=None, stream=None):
@@ -187,8 +209,9 @@ class Kv4Cache:
         first n_sink.  Returns out [B, n_head, head_dim]."""
         out = self._attn(q, k, v, window, n_sink, scale, out)
         B = q.shape[0]
-        _lib.check(self.lib.tmoe_kv4_attn_decode(self.h, self._stream(stream), self._cp, self._ap,
-                                                 self._index("pos", pos, B), B), self.h)
+        rc = self.lib.tmoe_kv4_attn_decode(self.h, self._stream(stream), self._cp, self._ap, self._index("pos", pos, B), B)
+        if rc:
+            _lib.check(rc, self.h)
         return out
 
     def prefill(self, q, k, v, seq: int = 0, pos0: int = 0, window: int = 0, n_sink: int = 0,
@@ -197,8 +220,9 @@ class Kv4Cache:
         (None: stored already), then query i of q [S, n_head, head_dim] attends to positions 0 .. pos0 + i (or
         its window and sinks).  Returns out [S, n_head, head_dim]."""
         out = self._attn(q, k, v, window, n_sink, scale, out)
-        _lib.check(self.lib.tmoe_kv4_attn_prefill(self.h, self._stream(stream), self._cp, self._ap, seq, pos0,
-                                                  q.shape[0]), self.h)
+        rc = self.lib.tmoe_kv4_attn_prefill(self.h, self._stream(stream), self._cp, self._ap, seq, pos0, q.shape[0])
+        if rc:
+            _lib.check(rc, self.h)
         return out
 
     def check(self):
