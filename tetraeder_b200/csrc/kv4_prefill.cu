@@ -8,8 +8,8 @@
 //   P           a thread per row: exp2(S c - ref) as f16, back into TMEM over S
 //   O += P V    tcgen05, P from TMEM, V f16 in shared memory as it lies (rows are positions: an N-major
 //               operand), O f32 in TMEM
-// Warps: 0-3 and 4-7 the softmax of A and B, 8-11 dequantise, 12 issues the MMAs, 13 the bulk copies.  While
-// the softmax of one tile runs, the tensor cores work on the other.
+// Warps: 0-3 and 4-7 the softmax of A and B, 8-11 dequantise K and 12-15 V, 16 issues the MMAs, 17 the
+// bulk copies.  While the softmax of one tile runs, the tensor cores work on the other.
 //
 // Bound: per 256 rows x 128 positions of 128-wide heads the MMAs take 2048 clocks and so do the exps (16 a
 // clock and SM); the dequantisation (13 instructions for 8 values, about 475 issue slots a scheduler)
@@ -17,9 +17,9 @@
 //   - A code under a mask is 1024 + c in f16; minus 1032, times the block's scale: f16(d (c - 8)).  The pairs that
 //     fall out of a word are values (0, 4), (1, 5), (2, 6), (3, 7); Q's chunks are written in that order,
 //     and O's columns come out in it.
-//   - The running reference of a row moves only when a score exceeds it by more than 2^8: until then P is
-//     taken against the old one (below 2^14 in f16, as it starts at 2^6), and O needs no rescaling.  A
-//     tile is first tried with the old reference, S still whole in TMEM; the rare failure is redone.
+//   - The running reference of a row moves only when P against it adds up to more than 2^14 in half a tile (P is 2^6
+//     at the reference, so that no P leaves f16 before that): no maximum is taken, and O needs no rescaling.
+//     A tile is first tried with the old reference, S still whole in TMEM; the rare failure is redone.
 //   - Q is scaled per row by a power of two into f16's range.  Scales are held to what f16 can carry times 8.
 //   - Few query rows leave SMs idle, so their positions are split over CTAs, and kv4_join_kernel adds the parts.
 #include "kernels.cuh"
@@ -31,11 +31,14 @@ namespace tmoe {
 constexpr int KP_M = 128;            // rows of a tile
 constexpr int KP_ROWS = 2 * KP_M;    // of a CTA
 constexpr int KP_N = 128;            // positions of a tile
-constexpr int KP_WARPS = 14;
-constexpr int KP_THREADS = 32 * KP_WARPS;
+constexpr int KP_THREADS = 640;
+// Registers per thread: the softmax warps take what the others give back (5 * 96 at launch)
+constexpr int KP_REGS_SOFTMAX = 152, KP_REGS_DEQUANT = 64, KP_REGS_ISSUE = 48;
+static_assert(2 * KP_REGS_SOFTMAX + 2 * KP_REGS_DEQUANT + KP_REGS_ISSUE <= 5 * 96, "the block's registers");
 constexpr int KP_RAW = 3;            // raw tiles (of K or of V) in flight
-constexpr float KP_ROOM = 8.0f;      // how far (log2) a score may exceed its row's reference
 constexpr float KP_BIAS = 6.0f;      // P is 2^KP_BIAS at the reference
+constexpr float KP_MOST = 16384.0f;  // a half tile's sum of P above which the row's reference moves
+constexpr int KP_POLY = 8;           // of so many exps, two are computed in multiply-adds
 constexpr float KP_SCALE_MAX = 8188.0f;  // 8 * this is f16's largest
 
 struct Kv4PrefillArgs {
@@ -55,12 +58,14 @@ struct Kv4PrefillCfg {
     static constexpr int TILE = HALVES * HALF;
     static constexpr int CODES = KP_N * HD / 2, SCALES = KP_N * NB * 2, RAW = CODES + SCALES;
     static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, R = V + 2 * TILE, BARS = R + KP_RAW * RAW;
-    static constexpr int SMEM = BARS + 256 + KP_ROWS * 4 + 1024 /* alignment */;
+    static constexpr int SMEM = BARS + 256 + 1024 /* alignment */;
 };
 
 struct KpBars {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], raw_full[KP_RAW], raw_empty[KP_RAW], s_full[2],
-        p_full[2], o_full[2];
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], raw_empty[KP_RAW], s_full[2],
+        p_full[2][2], o_half[2], o_full[2];
+    // a slot holds K and V by turns; each of the two has its own barrier of it, so that its readers see every phase
+    uint64_t raw_full[2][KP_RAW];
     uint32_t tmem;
 };
 static_assert(sizeof(KpBars) <= 256, "barrier room");
@@ -95,6 +100,25 @@ __device__ __forceinline__ uint4 kp_word(uint32_t w, __half2 d) {
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// 2^x of a pair: by the special function unit, or in multiply-adds (its share, KP_POLY, keeps the two even):
+// x = n + f with |f| <= 1/2, and 2^f as the cubic of least relative error there (7.5e-5; P is rounded to 2^-12).
+__device__ __forceinline__ float2 kp_exp2_pair(uint64_t x) {
+    const float2 f = tc::unpair(x);
+    return make_float2(kv4_exp2(f.x), kv4_exp2(f.y));
+}
+__device__ __forceinline__ float2 kp_poly2_pair(uint64_t x) {
+    const float2 u = tc::unpair(x);
+    const uint64_t c = tc::pair(fmaxf(u.x, -120.0f), fmaxf(u.y, -120.0f));  // -inf (hidden) ends as 2^-120
+    const uint64_t n = tc::add2(c, tc::pair(12582912.0f, 12582912.0f));     // 1.5 * 2^23: the integer in the low bits
+    const uint64_t f = tc::add2(c, tc::fma2(n, tc::pair(-1.0f, -1.0f), tc::pair(12582912.0f, 12582912.0f)));
+    uint64_t p = tc::fma2(f, tc::pair(0.05517167f, 0.05517167f), tc::pair(0.24261113f, 0.24261113f));
+    p = tc::fma2(p, f, tc::pair(0.69326097f, 0.69326097f));
+    p = tc::fma2(p, f, tc::pair(0.99992806f, 0.99992806f));
+    const float2 m = tc::unpair(n), r = tc::unpair(p);
+    return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(m.x) << 23)),
+                       __int_as_float(__float_as_int(r.y) + (__float_as_int(m.y) << 23)));
+}
+
 // Bounded waits: by one thread, or by a whole warp.  One that runs out latches the error and ends the role.
 #define KP_WAIT_WARP(bar, phase)                                                            \
     do {                                                                                    \
@@ -118,7 +142,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
     extern __shared__ uint8_t kp_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(kp_raw) + 1023) & ~(uintptr_t)1023);
     KpBars &bars = *reinterpret_cast<KpBars *>(smem + Cfg::BARS);
-    float *row_c = reinterpret_cast<float *>(smem + Cfg::BARS + 256);  // [KP_ROWS] log2 score of an accumulator's 1
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // ---- which rows and which tiles; the longest runs (the last tokens) come first
@@ -138,16 +161,19 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
             mbar_init(&bars.v_full[i], 4);
             mbar_init(&bars.v_empty[i], 1);
             mbar_init(&bars.s_full[i], 1);
-            mbar_init(&bars.p_full[i], 4);
+            mbar_init(&bars.p_full[i][0], 4);
+            mbar_init(&bars.p_full[i][1], 4);
+            mbar_init(&bars.o_half[i], 1);
             mbar_init(&bars.o_full[i], 1);
         }
         for (int i = 0; i < KP_RAW; i++) {
-            mbar_init(&bars.raw_full[i], 1);
+            mbar_init(&bars.raw_full[0][i], 1);
+            mbar_init(&bars.raw_full[1][i], 1);
             mbar_init(&bars.raw_empty[i], 4);
         }
         fence_barrier_init();
     }
-    if (warp == 12) tc::alloc(&bars.tmem, 512);
+    if (warp == 16) tc::alloc(&bars.tmem, 512);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -156,40 +182,71 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
     pdl_trigger();
 
     if (warp < 8) {
+        tc::more_registers<KP_REGS_SOFTMAX>();
         // ------------------------------------------------------------ Q, then the softmax: a thread per row
         const int m = warp >> 2;
         if (m < mt) {
-            // half a warp per row, 8 values a lane
-            for (int i = 0; i < 32; i += 32 / (HD / 8)) {
-                const int r = (warp & 3) * 32 + i + lane / (HD / 8), ch = lane % (HD / 8);  // row of the tile, chunk
-                const int row = row0 + m * KP_M + r;
-                float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (row < rows)
-                    kv4_load_row(reinterpret_cast<const T *>(a.q) + (int64_t)(row / G) * a.q_ld +
-                                     (int64_t)(g * G + row % G) * HD + 8 * ch, x);
-                float top = 0.0f;
+            // The warp's 32 rows into the operand's layout, a thread per row: bf16 by asynchronous copies, all in flight,
+            // and then in place; f32 read twice.  Loops stay rolled: their code is fetched anew by every CTA.
+            uint8_t *q_tile = smem + Cfg::Q + m * Cfg::TILE;
+            auto chunk = [&](int r, int ch) { return q_tile + (ch >> 3) * Cfg::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
+            const int my_r = (warp & 3) * 32 + lane, my_row = min(row0 + m * KP_M + my_r, rows - 1);
+            const T *my_q = reinterpret_cast<const T *>(a.q) + (int64_t)(my_row / G) * a.q_ld + (int64_t)(g * G + my_row % G) * HD;
+            constexpr int CH = HD / 8;
+            float top = 0.0f;
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll 4
+                for (int i = 0; i < 32; i += 32 / CH) {
+                    const int src = i + lane / CH, ch = lane % CH;
+                    const T *p = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, (unsigned long long)my_q, src)) + 8 * ch;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(chunk((warp & 3) * 32 + src, ch))), "l"(p)
+                                 : "memory");
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                __syncwarp();
+#pragma unroll 2
+                for (int ch = 0; ch < CH; ch++) {
+                    const uint4 u = *reinterpret_cast<const uint4 *>(chunk(my_r, ch));
+                    // magnitudes of bf16 order as their bits
+                    const uint32_t h = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu),
+                                                __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
+                    top = fmaxf(top, fmaxf(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)));
+                }
+            } else {
+#pragma unroll 2
+                for (int ch = 0; ch < CH; ch++) {
+                    float x[8];
+                    kv4_load_row(my_q + 8 * ch, x);
 #pragma unroll
-                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
-#pragma unroll
-                for (int o = HD / 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                // 2^e * top in [2^5, 2^6): exact for bf16 values down to 2^-22 of the largest
-                const int e = top > 0.0f && top <= FLT_MAX ? 5 - ilogbf(top) : 0;
-                const int e1 = e / 2, e2 = e - e1;
-                const float up1 = kv4_pow2(e1), up2 = kv4_pow2(e2);
-#pragma unroll
-                for (int i2 = 0; i2 < 8; i2++) x[i2] = x[i2] * up1 * up2;
-                uint8_t *dst = smem + Cfg::Q + m * Cfg::TILE + (ch >> 3) * Cfg::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-                *reinterpret_cast<uint4 *>(dst) = make_uint4(kv4_half2(x[0], x[4]), kv4_half2(x[1], x[5]),
-                                                             kv4_half2(x[2], x[6]), kv4_half2(x[3], x[7]));
-                if (ch == 0)  // never 0: masked scores are -inf times it
-                    row_c[m * KP_M + r] = fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(-e1) * kv4_pow2(-e2), FLT_MIN);
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
+                }
             }
+            // 2^e * top in [2^5, 2^6): exact for bf16 values down to 2^-22 of the largest
+            const int e = top > 0.0f && top <= FLT_MAX ? 5 - ilogbf(top) : 0;
+            const int e1 = e / 2, e2 = e - e1;
+            const float up1 = kv4_pow2(e1), up2 = kv4_pow2(e2);
+#pragma unroll 2
+            for (int ch = 0; ch < CH; ch++) {
+                uint4 *dst = reinterpret_cast<uint4 *>(chunk(my_r, ch));
+                float x[8];
+                if constexpr (sizeof(T) == 2) {
+                    const uint4 u = *dst;
+                    kv4_bf2(u.x, x[0], x[1]), kv4_bf2(u.y, x[2], x[3]), kv4_bf2(u.z, x[4], x[5]), kv4_bf2(u.w, x[6], x[7]);
+                } else {
+                    kv4_load_row(my_q + 8 * ch, x);
+                }
+#pragma unroll
+                for (int v = 0; v < 8; v++) x[v] = x[v] * up1 * up2;
+                *dst = make_uint4(kv4_half2(x[0], x[4]), kv4_half2(x[1], x[5]), kv4_half2(x[2], x[6]), kv4_half2(x[3], x[7]));
+            }
+            // log2 score of an accumulator's 1; never 0: masked scores are -inf times it
+            const float cs = fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(-e1) * kv4_pow2(-e2), FLT_MIN);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.q_full);
 
-            const int r = (warp & 3) * 32 + lane, row = row0 + m * KP_M + r;
-            const float cs = row_c[m * KP_M + r];
+            const int r = my_r, row = row0 + m * KP_M + r;
             const int t = a.pos0 + min(row, rows - 1) / G;  // the row's position
             const int t_lo = a.pos0 + (row0 + m * KP_M) / G, t_hi = a.pos0 + min(row0 + (m + 1) * KP_M - 1, rows - 1) / G;
             const int w_lo = a.window > 0 ? t - a.window : -1;  // positions above it are in the window
@@ -200,63 +257,93 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 KP_WAIT_WARP(bars.s_full[m], j & 1);
                 tc::fence_after();
                 const int p0 = seen.tile(tile0 + j) * KP_N;
-                const bool whole = p0 + KP_N - 1 <= t_lo && (a.window == 0 || p0 > t_hi - a.window || p0 + KP_N <= a.n_sink);
-                // P against `ref`, the largest score (scaled), the sum
-                uint32_t p[KP_N / 2];
-                auto attempt = [&](float neg_ref, float &mx, float &sum) {
-                    mx = -INFINITY, sum = 0.0f;
-                    float sum2 = 0.0f;
+                // In halves of 64 positions, so that the first one's product runs beside the second's exps
+#pragma unroll 1
+                for (int hf = 0; hf < 2; hf++) {
+                    const int ph = p0 + 64 * hf;
+                    const bool whole = ph + 63 <= t_lo && (a.window == 0 || ph > t_hi - a.window || ph + 64 <= a.n_sink);
+                    const uint32_t th = ts + 64 * hf;
+                    auto hide = [&](uint32_t (&s)[32], int ch) {
+                        if (whole) return;
 #pragma unroll
-                    for (int ch = 0; ch < KP_N; ch += 32) {
-                        uint32_t s[32];
-                        tc::ld32(ts + ch, s);
-                        tc::wait_ld();
-                        if (!whole) {
+                        for (int i = 0; i < 32; i++) {
+                            const int k = ph + ch + i;
+                            if (k > t || (k <= w_lo && k >= a.n_sink)) s[i] = 0xff800000u;  // -inf
+                        }
+                    };
+                    // P against a reference, and its sum
+                    uint32_t p[32];
+                    auto attempt = [&](float neg_ref) -> float {
+                        const uint64_t c2 = tc::pair(cs, cs), r2 = tc::pair(neg_ref, neg_ref);
+                        uint64_t sum0 = 0, sum1 = 0;
+                        auto part = [&](uint32_t (&s)[32], int ch) {
+                            hide(s, ch);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) {
-                                const int k = p0 + ch + i;
-                                if (k > t || (k <= w_lo && k >= a.n_sink)) s[i] = 0xff800000u;  // -inf
+                            for (int i = 0; i < 32; i += 4) {
+                                const uint64_t x = tc::fma2(tc::pair(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, r2);
+                                const uint64_t y = tc::fma2(tc::pair(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), c2, r2);
+                                const float2 e = kp_exp2_pair(x), f = i % KP_POLY == 0 ? kp_poly2_pair(y) : kp_exp2_pair(y);
+                                sum0 = tc::add2(sum0, tc::pair(e.x, e.y)), sum1 = tc::add2(sum1, tc::pair(f.x, f.y));
+                                p[(ch + i) / 2] = kv4_half2(e.x, e.y), p[(ch + i) / 2 + 1] = kv4_half2(f.x, f.y);
+                            }
+                        };
+                        uint32_t s0[32], s1[32];
+                        tc::ld32(th, s0);
+                        tc::wait_ld(s0);
+                        tc::ld32(th + 32, s1);
+                        part(s0, 0);
+                        tc::wait_ld(s1);
+                        part(s1, 32);
+                        const float2 x = tc::unpair(tc::add2(sum0, sum1));
+                        return x.x + x.y;
+                    };
+                    float sum = 0.0f;
+                    bool raise = __any_sync(0xffffffffu, ref == -INFINITY);
+#pragma unroll 1
+                    for (int tries = 0; tries < 2; tries++) {
+                        if (raise) {
+                            tries = 1;
+                            float mx = -INFINITY;
+#pragma unroll 1
+                            for (int ch = 0; ch < 64; ch += 32) {
+                                uint32_t s[32];
+                                tc::ld32(th + ch, s);
+                                tc::wait_ld(s);
+                                hide(s, ch);
+#pragma unroll
+                                for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(s[i]));
+                            }
+                            const float next = fmaxf(ref, mx * cs);
+                            const float f = ref == -INFINITY ? 0.0f : kv4_exp2(ref - next);
+                            ref = next;
+                            l *= f;
+                            if (hf) {  // the first half's product has to be in O
+                                KP_WAIT_WARP(bars.o_half[m], j & 1);
+                                tc::fence_after();
+                            }
+                            if (j > 0 || hf) {
+#pragma unroll 1
+                                for (int ch = 0; ch < HD; ch += 32) {
+                                    uint32_t o[32];
+                                    tc::ld32(to + ch, o);
+                                    tc::wait_ld(o);
+#pragma unroll
+                                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                    tc::st32(to + ch, o);
+                                }
                             }
                         }
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float s0 = __uint_as_float(s[i]), s1 = __uint_as_float(s[i + 1]);
-                            mx = fmaxf(mx, fmaxf(s0, s1));
-                            const float e0 = kv4_exp2(fmaf(s0, cs, neg_ref)), e1 = kv4_exp2(fmaf(s1, cs, neg_ref));
-                            sum += e0, sum2 += e1;
-                            p[(ch + i) / 2] = kv4_half2(e0, e1);
-                        }
+                        sum = attempt(KP_BIAS - (ref == -INFINITY ? 0.0f : ref));
+                        raise = __any_sync(0xffffffffu, sum > KP_MOST);
+                        if (!raise) break;
                     }
-                    mx *= cs;
-                    sum += sum2;
-                };
-                float mx, sum;
-                attempt(KP_BIAS - (ref == -INFINITY ? 0.0f : ref), mx, sum);
-                if (__any_sync(0xffffffffu, mx > ref + KP_ROOM || (mx > -INFINITY && ref == -INFINITY))) {
-                    const float next = fmaxf(ref, mx);
-                    const float f = ref == -INFINITY ? 0.0f : kv4_exp2(ref - next);
-                    ref = next;
-                    l *= f;
-                    if (j > 0) {
-#pragma unroll 1
-                        for (int ch = 0; ch < HD; ch += 32) {
-                            uint32_t o[32];
-                            tc::ld32(to + ch, o);
-                            tc::wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tc::st32(to + ch, o);
-                        }
-                    }
-                    attempt(KP_BIAS - (ref == -INFINITY ? 0.0f : ref), mx, sum);
+                    l += sum;
+                    tc::st32(th, p);
+                    tc::wait_st();
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.p_full[m][hf]);
                 }
-                l += sum;
-                tc::st32(ts, p);
-                tc::st32(ts + 32, p + 32);
-                tc::wait_st();
-                tc::fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.p_full[m]);
             }
             // ---- the rows' results
             float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -274,7 +361,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 for (int ch = 0; ch < HD; ch += 32) {
                     uint32_t o[32];
                     tc::ld32(to + ch, o);
-                    tc::wait_ld();
+                    tc::wait_ld(o);
                     if (row < rows) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {
@@ -295,15 +382,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 }
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
+        tc::fewer_registers<KP_REGS_DEQUANT>();
         // ------------------------------------------------------------ dequantise: a thread per position
-        const int r = threadIdx.x - 256;
+        const int r = threadIdx.x & 127;
+        const bool is_v = warp >= 12;
         const __half2 cap = __float2half2_rn(KP_SCALE_MAX), ncap = __float2half2_rn(-KP_SCALE_MAX);
-        for (int i = 0; i < 2 * n; i++) {
-            const int j = i >> 1, slot = j & 1, rs = i % KP_RAW;
-            const bool is_v = i & 1;
+        for (int j = 0; j < n; j++) {
+            const int i = 2 * j + is_v, slot = j & 1, rs = i % KP_RAW;
             uint8_t *dst = smem + (is_v ? Cfg::V : Cfg::K) + slot * Cfg::TILE;
-            KP_WAIT_WARP(bars.raw_full[rs], (i / KP_RAW) & 1);
+            KP_WAIT_WARP(bars.raw_full[is_v][rs], (j / KP_RAW) & 1);
             if (j >= 2) KP_WAIT_WARP(is_v ? bars.v_empty[slot] : bars.k_empty[slot], ((j >> 1) - 1) & 1);
             const uint8_t *raw = smem + Cfg::R + rs * Cfg::RAW;
             const int pos = seen.tile(tile0 + j) * KP_N + r;
@@ -337,50 +425,65 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 mbar_arrive(is_v ? &bars.v_full[slot] : &bars.k_full[slot]);
             }
         }
-    } else if (warp == 12) {
-        // ------------------------------------------------------------ the MMAs
-        if (lane == 0 && n > 0) {
-            constexpr uint32_t id_qk = tc::idesc(KP_M, KP_N, false), id_pv = tc::idesc(KP_M, HD, true);
-            const uint32_t q_at = smem_u32(smem + Cfg::Q), k_at = smem_u32(smem + Cfg::K), v_at = smem_u32(smem + Cfg::V);
-            auto qk = [&](int m, int j) {
+    } else {
+        tc::fewer_registers<KP_REGS_ISSUE>();
+        if (warp == 16) {
+            // -------------------------------------------------------- the MMAs
+            if (n > 0) {
+                constexpr uint32_t id_qk = tc::idesc(KP_M, KP_N, false), id_pv = tc::idesc(KP_M, HD, true);
+                const uint32_t q_lo = tc::desc_lo(smem_u32(smem + Cfg::Q), 16), k_lo = tc::desc_lo(smem_u32(smem + Cfg::K), 16),
+                               v_lo = tc::desc_lo(smem_u32(smem + Cfg::V), Cfg::HALF);
+                auto qk = [&](int m, int j) {
+                    const uint32_t a_lo = q_lo + m * (Cfg::TILE >> 4), b_lo = k_lo + (j & 1) * (Cfg::TILE >> 4);
+                    if (tc::elect()) {
 #pragma unroll
-                for (int k = 0; k < HD / 16; k++) {
-                    const uint32_t off = (k >> 2) * Cfg::HALF + (k & 3) * 32;
-                    tc::mma_ss(tmem + m * KP_N, tc::desc_kmajor(q_at + m * Cfg::TILE + off),
-                               tc::desc_kmajor(k_at + (j & 1) * Cfg::TILE + off), id_qk, k > 0);
-                }
-                tc::commit(&bars.s_full[m]);
-            };
-            auto pv = [&](int m, int j) {
+                        for (int k = 0; k < HD / 16; k++) {
+                            const uint32_t off = ((k >> 2) * Cfg::HALF + (k & 3) * 32) >> 4;
+                            tc::mma_ss(tmem + m * KP_N, a_lo + off, tc::DESC_HI, b_lo + off, tc::DESC_HI, id_qk, k > 0);
+                        }
+                        tc::commit(&bars.s_full[m]);
+                    }
+                    __syncwarp();
+                };
+                auto pv = [&](int m, int j, int hf) {
+                    const uint32_t b_lo = v_lo + (j & 1) * (Cfg::TILE >> 4) + hf * (64 * 128 >> 4);
+                    if (tc::elect()) {
 #pragma unroll
-                for (int k = 0; k < KP_N / 16; k++)
-                    tc::mma_ts(tmem + 256 + m * HD, tmem + m * KP_N + 8 * k,
-                               tc::desc_mnmajor(v_at + (j & 1) * Cfg::TILE + k * 2048, Cfg::HALF), id_pv, (j | k) > 0);
-            };
-            KP_WAIT(bars.q_full, 0);
-            KP_WAIT(bars.k_full[0], 0);
-            tc::fence_after();
-            for (int m = 0; m < mt; m++) qk(m, 0);
-            tc::commit(&bars.k_empty[0]);
-            for (int j = 0; j < n; j++) {
-                KP_WAIT(bars.v_full[j & 1], (j >> 1) & 1);
-                for (int m = 0; m < mt; m++) {
-                    KP_WAIT(bars.p_full[m], j & 1);
-                    tc::fence_after();
-                    pv(m, j);
-                    if (m == mt - 1) tc::commit(&bars.v_empty[j & 1]);
-                    if (j + 1 == n) {
-                        tc::commit(&bars.o_full[m]);
-                    } else {
-                        if (m == 0) KP_WAIT(bars.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
-                        tc::fence_after();
-                        qk(m, j + 1);
-                        if (m == mt - 1) tc::commit(&bars.k_empty[(j + 1) & 1]);
+                        for (int k = 0; k < 4; k++)
+                            tc::mma_ts(tmem + 256 + m * HD, tmem + m * KP_N + 64 * hf + 8 * k, b_lo + k * (2048 >> 4), tc::DESC_HI,
+                                       id_pv, k > 0 ? 1 : j | hf);
+                        if (hf == 0) {
+                            tc::commit(&bars.o_half[m]);
+                        } else {
+                            if (m == mt - 1) tc::commit(&bars.v_empty[j & 1]);
+                            if (j + 1 == n) tc::commit(&bars.o_full[m]);
+                        }
+                    }
+                    __syncwarp();
+                };
+                KP_WAIT_WARP(bars.q_full, 0);
+                KP_WAIT_WARP(bars.k_full[0], 0);
+                tc::fence_after();
+                for (int m = 0; m < mt; m++) qk(m, 0);
+                if (tc::elect()) tc::commit(&bars.k_empty[0]);
+                for (int j = 0; j < n; j++) {
+                    KP_WAIT_WARP(bars.v_full[j & 1], (j >> 1) & 1);
+                    for (int m = 0; m < mt; m++) {
+                        for (int hf = 0; hf < 2; hf++) {
+                            KP_WAIT_WARP(bars.p_full[m][hf], j & 1);
+                            tc::fence_after();
+                            pv(m, j, hf);
+                        }
+                        if (j + 1 < n) {
+                            if (m == 0) KP_WAIT_WARP(bars.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
+                            tc::fence_after();
+                            qk(m, j + 1);
+                            if (m == mt - 1 && tc::elect()) tc::commit(&bars.k_empty[(j + 1) & 1]);
+                        }
                     }
                 }
             }
-        }
-    } else {
+        } else if (warp == 17) {
         // ------------------------------------------------------------ raw tiles by bulk copies
         if (lane == 0) {
             const int64_t head = ((int64_t)a.seq * c.n_kv + g) * c.n_ctx;
@@ -390,18 +493,20 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 const int p0 = seen.tile(tile0 + (i >> 1)) * KP_N;
                 const int np = min(KP_N, c.n_ctx - p0);  // the cache may end inside the last tile (at 64)
                 uint8_t *dst = smem + Cfg::R + rs * Cfg::RAW;
-                mbar_arrive_expect_tx(&bars.raw_full[rs], (uint32_t)(np * (HD / 2 + NB * 2)));
-                bulk_g2s(dst, (i & 1 ? c.vc : c.kc) + (head + p0) * (HD / 2), (uint32_t)(np * (HD / 2)), &bars.raw_full[rs]);
+                uint64_t *full = &bars.raw_full[i & 1][rs];
+                mbar_arrive_expect_tx(full, (uint32_t)(np * (HD / 2 + NB * 2)));
+                bulk_g2s(dst, (i & 1 ? c.vc : c.kc) + (head + p0) * (HD / 2), (uint32_t)(np * (HD / 2)), full);
                 bulk_g2s(dst + Cfg::CODES, (i & 1 ? c.vs : c.ks) + (head + p0) * NB, (uint32_t)(np * NB * 2),
-                         &bars.raw_full[rs]);
+                         full);
             }
+        }
         }
     }
 done:
     __syncwarp();
     tc::fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         tc::fence_after();
         tc::dealloc(tmem, 512);
     }

@@ -16,17 +16,28 @@ __device__ __forceinline__ void alloc(uint32_t *dst, uint32_t ncols) {
 __device__ __forceinline__ void dealloc(uint32_t taddr, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
-// d (TMEM, f32) (+)= A B with f16 operands: A and B in shared memory, or A in TMEM
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// One lane of a whole warp.  The MMAs and commits below are issued by it from code that the warp runs
+// together, so that their operands stay in uniform registers.
+__device__ __forceinline__ bool elect() {
+    uint32_t one;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+    return one != 0;
+}
+// d (TMEM, f32) (+)= A B with f16 operands: A and B in shared memory, or A in TMEM.  Descriptors by halves:
+// only the low one holds the address.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                       uint32_t add) {
     asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "{ .reg .pred p; .reg .b64 a, b; setp.ne.b32 p, %6, 0; mov.b64 a, {%1, %2}; mov.b64 b, {%3, %4}; "
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p; }" ::"r"(d),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(add)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t add) {
     asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "{ .reg .pred p; .reg .b64 b; setp.ne.b32 p, %5, 0; mov.b64 b, {%2, %3}; "
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p; }" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(add)
         : "memory");
 }
 // Arrives on `bar` once every MMA that this thread issued before has completed.
@@ -36,7 +47,6 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 #define TMOE_R32(r) \
@@ -54,6 +64,32 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {
         : "memory");
 }
 #undef TMOE_R32
+__device__ __forceinline__ void ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+// Until every load of this thread has landed.  The registers pass through, so that no use moves above it.
+#define TMOE_W32(r) \
+    "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), \
+        "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), \
+        "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), \
+        "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : TMOE_W32(r)::"memory");
+}
+#undef TMOE_W32
 __device__ __forceinline__ void st32(uint32_t taddr, const uint32_t *r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -67,21 +103,47 @@ __device__ __forceinline__ void st32(uint32_t taddr, const uint32_t *r) {
 
 // Shared-memory descriptors in the 128-byte swizzle: rows of 128 bytes (64 f16), 16-byte chunk c of row r
 // at chunk c ^ (r & 7), groups of 8 rows 1024 bytes apart.
-//   kmajor   the rows are M (or N), the reduction runs along the 128 bytes
-//   mnmajor  the rows are the reduction, N runs along the 128 bytes; further blocks of 64 N `lead` bytes on
-__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lead) {
-    uint64_t d = (uint64_t)((saddr & 0x3ffffu) >> 4);
-    d |= (uint64_t)(lead >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;  // 8-row groups
-    d |= (uint64_t)1 << 46;            // descriptor version of sm_100
-    d |= (uint64_t)2 << 61;            // 128-byte swizzle
-    return d;
+//   K-major   the rows are M (or N), the reduction runs along the 128 bytes (lead 16)
+//   N-major   the rows are the reduction, N runs along the 128 bytes; further blocks of 64 N `lead` bytes on
+// Low half: address / 16 and lead / 16.  High half: stride 1024 / 16, the version of sm_100, 128-byte swizzle.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lead) {
+    return ((saddr & 0x3ffffu) >> 4) | (lead >> 4) << 16;
 }
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t saddr) { return desc(saddr, 16); }
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t saddr, uint32_t lead) { return desc(saddr, lead); }
+constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
 // Instruction descriptor of kind::f16: f16 A (K-major) and B, f32 D, M x N
 __host__ __device__ constexpr uint32_t idesc(int M, int N, bool b_mnmajor) {
     return (1u << 4) | ((b_mnmajor ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// Registers per thread of this warpgroup from here on
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// Pairs of floats in one instruction
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 }  // namespace tc
