@@ -38,7 +38,6 @@ static_assert(2 * KP_REGS_SOFTMAX + 2 * KP_REGS_DEQUANT + KP_REGS_ISSUE <= 5 * 9
 constexpr int KP_RAW = 3;            // raw tiles (of K or of V) in flight
 constexpr float KP_BIAS = 6.0f;      // P is 2^KP_BIAS at the reference
 constexpr float KP_MOST = 16384.0f;  // a half tile's sum of P above which the row's reference moves
-constexpr int KP_POLY = 8;           // of so many exps, two are computed in multiply-adds
 constexpr float KP_SCALE_MAX = 8188.0f;  // 8 * this is f16's largest
 
 struct Kv4PrefillArgs {
@@ -47,7 +46,7 @@ struct Kv4PrefillArgs {
     int64_t q_ld, out_ld;
     int seq, pos0, n_tok, n_head, window, n_sink, splits;
     float scale;
-    float *part;  // splits > 1: [cta][KP_ROWS][HD + 2]
+    float *part;  // splits > 1: [cta] of O as [HD / 4][KP_ROWS][4], then the references and sums as [2][KP_ROWS]
     int *err;
 };
 
@@ -100,24 +99,18 @@ __device__ __forceinline__ uint4 kp_word(uint32_t w, __half2 d) {
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// 2^x of a pair: by the special function unit, or in multiply-adds (its share, KP_POLY, keeps the two even):
-// x = n + f with |f| <= 1/2, and 2^f as the cubic of least relative error there (7.5e-5; P is rounded to 2^-12).
+// 2^x of a pair
 __device__ __forceinline__ float2 kp_exp2_pair(uint64_t x) {
     const float2 f = tc::unpair(x);
     return make_float2(kv4_exp2(f.x), kv4_exp2(f.y));
 }
-__device__ __forceinline__ float2 kp_poly2_pair(uint64_t x) {
-    const float2 u = tc::unpair(x);
-    const uint64_t c = tc::pair(fmaxf(u.x, -120.0f), fmaxf(u.y, -120.0f));  // -inf (hidden) ends as 2^-120
-    const uint64_t n = tc::add2(c, tc::pair(12582912.0f, 12582912.0f));     // 1.5 * 2^23: the integer in the low bits
-    const uint64_t f = tc::add2(c, tc::fma2(n, tc::pair(-1.0f, -1.0f), tc::pair(12582912.0f, 12582912.0f)));
-    uint64_t p = tc::fma2(f, tc::pair(0.05517167f, 0.05517167f), tc::pair(0.24261113f, 0.24261113f));
-    p = tc::fma2(p, f, tc::pair(0.69326097f, 0.69326097f));
-    p = tc::fma2(p, f, tc::pair(0.99992806f, 0.99992806f));
-    const float2 m = tc::unpair(n), r = tc::unpair(p);
-    return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(m.x) << 23)),
-                       __int_as_float(__float_as_int(r.y) + (__float_as_int(m.y) << 23)));
-}
+
+struct KpYes {
+    static constexpr bool value = true;
+};
+struct KpNo {
+    static constexpr bool value = false;
+};
 
 // Bounded waits: by one thread, or by a whole warp.  One that runs out latches the error and ends the role.
 #define KP_WAIT_WARP(bar, phase)                                                            \
@@ -253,51 +246,48 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t ts = tmem + m * KP_N + lanes, to = tmem + 256 + m * HD + lanes;
             float ref = -INFINITY, l = 0.0f;
+            // P of 32 columns of S against a reference (exponents s c + r), and its sum; positions from k0 on
+            auto exps = [&](const uint32_t (&s)[32], uint32_t *p, uint64_t c2, uint64_t r2, uint64_t (&sum)[2], int k0, auto masked) {
+                // by stages over all 32: a group at a time would wait for each result
+                uint64_t x[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    uint32_t v[2] = {s[2 * i], s[2 * i + 1]};
+                    if constexpr (decltype(masked)::value) {
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const int k = k0 + 2 * i + u;
+                            if (k > t || (k <= w_lo && k >= a.n_sink)) v[u] = 0xff800000u;  // -inf
+                        }
+                    }
+                    x[i] = tc::fma2(tc::pair(__uint_as_float(v[0]), __uint_as_float(v[1])), c2, r2);
+                }
+                float2 e[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) e[i] = kp_exp2_pair(x[i]);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    sum[i & 1] = tc::add2(sum[i & 1], tc::pair(e[i].x, e[i].y));
+                    p[i] = kv4_half2(e[i].x, e[i].y);
+                }
+            };
+            uint32_t s0[32], s1[32], p[32];  // 64 columns of S, and their P
+#pragma unroll 1
             for (int j = 0; j < n; j++) {
                 KP_WAIT_WARP(bars.s_full[m], j & 1);
                 tc::fence_after();
-                const int p0 = seen.tile(tile0 + j) * KP_N;
-                // In halves of 64 positions, so that the first one's product runs beside the second's exps
+                tc::ld32(ts, s0);
+                // In halves of 64 positions, so that the first one's product runs beside the second's exps; half of the
+                // next 64 columns is read while the second half of these is worked on
 #pragma unroll 1
                 for (int hf = 0; hf < 2; hf++) {
-                    const int ph = p0 + 64 * hf;
-                    const bool whole = ph + 63 <= t_lo && (a.window == 0 || ph > t_hi - a.window || ph + 64 <= a.n_sink);
+                    const int k0 = seen.tile(tile0 + j) * KP_N + 64 * hf;
+                    const bool whole = k0 + 63 <= t_lo && (a.window == 0 || k0 > t_hi - a.window || k0 + 64 <= a.n_sink);
                     const uint32_t th = ts + 64 * hf;
-                    auto hide = [&](uint32_t (&s)[32], int ch) {
-                        if (whole) return;
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const int k = ph + ch + i;
-                            if (k > t || (k <= w_lo && k >= a.n_sink)) s[i] = 0xff800000u;  // -inf
-                        }
-                    };
-                    // P against a reference, and its sum
-                    uint32_t p[32];
-                    auto attempt = [&](float neg_ref) -> float {
-                        const uint64_t c2 = tc::pair(cs, cs), r2 = tc::pair(neg_ref, neg_ref);
-                        uint64_t sum0 = 0, sum1 = 0;
-                        auto part = [&](uint32_t (&s)[32], int ch) {
-                            hide(s, ch);
-#pragma unroll
-                            for (int i = 0; i < 32; i += 4) {
-                                const uint64_t x = tc::fma2(tc::pair(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, r2);
-                                const uint64_t y = tc::fma2(tc::pair(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), c2, r2);
-                                const float2 e = kp_exp2_pair(x), f = i % KP_POLY == 0 ? kp_poly2_pair(y) : kp_exp2_pair(y);
-                                sum0 = tc::add2(sum0, tc::pair(e.x, e.y)), sum1 = tc::add2(sum1, tc::pair(f.x, f.y));
-                                p[(ch + i) / 2] = kv4_half2(e.x, e.y), p[(ch + i) / 2 + 1] = kv4_half2(f.x, f.y);
-                            }
-                        };
-                        uint32_t s0[32], s1[32];
-                        tc::ld32(th, s0);
-                        tc::wait_ld(s0);
-                        tc::ld32(th + 32, s1);
-                        part(s0, 0);
-                        tc::wait_ld(s1);
-                        part(s1, 32);
-                        const float2 x = tc::unpair(tc::add2(sum0, sum1));
-                        return x.x + x.y;
-                    };
-                    float sum = 0.0f;
+                    tc::ld32(th + 32, s1);
+                    tc::wait_ld(s0);
+                    tc::wait_ld(s1);
+                    float sum;
                     bool raise = __any_sync(0xffffffffu, ref == -INFINITY);
 #pragma unroll 1
                     for (int tries = 0; tries < 2; tries++) {
@@ -306,12 +296,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                             float mx = -INFINITY;
 #pragma unroll 1
                             for (int ch = 0; ch < 64; ch += 32) {
-                                uint32_t s[32];
-                                tc::ld32(th + ch, s);
-                                tc::wait_ld(s);
-                                hide(s, ch);
+                                tc::ld32(th + ch, s0);
+                                tc::wait_ld(s0);
 #pragma unroll
-                                for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(s[i]));
+                                for (int i = 0; i < 32; i++) {
+                                    const int k = k0 + ch + i;
+                                    if (k <= t && (k > w_lo || k < a.n_sink)) mx = fmaxf(mx, __uint_as_float(s0[i]));
+                                }
                             }
                             const float next = fmaxf(ref, mx * cs);
                             const float f = ref == -INFINITY ? 0.0f : kv4_exp2(ref - next);
@@ -324,18 +315,35 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                             if (j > 0 || hf) {
 #pragma unroll 1
                                 for (int ch = 0; ch < HD; ch += 32) {
-                                    uint32_t o[32];
-                                    tc::ld32(to + ch, o);
-                                    tc::wait_ld(o);
+                                    tc::ld32(to + ch, s0);
+                                    tc::wait_ld(s0);
 #pragma unroll
-                                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                    tc::st32(to + ch, o);
+                                    for (int i = 0; i < 32; i++) s0[i] = __float_as_uint(__uint_as_float(s0[i]) * f);
+                                    tc::st32(to + ch, s0);
                                 }
                             }
+                            tc::ld32(th, s0);
+                            tc::ld32(th + 32, s1);
+                            tc::wait_ld(s0);
+                            tc::wait_ld(s1);
                         }
-                        sum = attempt(KP_BIAS - (ref == -INFINITY ? 0.0f : ref));
+                        const float neg_ref = KP_BIAS - (ref == -INFINITY ? 0.0f : ref);
+                        const uint64_t c2 = tc::pair(cs, cs), r2 = tc::pair(neg_ref, neg_ref);
+                        uint64_t sums[2] = {0, 0};
+                        if (whole)
+                            exps(s0, p, c2, r2, sums, k0, KpNo{});
+                        else
+                            exps(s0, p, c2, r2, sums, k0, KpYes{});
+                        if (!hf) tc::ld32(ts + 64, s0);
+                        if (whole)
+                            exps(s1, p + 16, c2, r2, sums, k0 + 32, KpNo{});
+                        else
+                            exps(s1, p + 16, c2, r2, sums, k0 + 32, KpYes{});
+                        const float2 x = tc::unpair(tc::add2(sums[0], sums[1]));
+                        sum = x.x + x.y;
                         raise = __any_sync(0xffffffffu, sum > KP_MOST);
                         if (!raise) break;
+                        tc::wait_ld(s0);
                     }
                     l += sum;
                     tc::st32(th, p);
@@ -348,10 +356,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
             // ---- the rows' results
             float inv = l == 0.0f ? 0.0f : 1.0f / l;
             float *part = nullptr;
-            if (a.splits > 1) {
-                part = a.part + ((int64_t)blockIdx.x * KP_ROWS + m * KP_M + r) * (HD + 2);
-                part[0] = ref, part[1] = l;
-                inv = 1.0f;
+            if (a.splits > 1) {  // O as it is, rows side by side
+                part = a.part + (int64_t)blockIdx.x * KP_ROWS * (HD + 2) + (m * KP_M + r) * 4;
+                float *stats = a.part + (int64_t)blockIdx.x * KP_ROWS * (HD + 2) + KP_ROWS * HD + m * KP_M + r;
+                stats[0] = ref, stats[KP_ROWS] = l;
             }
             if (n > 0) {
                 KP_WAIT_WARP(bars.o_full[m], 0);
@@ -362,21 +370,19 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                     uint32_t o[32];
                     tc::ld32(to + ch, o);
                     tc::wait_ld(o);
-                    if (row < rows) {
+                    if (part) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4 *>(part + (ch + i) * KP_ROWS) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    } else if (row < rows) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {
                             // column 2e of a chunk is value e, column 2e + 1 value 4 + e
                             float x[8];
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                x[e] = __uint_as_float(o[i + 2 * e]) * inv, x[4 + e] = __uint_as_float(o[i + 2 * e + 1]) * inv;
-                            if (part) {
-#pragma unroll
-                                for (int e = 0; e < 8; e += 2)
-                                    *reinterpret_cast<float2 *>(part + 2 + ch + i + e) = make_float2(x[e], x[e + 1]);
-                            } else {
-                                kv4_store_row(out + ch + i, x);
-                            }
+                            for (int v = 0; v < 4; v++)
+                                x[v] = __uint_as_float(o[i + 2 * v]) * inv, x[4 + v] = __uint_as_float(o[i + 2 * v + 1]) * inv;
+                            kv4_store_row(out + ch + i, x);
                         }
                     }
                 }
@@ -512,51 +518,52 @@ done:
     }
 }
 
-// The rows' parts, in order: a warp per row.
+// The rows' parts, in order: a thread per row and 8 values, a block's rows side by side.
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) kv4_join_kernel(const float *__restrict__ part, T *__restrict__ out, int64_t out_ld,
-                                                       int n_tok, int n_head, int n_kv, int splits) {
-    constexpr int V = HD / 32;  // values a lane
+__global__ void __launch_bounds__(KP_ROWS) kv4_join_kernel(const float *__restrict__ part, T *__restrict__ out, int64_t out_ld,
+                                                           int n_tok, int n_head, int n_kv, int splits) {
     pdl_wait();
     pdl_trigger();
-    const int G = n_head / n_kv, rows = n_tok * G;
-    const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (u >= (int64_t)rows * n_kv) return;
-    const int g = (int)(u / rows), row = (int)(u % rows);
-    const int blocks = (rows + KP_ROWS - 1) / KP_ROWS;
-    const int64_t cta = ((int64_t)(blocks - 1 - row / KP_ROWS) * n_kv + g) * splits;
-    const float *p = part + (cta * KP_ROWS + row % KP_ROWS) * (HD + 2);
-    const int64_t step = (int64_t)KP_ROWS * (HD + 2);
-    // lane s (and s + 32, ...) looks at part s
-    float top = -INFINITY;
-    for (int s = lane; s < splits; s += 32) top = fmaxf(top, __ldcg(p + s * step));
+    const int G = n_head / n_kv, rows = n_tok * G, blocks = (rows + KP_ROWS - 1) / KP_ROWS;
+    const int g8 = blockIdx.x % (HD / 8), list = blockIdx.x / (HD / 8);  // of (block, KV head), as the CTAs were numbered
+    const int row = (blocks - 1 - list / n_kv) * KP_ROWS + (int)threadIdx.x, g = list % n_kv;
+    if (row >= rows) return;
+    constexpr int64_t STEP = (int64_t)KP_ROWS * (HD + 2);
+    const float *p = part + (int64_t)list * splits * STEP;
+    const float *stats = p + KP_ROWS * HD + threadIdx.x;
+    const float4 *o = reinterpret_cast<const float4 *>(p) + 2 * g8 * KP_ROWS + threadIdx.x;
+    float top = -INFINITY, L = 0.0f, x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+    for (int s0 = 0; s0 < splits; s0 += 4) {
+        float r[4], l[4];
+        float4 y[4][2];
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float L = 0.0f, x[V];
+        for (int u = 0; u < 4; u++) {
+            const bool in = s0 + u < splits;
+            const int64_t at = (s0 + u) * STEP;
+            r[u] = in ? __ldcg(stats + at) : -INFINITY, l[u] = in ? __ldcg(stats + at + KP_ROWS) : 0.0f;
+            y[u][0] = in ? __ldcg(o + at / 4) : make_float4(0, 0, 0, 0);
+            y[u][1] = in ? __ldcg(o + at / 4 + KP_ROWS) : make_float4(0, 0, 0, 0);
+        }
+        const float next = fmaxf(fmaxf(top, fmaxf(r[0], r[1])), fmaxf(r[2], r[3]));
+        const float f = top == -INFINITY ? 1.0f : kv4_exp2(top - next);
+        top = next, L *= f;
 #pragma unroll
-    for (int i = 0; i < V; i++) x[i] = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < splits; s++) {
-        const float2 rl = __ldcg(reinterpret_cast<const float2 *>(p + s * step));
-        if (rl.y == 0.0f) continue;  // nothing seen there: its sums were not written
-        const float f = rl.x == -INFINITY ? 1.0f : kv4_exp2(rl.x - top);
-        L += f * rl.y;
+        for (int e = 0; e < 8; e++) x[e] *= f;
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-            const float2 y = __ldcg(reinterpret_cast<const float2 *>(p + s * step + 2 + V * lane + i));
-            x[i] += f * y.x, x[i + 1] += f * y.y;
+        for (int u = 0; u < 4; u++) {
+            if (l[u] == 0.0f) continue;  // nothing seen there: its sums were not written
+            const float w = r[u] == -INFINITY ? 1.0f : kv4_exp2(r[u] - top);
+            L += w * l[u];
+            // column 2e of a chunk is value e, column 2e + 1 value 4 + e
+            x[0] += w * y[u][0].x, x[4] += w * y[u][0].y, x[1] += w * y[u][0].z, x[5] += w * y[u][0].w;
+            x[2] += w * y[u][1].x, x[6] += w * y[u][1].y, x[3] += w * y[u][1].z, x[7] += w * y[u][1].w;
         }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    T *o = out + (int64_t)(row / G) * out_ld + (int64_t)(g * G + row % G) * HD + V * lane;
 #pragma unroll
-    for (int i = 0; i < V; i += 2) {
-        if constexpr (sizeof(T) == 4)
-            *reinterpret_cast<float2 *>(o + i) = make_float2(x[i] * inv, x[i + 1] * inv);
-        else
-            *reinterpret_cast<uint32_t *>(o + i) = kv4_pack_bf2(x[i] * inv, x[i + 1] * inv);
-    }
+    for (int e = 0; e < 8; e++) x[e] *= inv;
+    kv4_store_row(out + (int64_t)(row / G) * out_ld + (int64_t)(g * G + row % G) * HD + 8 * g8, x);
 }
 
 // ------------------------------------------------------------------ launchers
@@ -592,7 +599,7 @@ static cudaError_t prefill_launch(const Kv4Attn &x, const Kv4Planes &c, float *p
     cudaError_t e = launch_k(kv4_prefill_kernel<HD, T>, dim3((unsigned)(ctas * splits)), dim3(KP_THREADS),
                              (size_t)Cfg::SMEM, st, a, c);
     if (e != cudaSuccess || splits == 1) return e;
-    return launch_k(kv4_join_kernel<HD, T>, dim3((unsigned)((rows * c.n_kv + 7) / 8)), dim3(256), 0, st,
+    return launch_k(kv4_join_kernel<HD, T>, dim3((unsigned)(ctas * (HD / 8))), dim3(KP_ROWS), 0, st,
                     (const float *)part, (T *)x.out, x.out_ld, x.n_tok, x.n_head, c.n_kv, (int)splits);
 }
 
