@@ -12,12 +12,19 @@ namespace tmoe {
 // ------------------------------------------------------------------ rows in and out
 // Row i of a call: its sequence and position; false: no row.  A negative position means "no row" to
 // the caller too; any other place outside the cache latches the device error.
-__device__ __forceinline__ bool kv4_place(const int32_t *seq, int seq0, const int32_t *pos, int pos0, int64_t i,
-                                          const Kv4Planes &c, int *err, int &s, int &p) {
-    const int64_t ps = pos ? pos[i] : pos0 + i, sq = seq ? seq[i] : seq0 >= 0 ? seq0 : i;
+struct Kv4RowArgs {
+    void *k, *v;
+    int64_t ld, n;
+    const int32_t *seq, *pos;  // nullptr: seq0 (or row i of sequence i where it is negative), pos0 + i
+    int seq0, pos0;
+    Kv4Planes c;
+    int *err;
+};
+__device__ __forceinline__ bool kv4_place(const Kv4RowArgs &a, int64_t i, int &s, int &p) {
+    const int64_t ps = a.pos ? a.pos[i] : a.pos0 + i, sq = a.seq ? a.seq[i] : a.seq0 >= 0 ? a.seq0 : i;
     if (ps < 0) return false;
-    if (ps >= c.n_ctx || sq < 0 || sq >= c.n_seq) {
-        latch_error(err, TMOE_DEV_ERR_BADPOS);
+    if (ps >= a.c.n_ctx || sq < 0 || sq >= a.c.n_seq) {
+        latch_error(a.err, TMOE_DEV_ERR_BADPOS);
         return false;
     }
     s = (int)sq, p = (int)ps;
@@ -29,10 +36,8 @@ __device__ __forceinline__ bool kv4_place(const int32_t *seq, int seq0, const in
 // chunks; rows run fastest over the threads, so that a run of positions writes one contiguous piece of a
 // head's plane.
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) kv4_store_kernel(const T *__restrict__ k, const T *__restrict__ v, int64_t ld,
-                                                        const int32_t *__restrict__ seq, int seq0,
-                                                        const int32_t *__restrict__ pos, int pos0, int64_t n,
-                                                        Kv4Planes c, int *err) {
+__global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowArgs a) {
+    const Kv4Planes &c = a.c;
     constexpr int TPR = HD / 8, NB = HD / 32;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t i = at / TPR;
@@ -43,8 +48,8 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const T *__restrict__ k,
     pdl_trigger();
     float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     int s = 0, p = 0;
-    const bool ok = i < n && kv4_place(seq, seq0, pos, pos0, i, c, err, s, p);
-    if (ok) kv4_load_row((is_v ? v : k) + i * ld + (int64_t)g * HD + 8 * sub, x);
+    const bool ok = i < a.n && kv4_place(a, i, s, p);
+    if (ok) kv4_load_row(reinterpret_cast<const T *>(is_v ? a.v : a.k) + i * a.ld + (int64_t)g * HD + 8 * sub, x);
     float hi = -FLT_MAX, lo = FLT_MAX;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -70,10 +75,8 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const T *__restrict__ k,
 }
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) kv4_load_kernel(T *__restrict__ k, T *__restrict__ v, int64_t ld,
-                                                       const int32_t *__restrict__ seq, int seq0,
-                                                       const int32_t *__restrict__ pos, int pos0, int64_t n,
-                                                       Kv4Planes c, int *err) {
+__global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
+    const Kv4Planes &c = a.c;
     constexpr int TPR = HD / 8, NB = HD / 32;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t i = at / TPR;
@@ -82,10 +85,10 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(T *__restrict__ k, T *__r
     const bool is_v = blockIdx.y & 1;
     pdl_wait();
     pdl_trigger();
-    if (i >= n) return;
+    if (i >= a.n) return;
     float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     int s, p;
-    if (kv4_place(seq, seq0, pos, pos0, i, c, err, s, p)) {
+    if (kv4_place(a, i, s, p)) {
         const int64_t row = ((int64_t)s * c.n_kv + g) * c.n_ctx + p;
         const uint8_t *codes = (is_v ? c.vc : c.kc) + row * (HD / 2);
         const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + 16 * (b ^ kv4_turn<HD>(p)) + 4 * (sub & 3));
@@ -93,7 +96,7 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(T *__restrict__ k, T *__r
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] = d * (float)((int)((w >> (4 * j)) & 15u) - 8);
     }
-    kv4_store_row((is_v ? v : k) + i * ld + (int64_t)g * HD + 8 * sub, x);
+    kv4_store_row(reinterpret_cast<T *>(is_v ? a.v : a.k) + i * a.ld + (int64_t)g * HD + 8 * sub, x);
 }
 
 // ------------------------------------------------------------------ attention of single tokens
@@ -130,7 +133,7 @@ constexpr int KA_TILE = 32;
 constexpr int KA_WARPS = 8;
 constexpr int KA_THREADS = 32 * KA_WARPS;
 constexpr int KA_HEADS = 8;
-constexpr int KA_PART = 16;
+constexpr int KA_PART = 32;
 constexpr float KA_ROOM = 8.0f;  // how far (log2) a score may exceed its head's reference
 constexpr float KA_BIAS = 6.0f;  // P times the V scale is held below 2^(KA_BIAS + KA_ROOM)
 
@@ -220,8 +223,6 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
     constexpr uint32_t M1 = 0x000f000fu, M16 = 0x00f000f0u;
     extern __shared__ __align__(128) uint8_t ka_smem[];
     uint64_t *bars = reinterpret_cast<uint64_t *>(ka_smem + Cfg::RING);
-    __shared__ int sh_sum[KA_WARPS];
-    __shared__ int sh_start[2];  // token and the list position of its first tile
     __shared__ int sh_last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t4 = lane & 3;
     const int G = a.n_head / c.n_kv, passes = (G + KA_HEADS - 1) / KA_HEADS, H = c.n_kv * passes;
@@ -229,6 +230,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
     if (lane == 0)
         for (int s = 0; s < ST; s++) mbar_init(&bar[s], 1);
     fence_barrier_init();
+    __syncwarp();  // a warp's barriers are its own
     pdl_wait();
     pdl_trigger();
 
@@ -237,58 +239,43 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         if (p >= c.n_ctx) return -2;
         return p < 0 ? -1 : (int)p;
     };
-    // the list: token t's segments, H of them (KV heads times passes), t ascending; below 2^31 entries by the
-    // host's check.  A segment of n tiles takes ka_length(n, per) entries
-    auto tiles_of = [&](int t) -> int {
-        const int p = t < a.n_tok ? pos_of(t) : -1;
-        return p < 0 ? 0 : Kv4Seen::of<KA_TILE>(p, a.window, a.n_sink).tiles;
-    };
-    // over 256 tokens' values: the sum before this thread's, and of all; CTA barriers inside
-    auto scan = [&](int n, int &before, int &sum) {
-        int inc = n;
+    // The list: token t's segments, H of them (KV heads times passes), t ascending; below 2^31 entries by the
+    // host's check.  Every warp works out the same: a lane takes `chunk` neighbouring tokens (one, up to 32).
+    const int chunk = (a.n_tok + 31) / 32, lane_t0 = lane * chunk, lane_t1 = min(lane_t0 + chunk, a.n_tok);
+    int p_first = -1, n_first = 0;  // of the lane's first token: its position, its tiles
+    auto tiles_at = [&](int p) { return p < 0 ? 0 : Kv4Seen::of<KA_TILE>(p, a.window, a.n_sink).tiles; };
+    auto tiles_of = [&](int t) { return t == lane_t0 ? n_first : tiles_at(pos_of(t)); };
+    int total = 0, live = 0;  // tiles and tokens with a query
+    if (lane_t0 < lane_t1) p_first = pos_of(lane_t0), n_first = tiles_at(p_first);
 #pragma unroll 1
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += up;
-        }
-        if (lane == 31) sh_sum[warp] = inc;
-        __syncthreads();
-        before = inc - n, sum = 0;
-        for (int w = 0; w < KA_WARPS; w++) {
-            if (w < warp) before += sh_sum[w];
-            sum += sh_sum[w];
-        }
-        __syncthreads();
-    };
-    int total = 0, live = 0, n_mine = 0;  // tiles and tokens with a query
-#pragma unroll 1
-    for (int base = 0; base < a.n_tok; base += KA_THREADS) {
-        int before, sum;
-        n_mine = tiles_of(base + threadIdx.x);
-        scan(n_mine, before, sum);
-        total += sum;
-        live += __syncthreads_count(n_mine > 0);
+    for (int t = lane_t0; t < lane_t1; t++) {
+        const int n = tiles_of(t);
+        total += n, live += n > 0;
     }
-    total *= H, live *= H;
+    total = __reduce_add_sync(0xffffffffu, total) * H;
+    live = __reduce_add_sync(0xffffffffu, live);
+    const bool idle = live < a.n_tok;
+    live *= H;
     const int grid = gridDim.x;
     // runs of whole segments' pieces, a tile a warp at least; or runs over the list as it comes
     const int alone = live < grid ? max((total + grid - live - 1) / (grid - live), KA_WARPS) : 0x7fffffff;
     const int across = (int)(((int64_t)total + (int64_t)live * KA_PART + grid - 1) / grid);
     const bool pad = alone <= across;
     const int per = max(pad ? alone : across, 1);
-    auto length = [&](int n) { return pad ? (n + per - 1) / per * per : n + KA_PART; };
-    // this thread's token (of the last 256) in the list, and the list's length
-    int before = 0, entries = 0, all = 0;
+    auto length = [&](int n) { return n == 0 ? 0 : pad ? (n + per - 1) / per * per : n + KA_PART; };
+    int entries = 0;  // of the lane's tokens
 #pragma unroll 1
-    for (int base = 0; base < a.n_tok; base += KA_THREADS) {
-        if (a.n_tok > KA_THREADS) n_mine = tiles_of(base + threadIdx.x);
-        entries = n_mine ? H * length(n_mine) : 0;
-        int sum;
-        scan(entries, before, sum);
-        all += sum;
+    for (int t = lane_t0; t < lane_t1; t++) entries += H * length(tiles_of(t));
+    int before = entries;  // of the tokens before the lane's
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += up;
     }
+    const int all = __shfl_sync(0xffffffffu, before, 31);
+    before -= entries;
     // tokens without a query: zeros
-    for (int t = blockIdx.x; t < a.n_tok; t += gridDim.x) {
+    for (int t = blockIdx.x; idle && t < a.n_tok; t += gridDim.x) {
         const int p = pos_of(t);
         if (p >= 0) continue;
         if (p == -2 && threadIdx.x == 0) latch_error(a.err, TMOE_DEV_ERR_BADPOS);
@@ -309,31 +296,29 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
     const __half2 off1 = __float2half2_rn(1032.0f), off16 = __float2half2_rn(1152.0f);
 
     const int run = blockIdx.x, start = run * per, end = min(start + per, all);
-    // the token whose entries hold `start`
-    if (threadIdx.x == 0) sh_start[0] = -1;
-    __syncthreads();
-    if (a.n_tok <= KA_THREADS) {
-        if (before <= start && start < before + entries) sh_start[0] = threadIdx.x, sh_start[1] = before;
-    } else {
-        int done = 0;
+    if (start >= end) return;
+    // the token whose entries hold `start`, where they begin, the token's position
+    int tok = 0, tok0 = 0, p_new = 0;
+    {
+        const bool mine = before <= start && start < before + entries;
+        if (mine) {
+            tok = lane_t0, tok0 = before, p_new = p_first;
 #pragma unroll 1
-        for (int base = 0; base < a.n_tok; base += KA_THREADS) {
-            int b4, sum;
-            const int n = tiles_of(base + threadIdx.x), len = n ? H * length(n) : 0;
-            scan(len, b4, sum);
-            b4 += done, done += sum;
-            if (b4 <= start && start < b4 + len) sh_start[0] = base + threadIdx.x, sh_start[1] = b4;
+            for (;;) {
+                const int len = H * length(tiles_of(tok));
+                if (start < tok0 + len) break;
+                tok0 += len, tok++;
+            }
+            if (tok != lane_t0) p_new = pos_of(tok);
         }
+        const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+        tok = __shfl_sync(0xffffffffu, tok, src), tok0 = __shfl_sync(0xffffffffu, tok0, src);
+        p_new = __shfl_sync(0xffffffffu, p_new, src);
     }
-    __syncthreads();
-    int tok = sh_start[0];
-    if (tok < 0) return;  // the list is shorter
-    int tok0 = sh_start[1];  // where the token's first segment starts
     int at = start;
     while (at < end) {
-        const int p_new = pos_of(tok);
         if (p_new < 0) {
-            tok++;
+            p_new = pos_of(++tok);
             continue;
         }
         const Kv4Seen seen = Kv4Seen::of<KA_TILE>(p_new, a.window, a.n_sink);
@@ -344,8 +329,8 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         if (pad) {
             parts = len / per, first_run = seg0 / per;
             const int i = run - first_run;
-            first = (int)((int64_t)seen.tiles * i / parts);
-            n_part = (int)((int64_t)seen.tiles * (i + 1) / parts) - first;
+            const int each = seen.tiles / parts, more = seen.tiles - each * parts;
+            first = i * each + min(i, more), n_part = each + (i < more);
         } else {
             // its tiles are the entries from seg0 + KA_PART on
             first = max(at - seg0 - KA_PART, 0);
@@ -353,9 +338,12 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             first_run = (seg0 + KA_PART) / per, parts = (seg0 + len - 1) / per - first_run + 1;
         }
         at = upto;
-        if (at == tok0 + H * len) tok0 = at, tok++;
+        const int t = tok, p_tok = p_new;
+        if (at == tok0 + H * len) {
+            tok0 = at, tok++;
+            if (at < end) p_new = pos_of(tok);
+        }
         if (n_part <= 0) continue;
-        const int t = at == tok0 ? tok - 1 : tok;
         const int g = hc / passes, h0 = (hc % passes) * KA_HEADS;
         const int heads = min(G - h0, KA_HEADS);
         const int64_t row0 = ((int64_t)(a.seq0 >= 0 ? a.seq0 : t) * c.n_kv + g) * c.n_ctx;
@@ -469,14 +457,14 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             st_read++;
             if (st_read == ST) st_read = 0, phase ^= 1;
             const int p0 = seen.tile(first + warp + j * KA_WARPS) * KA_TILE;
-            const bool whole = seen.whole(p0, KA_TILE, a.n_sink), newest = p0 + KA_TILE > p_new;
+            const bool whole = seen.whole(p0, KA_TILE, a.n_sink), newest = p0 + KA_TILE > p_tok;
             if (!dead) {
                 if (!whole || newest) {
                     uint8_t *ks = stage_p + Cfg::KSCALES, *vs = stage_p + Cfg::VSCALES;
                     if (a.k && newest) {
                         // the new row: quantised into the tile, and (one pass only) into the cache
                         constexpr int LANES = HD / 4;
-                        const int r = p_new % KA_TILE, b = lane >> 3;
+                        const int r = p_tok % KA_TILE, b = lane >> 3;
 #pragma unroll 1
                         for (int kv = 0; kv < 2; kv++) {
                             float x[4] = {0, 0, 0, 0};
@@ -499,12 +487,12 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
 #pragma unroll
                             for (int i = 0; i < 4; i++) w |= kv4_code(x[i], inv) << (4 * i);
                             if (lane < LANES) {
-                                const int byte = 16 * (b ^ kv4_turn<HD>(p_new)) + 2 * (lane & 7);
+                                const int byte = 16 * (b ^ kv4_turn<HD>(p_tok)) + 2 * (lane & 7);
                                 *reinterpret_cast<uint16_t *>(stage_p + (kv ? Cfg::VCODES : 0) + r * (HD / 2) + byte) =
                                     (uint16_t)w;
                                 if ((lane & 7) == 0) reinterpret_cast<__half *>(kv ? vs : ks)[r * NB + b] = d;
                                 if (h0 == 0) {
-                                    const int64_t row = row0 + p_new;
+                                    const int64_t row = row0 + p_tok;
                                     *reinterpret_cast<uint16_t *>((kv ? c.vc : c.kc) + row * (HD / 2) + byte) = (uint16_t)w;
                                     if ((lane & 7) == 0) (kv ? c.vs : c.ks)[row * NB + b] = d;
                                 }
@@ -787,10 +775,8 @@ template <int HD, typename T>
 static cudaError_t rows_launch(bool store, void *k, void *v, int64_t ld, const int32_t *seq, int seq0,
                                const int32_t *pos, int pos0, int64_t n, const Kv4Planes &c, int *err, cudaStream_t st) {
     const dim3 grid((unsigned)((n * (HD / 8) + 255) / 256), 2 * c.n_kv);
-    if (store)
-        return launch_k(kv4_store_kernel<HD, T>, grid, dim3(256), 0, st, (const T *)k, (const T *)v, ld, seq, seq0, pos,
-                        pos0, n, c, err);
-    return launch_k(kv4_load_kernel<HD, T>, grid, dim3(256), 0, st, (T *)k, (T *)v, ld, seq, seq0, pos, pos0, n, c, err);
+    const Kv4RowArgs a{k, v, ld, n, seq, pos, seq0, pos0, c, err};
+    return launch_k(store ? kv4_store_kernel<HD, T> : kv4_load_kernel<HD, T>, grid, dim3(256), 0, st, a);
 }
 
 cudaError_t launch_kv4_rows(bool store, bool f32, int head_dim, void *k, void *v, int64_t ld, const int32_t *seq,

@@ -90,7 +90,7 @@ class Kv4Cache:
         self._a.scratch = self._scratch.data_ptr()
         self._ap = C.addressof(self._a)
         self._dev, self._scale = self.device.index, self.head_dim ** -0.5
-        self._q_sig = self._kv_sig = None
+        self._q_sig = self._kv_sig = self._row_sig = None
         self._kv_ld = 0
 
     @property
@@ -169,8 +169,11 @@ class Kv4Cache:
         if ty is None:
             raise ValueError(f"rows come as float32 or bfloat16, not {dtype}")
         s, s0, p, p0 = self._place(n, pos, seq)
-        k = torch.empty((n, self.n_kv, self.head_dim), dtype=dtype, device=self.device)
-        v = torch.empty_like(k)
+        sig = (n, dtype)
+        if sig != self._row_sig:  # a shape to allocate by: no memory of its own
+            self._row_sig = sig
+            self._row_like = torch.empty(1, dtype=dtype, device=self.device).expand(n, self.n_kv, self.head_dim)
+        k, v = torch.empty_like(self._row_like), torch.empty_like(self._row_like)
         rc = self.lib.tmoe_kv4_load(self.h, self._stream(stream), self._cp, ty, k.data_ptr(), v.data_ptr(),
                                     self.n_kv * self.head_dim, s, s0, p, p0, n)
         if rc:
