@@ -156,7 +156,7 @@ struct Kv4AttnCfg {
     static constexpr int CODES = KA_TILE * HD / 2, SCALES = KA_TILE * NB * 2;
     static constexpr int STAGE = 2 * (CODES + SCALES);  // K codes, V codes, K scales, V scales
     static constexpr int VCODES = CODES, KSCALES = 2 * CODES, VSCALES = 2 * CODES + SCALES;
-    static constexpr int STAGES = 3 * (128 / HD);
+    static constexpr int STAGES = 2 * (128 / HD);
     static constexpr int CTAS = 2;  // per SM
     static constexpr int RING = KA_WARPS * STAGES * STAGE;
     static constexpr int SMEM = RING + KA_WARPS * STAGES * 8 + 128;

@@ -7,6 +7,10 @@ tmoe_argmax; a step is stream-ordered and allocation-free, so it can be captured
 (Qwen3MoeModel.graph).  Qwen3MoeModel.prefill runs the prompt of one sequence as one multi-token
 step (tmoe_attn_prefill for the causal attention).
 
+kv_type="q4" keeps the KV caches in 4 bits (kv4.Kv4Cache, 4.5 bits a value against 16) and attends over them
+as they are; with it a sliding window over the last `window` positions, with the first n_sink always in
+sight, bounds what a step reads.
+
 Weights come from a GGUF file (from_gguf: the reference's load_weights, qwen3moe.rs:2498-2584) or
 are synthetic (synthetic: seeded N(0, std) weights quantised on the device)."""
 from __future__ import annotations
@@ -17,6 +21,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
+from .kv4 import Kv4Cache
 from .moe import ExpertWeights, MoeLayer, _ptr, _stream, row_size
 
 TYPE_F32, TYPE_F16, TYPE_Q4_K, TYPE_Q6_K = 0, 1, 12, 14
@@ -40,9 +45,18 @@ def _row_bytes(t: int, cols: int) -> int:
 
 
 class Qwen3MoeModel:
-    def __init__(self, hp, weights: dict, max_batch: int, n_ctx: int, device: int = 0):
+    def __init__(self, hp, weights: dict, max_batch: int, n_ctx: int, device: int = 0, kv_type: str = "f16",
+                 window: int = 0, n_sink: int = 0):
         """hp: tetraeder_b200.gguf.Hparams; weights: GGUF tensor name -> Matrix (matrices, the
-        embedding) or float32 CUDA tensor (norms, router)."""
+        embedding) or float32 CUDA tensor (norms, router).  kv_type: "f16" or "q4"; window (0: none) and
+        n_sink go with "q4"."""
+        if kv_type not in ("f16", "q4"):
+            raise ValueError(f"KV caches are f16 or q4, not {kv_type}")
+        if (window or n_sink) and kv_type != "q4":
+            raise ValueError("a sliding window needs kv_type q4")
+        if window < 0 or n_sink < 0:
+            raise ValueError(f"window {window}, {n_sink} sinks")
+        self.kv_type, self.window, self.n_sink = kv_type, window, n_sink
         self.hp, self.w, self.max_batch, self.n_ctx = hp, weights, max_batch, n_ctx
         self.device = torch.device("cuda", device)
         d, nh, nkv = hp.head_dim, hp.n_head, hp.n_head_kv
@@ -64,8 +78,10 @@ class Qwen3MoeModel:
                         for il in range(hp.n_layer)]
         f = dict(dtype=torch.float32, device=self.device)
         B = max_batch
-        self.kc = [torch.zeros((B, n_ctx, nkv, d), dtype=torch.float16, device=self.device) for _ in range(hp.n_layer)]
-        self.vc = [torch.zeros((B, n_ctx, nkv, d), dtype=torch.float16, device=self.device) for _ in range(hp.n_layer)]
+        n_f16, n_q4 = (hp.n_layer, 0) if kv_type == "f16" else (0, hp.n_layer)
+        self.kc = [torch.zeros((B, n_ctx, nkv, d), dtype=torch.float16, device=self.device) for _ in range(n_f16)]
+        self.vc = [torch.zeros((B, n_ctx, nkv, d), dtype=torch.float16, device=self.device) for _ in range(n_f16)]
+        self.kv4 = [Kv4Cache(B, nkv, d, n_ctx, device=device, layer=self.moe) for _ in range(n_q4)]
         self.x = torch.empty((B, hp.n_embd), **f)
         self.cur = torch.empty((B, hp.n_embd), **f)
         self.q = torch.empty((B, nh * d), **f)
@@ -77,14 +93,15 @@ class Qwen3MoeModel:
         self.moe_out = torch.empty((B, hp.n_embd), **f)
         self.logits = torch.empty((B, hp.n_vocab), **f)
         self.next_tokens = torch.empty((B,), dtype=torch.int32, device=self.device)
-        nbytes = self.lib.tmoe_attn_decode_scratch_bytes(self.h, B, nh, nkv, d, n_ctx)
-        _lib.check(nbytes if nbytes < 0 else 0, self.h)
-        self.scratch = torch.empty((max(nbytes, 4) + 3) // 4, **f)
+        if kv_type == "f16":
+            nbytes = self.lib.tmoe_attn_decode_scratch_bytes(self.h, B, nh, nkv, d, n_ctx)
+            _lib.check(nbytes if nbytes < 0 else 0, self.h)
+            self.scratch = torch.empty((max(nbytes, 4) + 3) // 4, **f)
 
     # -- weights -------------------------------------------------------------------------
     @classmethod
-    def from_gguf(cls, g, max_batch: int, n_ctx: int, device: int = 0) -> "Qwen3MoeModel":
-        """Every tensor the step reads, from an open GgufFile (or a path)."""
+    def from_gguf(cls, g, max_batch: int, n_ctx: int, device: int = 0, **kv) -> "Qwen3MoeModel":
+        """Every tensor the step reads, from an open GgufFile (or a path).  kv: kv_type, window, n_sink."""
         from .gguf import GgufFile
         own = not isinstance(g, GgufFile)
         g = GgufFile(g) if own else g
@@ -100,14 +117,14 @@ class Qwen3MoeModel:
                 else:
                     rows = t.ne[1] * t.ne[2] * t.ne[3]
                     w[t.name] = Matrix(t.type, buf.view(rows, -1), rows, t.ne[0])
-            return cls(hp, w, max_batch, n_ctx, device)
+            return cls(hp, w, max_batch, n_ctx, device, **kv)
         finally:
             if own:
                 g.close()
 
     @classmethod
     def synthetic(cls, hp, max_batch: int, n_ctx: int, device: int = 0, seed: int = 1, attn_types=(12, 12, 14, 12),
-                  expert_types=(12, 12, 14), embd_type=12, out_type=14, std=0.02) -> "Qwen3MoeModel":
+                  expert_types=(12, 12, 14), embd_type=12, out_type=14, std=0.02, **kv) -> "Qwen3MoeModel":
         """Seeded N(0, std) weights quantised on the device (Q4_K_M-like types by default:
         attn_q/k/o Q4_K, attn_v Q6_K, experts Q4_K/Q4_K/Q6_K, token_embd Q4_K, output Q6_K)."""
         dev = torch.device("cuda", device)
@@ -151,7 +168,7 @@ class Qwen3MoeModel:
             w[p + "ffn_up_exps.weight"] = mat(expert_types[1], hp.n_ff_exp, H, hp.n_expert)
             w[p + "ffn_down_exps.weight"] = mat(expert_types[2], H, hp.n_ff_exp, hp.n_expert)
         torch.cuda.synchronize(dev)
-        return cls(hp, w, max_batch, n_ctx, device)
+        return cls(hp, w, max_batch, n_ctx, device, **kv)
 
     # -- the step ------------------------------------------------------------------------
     def _mm(self, m: Matrix, x: torch.Tensor, out: torch.Tensor, B: int, st, reuse: bool = False, h=None):
@@ -191,9 +208,13 @@ class Qwen3MoeModel:
                                     _ptr(self.k)))
                 chk(L.tmoe_rope_neox(h, st, _ptr(self.q), _ptr(pos), B, nh, d, hp.n_rot, hp.rope_freq_base))
                 chk(L.tmoe_rope_neox(h, st, _ptr(self.k), _ptr(pos), B, nkv, d, hp.n_rot, hp.rope_freq_base))
-            chk(L.tmoe_attn_decode(h, st, _ptr(self.q), _ptr(self.k), _ptr(self.v), _ptr(self.kc[il]),
-                                   _ptr(self.vc[il]), _ptr(pos), B, nh, nkv, d, self.n_ctx, 1.0 / d ** 0.5,
-                                   _ptr(self.scratch), _ptr(self.att)))
+            if self.kv4:
+                self.kv4[il].decode(self.q[:B].view(B, nh, d), self.k[:B].view(B, nkv, d), self.v[:B].view(B, nkv, d), pos,
+                                    window=self.window, n_sink=self.n_sink, out=self.att[:B].view(B, nh, d), stream=stream)
+            else:
+                chk(L.tmoe_attn_decode(h, st, _ptr(self.q), _ptr(self.k), _ptr(self.v), _ptr(self.kc[il]),
+                                       _ptr(self.vc[il]), _ptr(pos), B, nh, nkv, d, self.n_ctx, 1.0 / d ** 0.5,
+                                       _ptr(self.scratch), _ptr(self.att)))
             self._mm(w[p + "attn_output.weight"], self.att, self.o, B, st)
             chk(L.tmoe_add(h, st, _ptr(self.x), _ptr(self.o), _ptr(self.ffn_inp), B * H))
             self.moe.moe_ffn(self.ffn_inp[:B], self.experts[il], router_w=w[p + "ffn_gate_inp.weight"],
@@ -272,9 +293,13 @@ class Qwen3MoeModel:
             chk(L.tmoe_qk_norm_rope(h, st, _ptr(b["q"]), _ptr(b["k"]), _ptr(w[p + "attn_q_norm.weight"]),
                                     _ptr(w[p + "attn_k_norm.weight"]), _ptr(pos), S, nh, nkv, d, hp.n_rot,
                                     hp.rope_freq_base, hp.rms_eps))
-            chk(L.tmoe_attn_prefill(h, st, _ptr(b["q"]), _ptr(b["k"]), _ptr(b["v"]), _ptr(self.kc[il]),
-                                    _ptr(self.vc[il]), seq, self.max_batch, pos0, S, nh, nkv, d, self.n_ctx,
-                                    1.0 / d ** 0.5, _ptr(b["att"])))
+            if self.kv4:
+                self.kv4[il].prefill(b["q"].view(S, nh, d), b["k"].view(S, nkv, d), b["v"].view(S, nkv, d), seq=seq, pos0=pos0,
+                                     window=self.window, n_sink=self.n_sink, out=b["att"].view(S, nh, d), stream=stream)
+            else:
+                chk(L.tmoe_attn_prefill(h, st, _ptr(b["q"]), _ptr(b["k"]), _ptr(b["v"]), _ptr(self.kc[il]),
+                                        _ptr(self.vc[il]), seq, self.max_batch, pos0, S, nh, nkv, d, self.n_ctx,
+                                        1.0 / d ** 0.5, _ptr(b["att"])))
             self._mm(w[p + "attn_output.weight"], b["att"], b["o"], S, st)
             chk(L.tmoe_add(h, st, _ptr(b["x"]), _ptr(b["o"]), _ptr(b["ffn_inp"]), S * H))
             self._pf_moe.moe_ffn(b["ffn_inp"], self.experts[il], router_w=w[p + "ffn_gate_inp.weight"],
