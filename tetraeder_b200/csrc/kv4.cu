@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
 //     sums); the 8 heads are the 8 columns.  S^T = K Q^T: a 4-bit code under a mask is the f16 subnormal
 //     c * 2^-24 (or 16 times that), so a word of 8 codes becomes four operand registers with four ANDs and one
 //     shift.  The factor 16 is undone in Q.  A block's scale multiplies its own accumulator in f32: K
-//     enters exactly.  The codes' -8 is a product of its own, scales x (-8 sum of q per block), on m16n8k8.
+//     enters exactly.  The codes' -8 is a product of its own, scales x (-8 sum of q per block), on m16n8k8 (with
+//     f32 queries it is taken from the codes, as for V: sums around 0 keep the scores' last bits).
 //   - O^T += V^T P takes V as 1024 + c minus 1032 in f16 (here the -8 has to go before the product:
 //     averaged over many positions, sum(P c) - 8 sum(P) would cancel), its scale on P.
 //   - K's words through ldmatrix are the operand of two steps of 16 dimensions; V's 16-bit units (4 codes)
@@ -399,7 +400,9 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             const int e1 = e / 2, e2 = e - e1;
             const float up1 = kv4_pow2(e1), up2 = kv4_pow2(e2);
             // never 0: masked scores are -inf times it
-            const float c_gr = fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(12 - e1) * kv4_pow2(12 - e2), FLT_MIN);
+            constexpr int HALF_UNIT = PREC ? 0 : 12;  // codes count 1 with f32, 2^-24 with bf16
+            const float c_gr =
+                fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(HALF_UNIT - e1) * kv4_pow2(HALF_UNIT - e2), FLT_MIN);
             to_log2[0] = __shfl_sync(0xffffffffu, c_gr, 8 * t4);
             to_log2[1] = __shfl_sync(0xffffffffu, c_gr, 8 * t4 + 4);
             uint32_t sums[2] = {0, 0};  // [low]: of this lane's two blocks
@@ -530,19 +533,26 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                         d0[0] = *reinterpret_cast<const uint32_t *>(ks), d1[0] = *reinterpret_cast<const uint32_t *>(ks + 32);
                     }
                     s[hb][0] = s[hb][1] = s[hb][2] = s[hb][3] = 0.0f;
-                    if constexpr (HD == 128)
+                    if constexpr (PREC)
+                        ;  // the codes carry their -8
+                    else if constexpr (HD == 128)
                         ka_mma8(s[hb], t4 & 1 ? d0[1] : d0[0], t4 & 1 ? d1[1] : d1[0], q_sums);
                     else  // two blocks: lanes t4 = 0 (high) and 2 (low)
                         ka_mma8(s[hb], t4 & 1 ? 0u : d0[0], t4 & 1 ? 0u : d1[0], q_sums);
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
                         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        const uint32_t x0 = w0[b] >> 8, x1 = w1[b] >> 8;
-                        ka_mma(acc, w0[b] & M1, w1[b] & M1, w0[b] & M16, w1[b] & M16, qh[b][0], qh[b][1]);
-                        ka_mma(acc, x0 & M1, x1 & M1, x0 & M16, x1 & M16, qh[b][2], qh[b][3]);
-                        if constexpr (PREC) {
-                            ka_mma(acc, w0[b] & M1, w1[b] & M1, w0[b] & M16, w1[b] & M16, ql[b][0], ql[b][1]);
-                            ka_mma(acc, x0 & M1, x1 & M1, x0 & M16, x1 & M16, ql[b][2], ql[b][3]);
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const uint32_t x0 = i ? w0[b] >> 8 : w0[b], x1 = i ? w1[b] >> 8 : w1[b];
+                            if constexpr (PREC) {
+                                const uint32_t a0 = ka_codes(x0, M1, off1), a1 = ka_codes(x1, M1, off1);
+                                const uint32_t a2 = ka_codes(x0, M16, off16), a3 = ka_codes(x1, M16, off16);
+                                ka_mma(acc, a0, a1, a2, a3, qh[b][2 * i], qh[b][2 * i + 1]);
+                                ka_mma(acc, a0, a1, a2, a3, ql[b][2 * i], ql[b][2 * i + 1]);
+                            } else {
+                                ka_mma(acc, x0 & M1, x1 & M1, x0 & M16, x1 & M16, qh[b][2 * i], qh[b][2 * i + 1]);
+                            }
                         }
                         const float2 f0 = ka_float2(d0[b / 2]), f1 = ka_float2(d1[b / 2]);
                         const float e0 = b & 1 ? f0.y : f0.x, e1 = b & 1 ? f1.y : f1.x;
