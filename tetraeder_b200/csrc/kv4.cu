@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
 // CTA has more than one (the cheaper of the two by its longest run).  A warp takes every 8th tile of a
 // run, fetched by bulk copies into its own ring.  Runs that hold less than a segment leave partial sums in
 // scratch; the CTA that arrives last there joins them, in run order (the same sums every call).
-constexpr int KA_TILE = 32;
+constexpr int KA_TILE_VALUES = 4096;  // of K, and of V, in a tile: 32 positions of 128-wide heads
 constexpr int KA_WARPS = 8;
 constexpr int KA_THREADS = 32 * KA_WARPS;
 constexpr int KA_HEADS = 8;
@@ -154,10 +154,11 @@ struct Kv4AttnArgs {
 template <int HD, bool PREC>
 struct Kv4AttnCfg {
     static constexpr int NB = HD / 32;
-    static constexpr int CODES = KA_TILE * HD / 2, SCALES = KA_TILE * NB * 2;
+    static constexpr int TILE = KA_TILE_VALUES / HD;  // positions
+    static constexpr int CODES = TILE * HD / 2, SCALES = TILE * NB * 2;
     static constexpr int STAGE = 2 * (CODES + SCALES);  // K codes, V codes, K scales, V scales
     static constexpr int VCODES = CODES, KSCALES = 2 * CODES, VSCALES = 2 * CODES + SCALES;
-    static constexpr int STAGES = 2 * (128 / HD);
+    static constexpr int STAGES = 2;
     static constexpr int CTAS = 2;  // per SM
     static constexpr int RING = KA_WARPS * STAGES * STAGE;
     static constexpr int SMEM = RING + KA_WARPS * STAGES * 8 + 128;
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
     kv4_attn_kernel(const Kv4AttnArgs a, const Kv4Planes c) {
     constexpr bool PREC = sizeof(T) == 4;
     using Cfg = Kv4AttnCfg<HD, PREC>;
-    constexpr int NB = Cfg::NB, ST = Cfg::STAGES, RW = HD + 2;
+    constexpr int NB = Cfg::NB, ST = Cfg::STAGES, RW = HD + 2, TILE = Cfg::TILE, HB = TILE / 16;
     constexpr uint32_t M1 = 0x000f000fu, M16 = 0x00f000f0u;
     extern __shared__ __align__(128) uint8_t ka_smem[];
     uint64_t *bars = reinterpret_cast<uint64_t *>(ka_smem + Cfg::RING);
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
     // host's check.  Every warp works out the same: a lane takes `chunk` neighbouring tokens (one, up to 32).
     const int chunk = (a.n_tok + 31) / 32, lane_t0 = lane * chunk, lane_t1 = min(lane_t0 + chunk, a.n_tok);
     int p_first = -1, n_first = 0;  // of the lane's first token: its position, its tiles
-    auto tiles_at = [&](int p) { return p < 0 ? 0 : Kv4Seen::of<KA_TILE>(p, a.window, a.n_sink).tiles; };
+    auto tiles_at = [&](int p) { return p < 0 ? 0 : Kv4Seen::of<TILE>(p, a.window, a.n_sink).tiles; };
     auto tiles_of = [&](int t) { return t == lane_t0 ? n_first : tiles_at(pos_of(t)); };
     int total = 0, live = 0;  // tiles and tokens with a query
     if (lane_t0 < lane_t1) p_first = pos_of(lane_t0), n_first = tiles_at(p_first);
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             p_new = pos_of(++tok);
             continue;
         }
-        const Kv4Seen seen = Kv4Seen::of<KA_TILE>(p_new, a.window, a.n_sink);
+        const Kv4Seen seen = Kv4Seen::of<TILE>(p_new, a.window, a.n_sink);
         const int len = length(seen.tiles), hc = (at - tok0) / len;
         const int seg0 = tok0 + hc * len, upto = min(end, seg0 + len);
         // the segment's tiles first .. first + n_part - 1, and whose runs hold the others
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             piece = is_scale ? Cfg::SCALES : Cfg::CODES;
             dst = ring + (is_scale ? Cfg::KSCALES : 0) + (is_v ? piece : 0);
             src = (is_scale ? reinterpret_cast<const uint8_t *>(is_v ? c.vs : c.ks) : is_v ? c.vc : c.kc) +
-                  row0 * (piece / KA_TILE);
+                  row0 * (piece / TILE);
         }
         auto fill = [&](int j) {
             uint64_t *b = &bar[st_fill];
@@ -459,15 +460,15 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             uint8_t *const stage_p = ka_smem + (stage - smem_u32(ka_smem));
             st_read++;
             if (st_read == ST) st_read = 0, phase ^= 1;
-            const int p0 = seen.tile(first + warp + j * KA_WARPS) * KA_TILE;
-            const bool whole = seen.whole(p0, KA_TILE, a.n_sink), newest = p0 + KA_TILE > p_tok;
+            const int p0 = seen.tile(first + warp + j * KA_WARPS) * TILE;
+            const bool whole = seen.whole(p0, TILE, a.n_sink), newest = p0 + TILE > p_tok;
             if (!dead) {
                 if (!whole || newest) {
                     uint8_t *ks = stage_p + Cfg::KSCALES, *vs = stage_p + Cfg::VSCALES;
                     if (a.k && newest) {
                         // the new row: quantised into the tile, and (one pass only) into the cache
                         constexpr int LANES = HD / 4;
-                        const int r = p_tok % KA_TILE, b = lane >> 3;
+                        const int r = p_tok % TILE, b = lane >> 3;
 #pragma unroll 1
                         for (int kv = 0; kv < 2; kv++) {
                             float x[4] = {0, 0, 0, 0};
@@ -503,23 +504,24 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                         }
                         __syncwarp();
                     }
-                    if (!seen.sees(p0 + lane, a.n_sink)) {
-                        // rows that are not seen may hold anything: their scales become zero
+                    // rows that are not seen may hold anything: their scales become zero
+                    for (int r = lane; r < TILE; r += 32)
+                        if (!seen.sees(p0 + r, a.n_sink)) {
 #pragma unroll
-                        for (int b = 0; b < NB; b += 2) {
-                            *reinterpret_cast<uint32_t *>(ks + (lane * NB + b) * 2) = 0u;
-                            *reinterpret_cast<uint32_t *>(vs + (lane * NB + b) * 2) = 0u;
+                            for (int b = 0; b < NB; b += 2) {
+                                *reinterpret_cast<uint32_t *>(ks + (r * NB + b) * 2) = 0u;
+                                *reinterpret_cast<uint32_t *>(vs + (r * NB + b) * 2) = 0u;
+                            }
                         }
-                    }
                     // shared memory that a later bulk copy fills again
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
 
                 // ---- S^T: rows positions 16 hb + gr + {0, 8}, columns heads 2 t4 + {0, 1}
-                float s[2][4];
+                float s[HB][4];
 #pragma unroll
-                for (int hb = 0; hb < 2; hb++) {
+                for (int hb = 0; hb < HB; hb++) {
                     uint32_t w0[NB], w1[NB];  // words t4 of rows gr, gr + 8
                     uint32_t d0[NB / 2], d1[NB / 2];
                     const uint8_t *ks = stage_p + Cfg::KSCALES + (16 * hb + gr) * NB * 2;
@@ -562,22 +564,23 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                 }
                 if (!whole) {
 #pragma unroll
-                    for (int hb = 0; hb < 2; hb++)
+                    for (int hb = 0; hb < HB; hb++)
 #pragma unroll
                         for (int i = 0; i < 2; i++)
                             if (!seen.sees(p0 + 16 * hb + gr + 8 * i, a.n_sink)) s[hb][2 * i] = s[hb][2 * i + 1] = -INFINITY;
                 }
                 // ---- the references and the largest V scale, which seldom grow
                 float mx[2];
-                mx[0] = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])) * to_log2[0];
-                mx[1] = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3])) * to_log2[1];
-                uint32_t dm;  // this lane's position: its largest V scale
-                if constexpr (HD == 128) {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(stage_p + Cfg::VSCALES + lane * 8);
-                    dm = __vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu);
-                } else {
-                    dm = *reinterpret_cast<const uint32_t *>(stage_p + Cfg::VSCALES + lane * 4) & 0x7fff7fffu;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    mx[i] = fmaxf(s[0][i], s[0][2 + i]);
+#pragma unroll
+                    for (int hb = 1; hb < HB; hb++) mx[i] = fmaxf(mx[i], fmaxf(s[hb][i], s[hb][2 + i]));
+                    mx[i] *= to_log2[i];
                 }
+                static_assert(Cfg::SCALES == 32 * 8, "8 bytes of V scales a lane");
+                const uint2 u = *reinterpret_cast<const uint2 *>(stage_p + Cfg::VSCALES + lane * 8);
+                uint32_t dm = __vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu);  // the largest of this lane's V scales
                 dm = max(dm & 0xffffu, dm >> 16);
                 if (__any_sync(0xffffffffu, mx[0] > ref[0] + KA_ROOM || mx[1] > ref[1] + KA_ROOM || dm > v_top)) {
                     float f[2];
@@ -607,7 +610,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
 #pragma unroll
                 for (int i = 0; i < 2; i++) nr[i] = (PREC ? 0.0f : KA_BIAS) - (ref[i] == -INFINITY ? 0.0f : ref[i]);
 #pragma unroll
-                for (int hb = 0; hb < 2; hb++)
+                for (int hb = 0; hb < HB; hb++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         s[hb][i] = kv4_exp2(fmaf(s[hb][i], to_log2[i & 1], nr[i & 1]));
@@ -617,7 +620,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                 const float room = kv4_pow2(-v_exp);
                 const __half2 room2 = __float2half2_rn(room);
 #pragma unroll
-                for (int hb = 0; hb < 2; hb++) {
+                for (int hb = 0; hb < HB; hb++) {
                     uint32_t ph[NB][2], pl[PREC ? NB : 1][2];  // positions 2 t4 + {0, 1} and + 8, column head gr
                     if constexpr (PREC) {
                         const uint8_t *vs = stage_p + Cfg::VSCALES + (16 * hb + gr) * NB * 2;
@@ -822,9 +825,9 @@ static cudaError_t attn_launch(Kv4Attn &x, const Kv4Planes &c, void *scratch, in
     }
     // as many CTAs as the most tiles that the cache allows need, at a tile a warp, and at most what is resident
     const int G = x.n_head / c.n_kv, passes = (G + KA_HEADS - 1) / KA_HEADS;
-    const int most = x.window > 0 && x.window < c.n_ctx ? x.window + 2 * KA_TILE + x.n_sink : c.n_ctx;
+    const int most = x.window > 0 && x.window < c.n_ctx ? x.window + 2 * Cfg::TILE + x.n_sink : c.n_ctx;
     const int64_t segments = (int64_t)x.n_tok * c.n_kv * passes;
-    const int64_t tiles = segments * (((most < c.n_ctx ? most : c.n_ctx) + KA_TILE - 1) / KA_TILE);
+    const int64_t tiles = segments * (((most < c.n_ctx ? most : c.n_ctx) + Cfg::TILE - 1) / Cfg::TILE);
     if (tiles + KA_PART * segments > (1ll << 30)) return cudaErrorInvalidValue;  // list positions are 32-bit
     const int64_t want = segments + (tiles + KA_WARPS - 1) / KA_WARPS, cap = (int64_t)Cfg::CTAS * sm_count;
     Kv4AttnArgs a;
