@@ -130,9 +130,6 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
 // CTA has more than one (the cheaper of the two by its longest run).  A warp takes every 8th tile of a
 // run, fetched by bulk copies into its own ring.  Runs that hold less than a segment leave partial sums in
 // scratch; the CTA that arrives last there joins them, in run order (the same sums every call).
-constexpr int KA_TILE_VALUES = 4096;  // of K, and of V, in a tile: 32 positions of 128-wide heads
-constexpr int KA_WARPS = 8;
-constexpr int KA_THREADS = 32 * KA_WARPS;
 constexpr int KA_HEADS = 8;
 constexpr int KA_PART = 32;
 constexpr float KA_ROOM = 8.0f;  // how far (log2) a score may exceed its head's reference
@@ -154,15 +151,16 @@ struct Kv4AttnArgs {
 template <int HD, bool PREC>
 struct Kv4AttnCfg {
     static constexpr int NB = HD / 32;
-    static constexpr int TILE = KA_TILE_VALUES / HD;  // positions
+    static constexpr int TILE = 64;  // positions
+    static constexpr int WARPS = HD == 128 ? (PREC ? 8 : 12) : (PREC ? 6 : 6), STAGES = HD == 128 ? (PREC ? 3 : 2) : (PREC ? 4 : 4);
+    static constexpr int CTAS = HD == 128 ? (PREC ? 1 : 1) : (PREC ? 2 : 2);  // per SM
+    static constexpr int THREADS = 32 * WARPS;
     static constexpr int CODES = TILE * HD / 2, SCALES = TILE * NB * 2;
     static constexpr int STAGE = 2 * (CODES + SCALES);  // K codes, V codes, K scales, V scales
     static constexpr int VCODES = CODES, KSCALES = 2 * CODES, VSCALES = 2 * CODES + SCALES;
-    static constexpr int STAGES = 2;
-    static constexpr int CTAS = 2;  // per SM
-    static constexpr int RING = KA_WARPS * STAGES * STAGE;
-    static constexpr int SMEM = RING + KA_WARPS * STAGES * 8 + 128;
-    static_assert(KA_WARPS * KA_HEADS * (HD + 2) * 4 <= RING, "the warps' sums are joined in the ring's space");
+    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int SMEM = RING + WARPS * STAGES * 8 + 128;
+    static_assert(WARPS * KA_HEADS * (HD + 2) * 4 <= RING, "the warps' sums are joined in the ring's space");
 };
 
 __device__ __forceinline__ void ka_ldsm(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
@@ -217,11 +215,11 @@ __device__ __forceinline__ uint32_t ka_codes(uint32_t u, uint32_t mask, __half2 
 }
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::CTAS))
+__global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4>::THREADS), (Kv4AttnCfg<HD, sizeof(T) == 4>::CTAS))
     kv4_attn_kernel(const Kv4AttnArgs a, const Kv4Planes c) {
     constexpr bool PREC = sizeof(T) == 4;
     using Cfg = Kv4AttnCfg<HD, PREC>;
-    constexpr int NB = Cfg::NB, ST = Cfg::STAGES, RW = HD + 2, TILE = Cfg::TILE, HB = TILE / 16;
+    constexpr int NB = Cfg::NB, ST = Cfg::STAGES, RW = HD + 2, TILE = Cfg::TILE, HB = TILE / 16, WARPS = Cfg::WARPS;
     constexpr uint32_t M1 = 0x000f000fu, M16 = 0x00f000f0u;
     extern __shared__ __align__(128) uint8_t ka_smem[];
     uint64_t *bars = reinterpret_cast<uint64_t *>(ka_smem + Cfg::RING);
@@ -260,7 +258,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
     live *= H;
     const int grid = gridDim.x;
     // runs of whole segments' pieces, a tile a warp at least; or runs over the list as it comes
-    const int alone = live < grid ? max((total + grid - live - 1) / (grid - live), KA_WARPS) : 0x7fffffff;
+    const int alone = live < grid ? max((total + grid - live - 1) / (grid - live), WARPS) : 0x7fffffff;
     const int across = (int)(((int64_t)total + (int64_t)live * KA_PART + grid - 1) / grid);
     const bool pad = alone <= across;
     const int per = max(pad ? alone : across, 1);
@@ -283,7 +281,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         if (p == -2 && threadIdx.x == 0) latch_error(a.err, TMOE_DEV_ERR_BADPOS);
         T *o = reinterpret_cast<T *>(a.out) + (int64_t)t * a.out_ld;
         const float z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        for (int i = threadIdx.x; i < a.n_head * HD / 8; i += KA_THREADS) kv4_store_row(o + 8 * i, z);
+        for (int i = threadIdx.x; i < a.n_head * HD / 8; i += Cfg::THREADS) kv4_store_row(o + 8 * i, z);
     }
     // the ring: the next stage to fill and to read, and the phase of the latter
     int st_fill = 0, st_read = 0;
@@ -351,7 +349,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         const int64_t row0 = ((int64_t)(a.seq0 >= 0 ? a.seq0 : t) * c.n_kv + g) * c.n_ctx;
 
         // ---- this warp's tiles: first + warp, first + warp + 8, ...  Lanes 0..3 copy a plane's piece each
-        const int mine = n_part > warp ? (n_part - warp + KA_WARPS - 1) / KA_WARPS : 0;
+        const int mine = n_part > warp ? (n_part - warp + WARPS - 1) / WARPS : 0;
         const uint8_t *src;
         uint32_t piece, dst;
         {
@@ -368,7 +366,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                 asm volatile(
                     "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                         dst + st_fill * Cfg::STAGE),
-                    "l"(src + (int64_t)seen.tile(first + warp + j * KA_WARPS) * piece), "r"(piece), "r"(smem_u32(b))
+                    "l"(src + (int64_t)seen.tile(first + warp + j * WARPS) * piece), "r"(piece), "r"(smem_u32(b))
                     : "memory");
             st_fill = st_fill + 1 == ST ? 0 : st_fill + 1;
         };
@@ -460,7 +458,7 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
             uint8_t *const stage_p = ka_smem + (stage - smem_u32(ka_smem));
             st_read++;
             if (st_read == ST) st_read = 0, phase ^= 1;
-            const int p0 = seen.tile(first + warp + j * KA_WARPS) * TILE;
+            const int p0 = seen.tile(first + warp + j * WARPS) * TILE;
             const bool whole = seen.whole(p0, TILE, a.n_sink), newest = p0 + TILE > p_tok;
             if (!dead) {
                 if (!whole || newest) {
@@ -578,9 +576,12 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                     for (int hb = 1; hb < HB; hb++) mx[i] = fmaxf(mx[i], fmaxf(s[hb][i], s[hb][2 + i]));
                     mx[i] *= to_log2[i];
                 }
-                static_assert(Cfg::SCALES == 32 * 8, "8 bytes of V scales a lane");
-                const uint2 u = *reinterpret_cast<const uint2 *>(stage_p + Cfg::VSCALES + lane * 8);
-                uint32_t dm = __vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu);  // the largest of this lane's V scales
+                uint32_t dm = 0;  // the largest of this lane's share of V scales
+#pragma unroll
+                for (int i = 0; i < Cfg::SCALES; i += 256) {
+                    const uint2 u = *reinterpret_cast<const uint2 *>(stage_p + Cfg::VSCALES + i + lane * 8);
+                    dm = __vmaxu2(dm, __vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu));
+                }
                 dm = max(dm & 0xffffu, dm >> 16);
                 if (__any_sync(0xffffffffu, mx[0] > ref[0] + KA_ROOM || mx[1] > ref[1] + KA_ROOM || dm > v_top)) {
                     float f[2];
@@ -708,39 +709,42 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
         // A run's part of a segment that started in an earlier run is in its slot 0, else in slot 1
         float *mine_out = a.part + ((int64_t)run * 2 + (run == first_run)) * KA_HEADS * RW;
         T *out = reinterpret_cast<T *>(a.out) + (int64_t)t * a.out_ld + (int64_t)(g * G + h0) * HD;
-        // A thread joins 4 values of a head.  A sum whose reference is still -inf counts only if it is not zero
-        // (a NaN, which must come out)
-        static_assert(KA_HEADS * HD / 4 <= KA_THREADS, "a thread each");
-        const int h = threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
-        float top_ref = -INFINITY, L = 0.0f, x[4] = {0, 0, 0, 0};
-        auto add = [&](float r, float l_, float2 y0, float2 y1, float top) {
-            if (l_ == 0.0f) return;
-            const float f = r == -INFINITY ? 1.0f : kv4_exp2(r - top);
-            L += f * l_;
-            x[0] += f * y0.x, x[1] += f * y0.y, x[2] += f * y1.x, x[3] += f * y1.y;
+        // A thread joins 4 values of a head at a time.  A sum whose reference is still -inf counts only if it is not
+        // zero (a NaN, which must come out)
+        struct Sum {
+            float top = -INFINITY, l = 0.0f, x[4] = {0, 0, 0, 0};
+            __device__ __forceinline__ void add(float r, float l_, float2 y0, float2 y1) {
+                if (l_ == 0.0f) return;
+                const float f = r == -INFINITY ? 1.0f : kv4_exp2(r - top);
+                l += f * l_;
+                x[0] += f * y0.x, x[1] += f * y0.y, x[2] += f * y1.x, x[3] += f * y1.y;
+            }
+            __device__ __forceinline__ void store(T *p) const {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                if constexpr (sizeof(T) == 4)
+                    *reinterpret_cast<float4 *>(p) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+                else
+                    *reinterpret_cast<uint2 *>(p) =
+                        make_uint2(kv4_pack_bf2(x[0] * inv, x[1] * inv), kv4_pack_bf2(x[2] * inv, x[3] * inv));
+            }
         };
-        auto finish = [&]() {
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            T *p = out + h * HD + d;
-            if constexpr (PREC)
-                *reinterpret_cast<float4 *>(p) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-            else
-                *reinterpret_cast<uint2 *>(p) = make_uint2(kv4_pack_bf2(x[0] * inv, x[1] * inv), kv4_pack_bf2(x[2] * inv, x[3] * inv));
-        };
-        if (h < heads) {
+#pragma unroll 1
+        for (int i = threadIdx.x; i < heads * (HD / 4); i += Cfg::THREADS) {
+            const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
+            Sum sum;
 #pragma unroll
-            for (int w = 0; w < KA_WARPS; w++) top_ref = fmaxf(top_ref, sums[(w * KA_HEADS + h) * RW]);
+            for (int w = 0; w < WARPS; w++) sum.top = fmaxf(sum.top, sums[(w * KA_HEADS + h) * RW]);
 #pragma unroll
-            for (int w = 0; w < KA_WARPS; w++) {
+            for (int w = 0; w < WARPS; w++) {
                 const float *r = sums + (w * KA_HEADS + h) * RW;
-                add(r[0], r[1], *reinterpret_cast<const float2 *>(r + 2 + d), *reinterpret_cast<const float2 *>(r + 4 + d), top_ref);
+                sum.add(r[0], r[1], *reinterpret_cast<const float2 *>(r + 2 + d), *reinterpret_cast<const float2 *>(r + 4 + d));
             }
             if (split) {
                 float2 *r = reinterpret_cast<float2 *>(mine_out + h * RW);
-                if (d == 0) r[0] = make_float2(top_ref, L);
-                r[1 + d / 2] = make_float2(x[0], x[1]), r[2 + d / 2] = make_float2(x[2], x[3]);
+                if (d == 0) r[0] = make_float2(sum.top, sum.l);
+                r[1 + d / 2] = make_float2(sum.x[0], sum.x[1]), r[2 + d / 2] = make_float2(sum.x[2], sum.x[3]);
             } else {
-                finish();
+                sum.store(out + h * HD + d);
             }
         }
         if (split) {
@@ -752,13 +756,14 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                 if (sh_last) a.arrived[first_run] = 0;
             }
             __syncthreads();
-            if (sh_last && h < heads) {
+#pragma unroll 1
+            for (int i = threadIdx.x; sh_last && i < heads * (HD / 4); i += Cfg::THREADS) {
+                const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
                 const float *p = a.part + ((int64_t)first_run * 2 * KA_HEADS + h) * RW;
-                top_ref = -INFINITY, L = 0.0f, x[0] = x[1] = x[2] = x[3] = 0.0f;
+                Sum sum;
 #pragma unroll 1
                 for (int w0 = 0; w0 < parts; w0 += 8) {
                     float2 rl[8], y0[8], y1[8];
-                    float top = top_ref;
 #pragma unroll
                     for (int w = 0; w < 8; w++) {
                         rl[w] = make_float2(-INFINITY, 0.0f), y0[w] = y1[w] = make_float2(0.0f, 0.0f);
@@ -767,15 +772,16 @@ __global__ void __launch_bounds__(KA_THREADS, (Kv4AttnCfg<HD, sizeof(T) == 4>::C
                             rl[w] = __ldcg(r), y0[w] = __ldcg(r + 1 + d / 2), y1[w] = __ldcg(r + 2 + d / 2);
                         }
                     }
+                    float top = sum.top;
 #pragma unroll
                     for (int w = 0; w < 8; w++) top = fmaxf(top, rl[w].x);
-                    const float f = top_ref == -INFINITY ? 1.0f : kv4_exp2(top_ref - top);
-                    L *= f, x[0] *= f, x[1] *= f, x[2] *= f, x[3] *= f;
-                    top_ref = top;
+                    const float f = sum.top == -INFINITY ? 1.0f : kv4_exp2(sum.top - top);
+                    sum.l *= f, sum.x[0] *= f, sum.x[1] *= f, sum.x[2] *= f, sum.x[3] *= f;
+                    sum.top = top;
 #pragma unroll
-                    for (int w = 0; w < 8; w++) add(rl[w].x, rl[w].y, y0[w], y1[w], top);
+                    for (int w = 0; w < 8; w++) sum.add(rl[w].x, rl[w].y, y0[w], y1[w]);
                 }
-                finish();
+                sum.store(out + h * HD + d);
             }
         }
         __syncthreads();  // the sums are read; the ring may be filled again
@@ -829,7 +835,7 @@ static cudaError_t attn_launch(Kv4Attn &x, const Kv4Planes &c, void *scratch, in
     const int64_t segments = (int64_t)x.n_tok * c.n_kv * passes;
     const int64_t tiles = segments * (((most < c.n_ctx ? most : c.n_ctx) + Cfg::TILE - 1) / Cfg::TILE);
     if (tiles + KA_PART * segments > (1ll << 30)) return cudaErrorInvalidValue;  // list positions are 32-bit
-    const int64_t want = segments + (tiles + KA_WARPS - 1) / KA_WARPS, cap = (int64_t)Cfg::CTAS * sm_count;
+    const int64_t want = segments + (tiles + Cfg::WARPS - 1) / Cfg::WARPS, cap = (int64_t)Cfg::CTAS * sm_count;
     Kv4AttnArgs a;
     a.q = x.q, a.k = x.k, a.v = x.v, a.out = x.out;
     a.q_ld = x.q_ld, a.kv_ld = x.kv_ld, a.out_ld = x.out_ld;
@@ -838,7 +844,7 @@ static cudaError_t attn_launch(Kv4Attn &x, const Kv4Planes &c, void *scratch, in
     a.arrived = (int *)scratch;
     a.part = kv4_scratch_parts(scratch, sm_count);
     a.err = err;
-    return launch_k(kv4_attn_kernel<HD, T>, dim3((unsigned)(want < cap ? want : cap)), dim3(KA_THREADS),
+    return launch_k(kv4_attn_kernel<HD, T>, dim3((unsigned)(want < cap ? want : cap)), dim3(Cfg::THREADS),
                     (size_t)Cfg::SMEM, st, a, c);
 }
 
