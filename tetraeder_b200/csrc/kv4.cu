@@ -31,47 +31,49 @@ __device__ __forceinline__ bool kv4_place(const Kv4RowArgs &a, int64_t i, int &s
     return true;
 }
 
-// Rows are independent and only moved once: HBM-bound.  A thread takes 8 values (a block is 4 threads,
-// its extremes two shuffles each way), so that a warp reads whole 128-byte lines and writes 8 blocks'
-// chunks; rows run fastest over the threads, so that a run of positions writes one contiguous piece of a
+// Rows are independent and only moved once: HBM-bound, if the codes cost few instructions.  A thread takes 16
+// values (a block is two threads, its extremes one shuffle each), so that a warp reads whole 128-byte
+// lines; rows run fastest over the threads, so that a run of positions writes one contiguous piece of a
 // head's plane.
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowArgs a) {
     const Kv4Planes &c = a.c;
-    constexpr int TPR = HD / 8, NB = HD / 32;
+    constexpr int TPR = HD / 16, NB = HD / 32;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t i = at / TPR;
-    const int sub = (int)(at % TPR), b = sub >> 2;
+    const int sub = (int)(at % TPR), b = sub >> 1;
     const int g = blockIdx.y >> 1;
     const bool is_v = blockIdx.y & 1;
     pdl_wait();
     pdl_trigger();
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    float x[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) x[j] = 0.0f;
     int s = 0, p = 0;
     const bool ok = i < a.n && kv4_place(a, i, s, p);
-    if (ok) kv4_load_row(reinterpret_cast<const T *>(is_v ? a.v : a.k) + i * a.ld + (int64_t)g * HD + 8 * sub, x);
-    float hi = -FLT_MAX, lo = FLT_MAX;
+    if (ok) kv4_load_row(reinterpret_cast<const T *>(is_v ? a.v : a.k) + i * a.ld + (int64_t)g * HD + 16 * sub, x);
+    // NaN and infinity have the largest exponent: seldom there
+    uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        x[j] = kv4_finite(x[j]);
-        hi = fmaxf(hi, x[j]), lo = fminf(lo, x[j]);
-    }
+    for (int j = 0; j < 16; j++) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+    if (top >= 0x7f800000u) {
 #pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        for (int j = 0; j < 16; j++) x[j] = kv4_finite(x[j]);
     }
+    float hi = x[0], lo = x[0];
+#pragma unroll
+    for (int j = 1; j < 16; j++) hi = fmaxf(hi, x[j]), lo = fminf(lo, x[j]);
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
     __half d;
     float inv;
     kv4_scale(hi, lo, d, inv);
-    uint32_t w = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) w |= kv4_code(x[j], inv) << (4 * j);
     if (!ok) return;
     const int64_t row = ((int64_t)s * c.n_kv + g) * c.n_ctx + p;
     uint8_t *codes = (is_v ? c.vc : c.kc) + row * (HD / 2);
-    *reinterpret_cast<uint32_t *>(codes + 16 * (b ^ kv4_turn<HD>(p)) + 4 * (sub & 3)) = w;
-    if ((sub & 3) == 0) (is_v ? c.vs : c.ks)[row * NB + b] = d;
+    *reinterpret_cast<uint2 *>(codes + 16 * (b ^ kv4_turn<HD>(p)) + 8 * (sub & 1)) =
+        make_uint2(kv4_word<8>(x, inv), kv4_word<8>(x + 8, inv));
+    if ((sub & 1) == 0) (is_v ? c.vs : c.ks)[row * NB + b] = d;
 }
 
 template <int HD, typename T>
@@ -485,9 +487,7 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4>::THREADS), (Kv
                             __half d;
                             float inv;
                             kv4_scale(hi, lo, d, inv);
-                            uint32_t w = 0;
-#pragma unroll
-                            for (int i = 0; i < 4; i++) w |= kv4_code(x[i], inv) << (4 * i);
+                            const uint32_t w = kv4_word<4>(x, inv);
                             if (lane < LANES) {
                                 const int byte = 16 * (b ^ kv4_turn<HD>(p_tok)) + 2 * (lane & 7);
                                 *reinterpret_cast<uint16_t *>(stage_p + (kv ? Cfg::VCODES : 0) + r * (HD / 2) + byte) =
@@ -793,7 +793,7 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4>::THREADS), (Kv
 template <int HD, typename T>
 static cudaError_t rows_launch(bool store, void *k, void *v, int64_t ld, const int32_t *seq, int seq0,
                                const int32_t *pos, int pos0, int64_t n, const Kv4Planes &c, int *err, cudaStream_t st) {
-    const dim3 grid((unsigned)((n * (HD / 8) + 255) / 256), 2 * c.n_kv);
+    const dim3 grid((unsigned)((n * (HD / (store ? 16 : 8)) + 255) / 256), 2 * c.n_kv);
     const Kv4RowArgs a{k, v, ld, n, seq, pos, seq0, pos0, c, err};
     return launch_k(store ? kv4_store_kernel<HD, T> : kv4_load_kernel<HD, T>, grid, dim3(256), 0, st, a);
 }

@@ -47,8 +47,19 @@ __device__ __forceinline__ void kv4_scale(float hi, float lo, __half &d16, float
     d16 = __float2half_rn(d);
     inv = (__half_as_ushort(d16) & 0x7fffu) == 0 ? 0.0f : __fdiv_rn(1.0f, d);
 }
-__device__ __forceinline__ uint32_t kv4_code(float x, float inv) {
-    return (uint32_t)fminf(fmaxf(floorf(__fadd_rn(__fmul_rn(x, inv), 8.5f)), 0.0f), 15.0f);
+// floor(x inv + 8.5) within 0 .. 15 in the low bits of a float of 2^23's exponent: adding 2^23 downwards leaves the
+// floor there, at full rate, where the conversion and floor instructions run at a quarter of it.
+__device__ __forceinline__ uint32_t kv4_code_bits(float x, float inv) {
+    const float t = fminf(fmaxf(__fadd_rn(__fmul_rn(x, inv), 8.5f), 0.0f), 15.5f);
+    return __float_as_uint(__fadd_rd(t, 8388608.0f));
+}
+// The codes of N <= 8 values as a word, the first in the low bits
+template <int N>
+__device__ __forceinline__ uint32_t kv4_word(const float *x, float inv) {
+    uint32_t w = 0, base = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) w += kv4_code_bits(x[i], inv) << (4 * i), base += 0x4b000000u << (4 * i);
+    return w - base;
 }
 
 // N consecutive activations as f32 (N a multiple of 4; 16-byte aligned, or 8 for four bf16).
