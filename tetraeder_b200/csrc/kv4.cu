@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
         const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + 16 * (b ^ kv4_turn<HD>(p)) + 4 * (sub & 3));
         const float d = __half2float((is_v ? c.vs : c.ks)[row * NB + b]);
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = d * (float)((int)((w >> (4 * j)) & 15u) - 8);
+        for (int j = 0; j < 8; j++) x[j] = d * (__uint_as_float(0x4b000000u | ((w >> (4 * j)) & 15u)) - 8388616.0f);
     }
     kv4_store_row(reinterpret_cast<T *>(is_v ? a.v : a.k) + i * a.ld + (int64_t)g * HD + 8 * sub, x);
 }
