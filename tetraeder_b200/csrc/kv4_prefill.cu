@@ -33,41 +33,13 @@ constexpr int KP_ROWS = 2 * KP_M;    // of a CTA
 constexpr int KP_N = 128;            // positions of a tile
 constexpr int KP_THREADS = 640;
 // Registers per thread: the softmax warps take what the others give back (5 * 96 at launch)
-constexpr int KP_REGS_SOFTMAX = 152, KP_REGS_DEQUANT = 64, KP_REGS_ISSUE = 48;
+constexpr int KP_REGS_SOFTMAX = 144, KP_REGS_DEQUANT = 64, KP_REGS_ISSUE = 64;
 static_assert(2 * KP_REGS_SOFTMAX + 2 * KP_REGS_DEQUANT + KP_REGS_ISSUE <= 5 * 96, "the block's registers");
 constexpr int KP_RAW = 3;            // raw tiles (of K or of V) in flight
+constexpr int KP_UNITS = 8, KP_UNITS1 = 5, KP_UNITS_BLOCK = 20;  // work of a tile of positions, of a block (see KpItem)
 constexpr float KP_BIAS = 6.0f;      // P is 2^KP_BIAS at the reference
 constexpr float KP_MOST = 16384.0f;  // a half tile's sum of P above which the row's reference moves
 constexpr float KP_SCALE_MAX = 8188.0f;  // 8 * this is f16's largest
-
-struct Kv4PrefillArgs {
-    const void *q;
-    void *out;
-    int64_t q_ld, out_ld;
-    int seq, pos0, n_tok, n_head, window, n_sink, splits;
-    float scale;
-    float *part;  // splits > 1: [cta] of O as [HD / 4][KP_ROWS][4], then the references and sums as [2][KP_ROWS]
-    int *err;
-};
-
-template <int HD>
-struct Kv4PrefillCfg {
-    static constexpr int NB = HD / 32, HALVES = HD / 64;  // 64-wide halves of a row: 128 bytes of f16
-    static constexpr int HALF = KP_N * 128;               // bytes of a half tile
-    static constexpr int TILE = HALVES * HALF;
-    static constexpr int CODES = KP_N * HD / 2, SCALES = KP_N * NB * 2, RAW = CODES + SCALES;
-    static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, R = V + 2 * TILE, BARS = R + KP_RAW * RAW;
-    static constexpr int SMEM = BARS + 256 + 1024 /* alignment */;
-};
-
-struct KpBars {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], raw_empty[KP_RAW], s_full[2],
-        p_full[2][2], o_half[2], o_full[2];
-    // a slot holds K and V by turns; each of the two has its own barrier of it, so that its readers see every phase
-    uint64_t raw_full[2][KP_RAW];
-    uint32_t tmem;
-};
-static_assert(sizeof(KpBars) <= 256, "barrier room");
 
 // Which positions the tokens t0 .. t1 see between them, as tiles of KP_N (see Kv4Seen).
 __host__ __device__ __forceinline__ Kv4Seen kp_seen(int pos0, int t0, int t1, int window, int n_sink) {
@@ -80,6 +52,93 @@ __host__ __device__ __forceinline__ Kv4Seen kp_seen(int pos0, int t0, int t1, in
     s.tiles = s.head + (s.len + KP_N - 1) / KP_N - s.body;
     return s;
 }
+
+// A run's first block, where the run begins inside it: its rows' place and the first and last of the runs that share it
+struct KpCut {
+    int blk, g, first, last;  // first < 0: no such block
+};
+struct Kv4PrefillArgs {
+    const void *q;
+    void *out;
+    int64_t q_ld, out_ld;
+    int seq, pos0, n_tok, window, n_sink;
+    int group, blocks;       // query heads of a KV head; blocks of KP_ROWS rows of one
+    uint64_t group_inv;      // floor((2^64 - 1) / group) + 1, or 0 for a group of 1
+    int64_t head_units;      // a KV head's work (see KpItem)
+    float scale;
+    KpCut *cuts;  // [cta]
+    float *part;  // [cta][head, tail of its run] of O as [HD / 4][KP_ROWS][4], then the references and sums as [2][KP_ROWS]
+    int *err;
+    // row / group, exact for rows below 2^32
+    __device__ __forceinline__ int token(int row) const { return group_inv ? (int)__umul64hi((uint64_t)row, group_inv) : row; }
+};
+
+// A value that all lanes have alike
+__device__ __forceinline__ int kp_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// The work is one list: KV head by KV head, block by block, tile by tile.  A block costs KP_UNITS_BLOCK, then a tile
+// KP_UNITS (KP_UNITS1 where there are no rows in B).  Every CTA takes an even run of the list, so a block may be cut: its pieces
+// go to `part` and kv4_join_kernel adds them.
+struct KpItem {
+    int g, blk, s;  // s: the block's first unit, from the run's first
+    int row0, n_rows, tiles, tile0, n;
+    Kv4Seen seen;
+    __device__ __forceinline__ int mt() const { return n_rows > KP_M ? 2 : 1; }
+    __device__ __forceinline__ bool whole() const { return n == tiles; }
+    __device__ __forceinline__ int tiles_before(int units) const {  // tiles that begin before the block's first `units`
+        const int u = units - KP_UNITS_BLOCK;
+        return u <= 0 ? 0 : min(tiles, mt() == 2 ? (u + KP_UNITS - 1) / KP_UNITS : (u + KP_UNITS1 - 1) / KP_UNITS1);
+    }
+    __device__ __forceinline__ int units() const { return KP_UNITS_BLOCK + tiles * (mt() == 2 ? KP_UNITS : KP_UNITS1); }
+    // The part of this block in a run of `len` units: tiles tile0 .. tile0 + n - 1 of `tiles`; false: beyond the run
+    __device__ __forceinline__ bool in_run(const Kv4PrefillArgs &a, int len) {
+        if (s >= len) return false;
+        row0 = blk * KP_ROWS, n_rows = min(KP_ROWS, a.n_tok * a.group - row0);
+        seen = kp_seen(a.pos0, a.token(row0), a.token(row0 + n_rows - 1), a.window, a.n_sink);
+        tiles = seen.tiles;
+        tile0 = tiles_before(-s), n = tiles_before(len - s) - tile0;
+        return true;
+    }
+    // The same by a whole warp, the results in uniform registers: what depends on them (branches, descriptors) is the
+    // warp's then, not each lane's, and costs less
+    __device__ __forceinline__ bool in_run_warp(const Kv4PrefillArgs &a, int len) {
+        if (!__any_sync(0xffffffffu, in_run(a, len))) return false;
+        for (int *x : {&g, &blk, &s, &row0, &n_rows, &tiles, &tile0, &n, &seen.len, &seen.from, &seen.head, &seen.body})
+            *x = kp_uniform(*x);
+        return true;
+    }
+    __device__ __forceinline__ void next(const Kv4PrefillArgs &a) {
+        s += units();
+        if (++blk == a.blocks) blk = 0, g++;
+    }
+};
+// The run that holds a unit, of `ctas` runs that begin at total * cta / ctas
+__device__ __forceinline__ int kp_run_of(int64_t unit, int64_t total, int ctas) {
+    return (int)(((unit + 1) * ctas - 1) / total);
+}
+
+template <int HD>
+struct Kv4PrefillCfg {
+    static constexpr int NB = HD / 32, HALVES = HD / 64;  // 64-wide halves of a row: 128 bytes of f16
+    static constexpr int HALF = KP_N * 128;               // bytes of a half tile
+    static constexpr int TILE = HALVES * HALF;
+    static constexpr int CODES = KP_N * HD / 2, SCALES = KP_N * NB * 2, RAW = CODES + SCALES;
+    static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, R = V + 2 * TILE, CS = R + KP_RAW * RAW, BARS = CS + KP_ROWS * 4;
+    static constexpr int SMEM = BARS + 1024;
+    static constexpr int64_t PART = KP_ROWS * (HD + 2);  // floats of a piece
+};
+
+struct KpBars {
+    uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], raw_empty[KP_RAW], s_full[2],
+        p_full[2][2], o_half[2], o_full[2];
+    // a slot holds K and V by turns; each of the two has its own barrier of it, so that its readers see every phase
+    uint64_t raw_full[2][KP_RAW];
+    uint32_t tmem;
+    int g, blk, s, len;  // the run: its first block, that one's first unit from the run's first, its units
+    KpCut cut;
+    KpItem item[8];  // the softmax warps'
+};
+static_assert(sizeof(KpBars) <= 1024, "barrier room");
 
 // Four f16 pairs d (c - 8) of a word of codes: values (0, 4), (1, 5), (2, 6), (3, 7).
 __device__ __forceinline__ uint4 kp_word(uint32_t w, __half2 d) {
@@ -132,23 +191,18 @@ template <int HD, typename T>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4PrefillArgs a, const Kv4Planes c) {
     using Cfg = Kv4PrefillCfg<HD>;
     constexpr int NB = Cfg::NB;
-    extern __shared__ uint8_t kp_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(kp_raw) + 1023) & ~(uintptr_t)1023);
+    extern __shared__ __align__(1024) uint8_t smem[];  // as declared, so that addresses in it are constants
+    if (smem_u32(smem) & 1023) {  // the swizzle needs it
+        if (threadIdx.x == 0) latch_error(a.err, TMOE_DEV_ERR_TIMEOUT);
+        return;
+    }
     KpBars &bars = *reinterpret_cast<KpBars *>(smem + Cfg::BARS);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-    // ---- which rows and which tiles; the longest runs (the last tokens) come first
-    const int G = a.n_head / c.n_kv, rows = a.n_tok * G, blocks = (rows + KP_ROWS - 1) / KP_ROWS;
-    const int sp = blockIdx.x % a.splits, g = (blockIdx.x / a.splits) % c.n_kv;
-    const int blk = blocks - 1 - blockIdx.x / (a.splits * c.n_kv);
-    const int row0 = blk * KP_ROWS, n_rows = min(KP_ROWS, rows - row0);
-    const int mt = n_rows > KP_M ? 2 : 1;
-    const Kv4Seen seen = kp_seen(a.pos0, row0 / G, (row0 + n_rows - 1) / G, a.window, a.n_sink);
-    const int tile0 = (int)((int64_t)seen.tiles * sp / a.splits), n = (int)((int64_t)seen.tiles * (sp + 1) / a.splits) - tile0;
+    const int warp = kp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        mbar_init(&bars.q_full, 4 * mt);
         for (int i = 0; i < 2; i++) {
+            mbar_init(&bars.q_full[i], 4);
+            mbar_init(&bars.q_empty[i], 1 + 4);
             mbar_init(&bars.k_full[i], 4);
             mbar_init(&bars.k_empty[i], 1);
             mbar_init(&bars.v_full[i], 4);
@@ -167,87 +221,83 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
         fence_barrier_init();
     }
     if (warp == 16) tc::alloc(&bars.tmem, 512);
+    if (warp == 17) {
+        // the run, by a scan over a head's blocks
+        const int64_t total = a.head_units * c.n_kv, u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
+        const int g = (int)(u0 / a.head_units);
+        const int64_t off = u0 - g * a.head_units;
+        int64_t before = 0;  // units of the blocks before
+        for (int b0 = 0; b0 < a.blocks; b0 += 32) {
+            KpItem x;
+            x.g = g, x.blk = b0 + lane, x.s = 0;
+            int units = 0;
+            if (x.blk < a.blocks) {
+                x.in_run(a, 1);
+                units = x.units();
+            }
+            int64_t end = units;
+#pragma unroll
+            for (int i = 1; i < 32; i <<= 1) {
+                const int64_t v = __shfl_up_sync(0xffffffffu, end, i);
+                if (lane >= i) end += v;
+            }
+            end += before;
+            const unsigned found = __ballot_sync(0xffffffffu, end > off);
+            if (found) {
+                if (lane == __ffs(found) - 1) {
+                    const int64_t at = g * a.head_units + end - units;  // the block's first unit
+                    bars.g = g, bars.blk = x.blk, bars.s = (int)(at - u0), bars.len = (int)(u1 - u0);
+                    x.s = bars.s;
+                    x.in_run(a, bars.len);
+                    const int w = x.mt() == 2 ? KP_UNITS : KP_UNITS1, ctas = (int)gridDim.x;
+                    const bool cut = x.tile0 > 0 && x.n > 0;
+                    bars.cut = KpCut{x.blk, g, cut ? kp_run_of(at + KP_UNITS_BLOCK, total, ctas) : -1,
+                                     kp_run_of(at + KP_UNITS_BLOCK + (int64_t)(x.tiles - 1) * w, total, ctas)};
+                }
+                break;
+            }
+            before = __shfl_sync(0xffffffffu, end, 31);
+        }
+    }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = bars.tmem;
+    KpItem it;
+    it.g = bars.g, it.blk = bars.blk, it.s = bars.s;
+    const int len = bars.len;
+    float *cs_smem = reinterpret_cast<float *>(smem + Cfg::CS);  // [KP_ROWS]
     pdl_wait();
     pdl_trigger();
+    if (threadIdx.x == 17 * 32) a.cuts[blockIdx.x] = bars.cut;
 
     if (warp < 8) {
         tc::more_registers<KP_REGS_SOFTMAX>();
-        // ------------------------------------------------------------ Q, then the softmax: a thread per row
-        const int m = warp >> 2;
-        if (m < mt) {
-            // The warp's 32 rows into the operand's layout, a thread per row: bf16 by asynchronous copies, all in flight,
-            // and then in place; f32 read twice.  Loops stay rolled: their code is fetched anew by every CTA.
-            uint8_t *q_tile = smem + Cfg::Q + m * Cfg::TILE;
-            auto chunk = [&](int r, int ch) { return q_tile + (ch >> 3) * Cfg::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
-            const int my_r = (warp & 3) * 32 + lane, my_row = min(row0 + m * KP_M + my_r, rows - 1);
-            const T *my_q = reinterpret_cast<const T *>(a.q) + (int64_t)(my_row / G) * a.q_ld + (int64_t)(g * G + my_row % G) * HD;
-            constexpr int CH = HD / 8;
-            float top = 0.0f;
-            if constexpr (sizeof(T) == 2) {
-#pragma unroll 4
-                for (int i = 0; i < 32; i += 32 / CH) {
-                    const int src = i + lane / CH, ch = lane % CH;
-                    const T *p = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, (unsigned long long)my_q, src)) + 8 * ch;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(chunk((warp & 3) * 32 + src, ch))), "l"(p)
-                                 : "memory");
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                __syncwarp();
-#pragma unroll 2
-                for (int ch = 0; ch < CH; ch++) {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(chunk(my_r, ch));
-                    // magnitudes of bf16 order as their bits
-                    const uint32_t h = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu),
-                                                __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
-                    top = fmaxf(top, fmaxf(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)));
-                }
-            } else {
-#pragma unroll 2
-                for (int ch = 0; ch < CH; ch++) {
-                    float x[8];
-                    kv4_load_row(my_q + 8 * ch, x);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
-                }
-            }
-            // 2^e * top in [2^5, 2^6): exact for bf16 values down to 2^-22 of the largest
-            const int e = top > 0.0f && top <= FLT_MAX ? 5 - ilogbf(top) : 0;
-            const int e1 = e / 2, e2 = e - e1;
-            const float up1 = kv4_pow2(e1), up2 = kv4_pow2(e2);
-#pragma unroll 2
-            for (int ch = 0; ch < CH; ch++) {
-                uint4 *dst = reinterpret_cast<uint4 *>(chunk(my_r, ch));
-                float x[8];
-                if constexpr (sizeof(T) == 2) {
-                    const uint4 u = *dst;
-                    kv4_bf2(u.x, x[0], x[1]), kv4_bf2(u.y, x[2], x[3]), kv4_bf2(u.z, x[4], x[5]), kv4_bf2(u.w, x[6], x[7]);
-                } else {
-                    kv4_load_row(my_q + 8 * ch, x);
-                }
-#pragma unroll
-                for (int v = 0; v < 8; v++) x[v] = x[v] * up1 * up2;
-                *dst = make_uint4(kv4_half2(x[0], x[4]), kv4_half2(x[1], x[5]), kv4_half2(x[2], x[6]), kv4_half2(x[3], x[7]));
-            }
-            // log2 score of an accumulator's 1; never 0: masked scores are -inf times it
-            const float cs = fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(-e1) * kv4_pow2(-e2), FLT_MIN);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        // ------------------------------------------------------------ the softmax: a thread per row
+        const int m = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + m * KP_N + lanes, to = tmem + 256 + m * HD + lanes;
+        int nt = 0, items = 0;  // tiles and blocks before
+        for (; it.in_run_warp(a, len); it.next(a)) {
+            if (it.n == 0 || m >= it.mt()) continue;
+            KP_WAIT_WARP(bars.q_full[m], items & 1);
+            const float cs = cs_smem[m * KP_M + r];
+            const int t = a.pos0 + a.token(min(it.row0 + m * KP_M + r, it.row0 + it.n_rows - 1));  // the row's position
+            const int row_lo = it.row0 + m * KP_M, row_hi = min(row_lo + KP_M, it.row0 + it.n_rows) - 1;
+            // the tile's first and last position, and the last positions before their windows
+            const int t_lo = kp_uniform(a.pos0 + a.token(row_lo)), t_hi = kp_uniform(a.pos0 + a.token(row_hi));
+            const int w_lo = a.window > 0 ? t_lo - a.window : -1, w_hi = a.window > 0 ? t_hi - a.window : -1;
+            if (lane == 0) bars.item[warp] = it;  // out of the registers while the tiles are worked on
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.q_full);
-
-            const int r = my_r, row = row0 + m * KP_M + r;
-            const int t = a.pos0 + min(row, rows - 1) / G;  // the row's position
-            const int t_lo = a.pos0 + (row0 + m * KP_M) / G, t_hi = a.pos0 + min(row0 + (m + 1) * KP_M - 1, rows - 1) / G;
-            const int w_lo = a.window > 0 ? t - a.window : -1;  // positions above it are in the window
-            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            const uint32_t ts = tmem + m * KP_N + lanes, to = tmem + 256 + m * HD + lanes;
+            if (lane == 0) mbar_arrive(&bars.q_empty[m]);
             float ref = -INFINITY, l = 0.0f;
-            // P of 32 columns of S against a reference (exponents s c + r), and its sum; positions from k0 on
-            auto exps = [&](const uint32_t (&s)[32], uint32_t *p, uint64_t c2, uint64_t r2, uint64_t (&sum)[2], int k0, auto masked) {
+            // which of the positions k0 .. k0 + 31 the row sees: those up to its own, of them the window's and the sinks
+            auto sees32 = [&](int k0) {
+                auto below = [](int x) { return (uint32_t)((1ull << min(max(x, 0), 32)) - 1); };
+                return below(t + 1 - k0) & (a.window > 0 ? ~below(t - a.window + 1 - k0) | below(a.n_sink - k0) : ~0u);
+            };
+            // P of 32 columns of S against a reference (exponents s c + r), and its sum
+            auto exps = [&](const uint32_t (&s)[32], uint32_t *p, uint64_t c2, uint64_t r2, uint64_t (&sum)[2], uint32_t see, auto masked) {
                 // by stages over all 32: a group at a time would wait for each result
                 uint64_t x[16];
 #pragma unroll
@@ -255,10 +305,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                     uint32_t v[2] = {s[2 * i], s[2 * i + 1]};
                     if constexpr (decltype(masked)::value) {
 #pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const int k = k0 + 2 * i + u;
-                            if (k > t || (k <= w_lo && k >= a.n_sink)) v[u] = 0xff800000u;  // -inf
-                        }
+                        for (int u = 0; u < 2; u++)
+                            if (!(see & (1u << (2 * i + u)))) v[u] = 0xff800000u;  // -inf
                     }
                     x[i] = tc::fma2(tc::pair(__uint_as_float(v[0]), __uint_as_float(v[1])), c2, r2);
                 }
@@ -272,238 +320,394 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 }
             };
             uint32_t s0[32], s1[32], p[32];  // 64 columns of S, and their P
+            int left = it.n, k_tile = it.seen.tile(it.tile0) * KP_N;
+            int sinks = it.seen.head - it.tile0;  // tiles to the last of the sinks'
+            const int k_body = it.seen.body * KP_N;
+            bool fresh = true;  // there is a row without a reference
 #pragma unroll 1
-            for (int j = 0; j < n; j++) {
-                KP_WAIT_WARP(bars.s_full[m], j & 1);
+            for (; left > 0; left--, nt++) {
+                // settled before the wait, so that it is not on the way from S to P
+                const bool whole = k_tile + KP_N - 1 <= t_lo && (k_tile > w_hi || k_tile + KP_N <= a.n_sink);
+                KP_WAIT_WARP(bars.s_full[m], nt & 1);
                 tc::fence_after();
                 tc::ld32(ts, s0);
                 // In halves of 64 positions, so that the first one's product runs beside the second's exps; half of the
                 // next 64 columns is read while the second half of these is worked on
 #pragma unroll 1
                 for (int hf = 0; hf < 2; hf++) {
-                    const int k0 = seen.tile(tile0 + j) * KP_N + 64 * hf;
-                    const bool whole = k0 + 63 <= t_lo && (a.window == 0 || k0 > t_hi - a.window || k0 + 64 <= a.n_sink);
+                    const int k0 = k_tile + 64 * hf;
                     const uint32_t th = ts + 64 * hf;
                     tc::ld32(th + 32, s1);
                     tc::wait_ld(s0);
                     tc::wait_ld(s1);
-                    float sum;
-                    bool raise = __any_sync(0xffffffffu, ref == -INFINITY);
+                    if (!whole && (k0 > t_hi || (k0 + 63 <= w_lo && k0 >= a.n_sink))) {  // no row sees any
+#pragma unroll
+                        for (int i = 0; i < 32; i++) p[i] = 0;
+                        if (!hf) tc::ld32(ts + 64, s0);
+                    } else {
+                        bool raise = fresh;
+                        float sum;
 #pragma unroll 1
-                    for (int tries = 0; tries < 2; tries++) {
-                        if (raise) {
-                            tries = 1;
-                            float mx = -INFINITY;
-#pragma unroll 1
-                            for (int ch = 0; ch < 64; ch += 32) {
-                                tc::ld32(th + ch, s0);
-                                tc::wait_ld(s0);
+                        for (int again = 0;; again = 1) {
+                            if (raise) {
+                                if (again) {
+                                    tc::wait_ld(s0);
+                                    tc::ld32(th, s0);
+                                    tc::ld32(th + 32, s1);
+                                    tc::wait_ld(s0);
+                                    tc::wait_ld(s1);
+                                }
+                                float mx = -INFINITY;
+                                const uint32_t see0 = sees32(k0), see1 = sees32(k0 + 32);
 #pragma unroll
                                 for (int i = 0; i < 32; i++) {
-                                    const int k = k0 + ch + i;
-                                    if (k <= t && (k > w_lo || k < a.n_sink)) mx = fmaxf(mx, __uint_as_float(s0[i]));
+                                    mx = fmaxf(mx, see0 & (1u << i) ? __uint_as_float(s0[i]) : -INFINITY);
+                                    mx = fmaxf(mx, see1 & (1u << i) ? __uint_as_float(s1[i]) : -INFINITY);
                                 }
-                            }
-                            const float next = fmaxf(ref, mx * cs);
-                            const float f = ref == -INFINITY ? 0.0f : kv4_exp2(ref - next);
-                            ref = next;
-                            l *= f;
-                            if (hf) {  // the first half's product has to be in O
-                                KP_WAIT_WARP(bars.o_half[m], j & 1);
-                                tc::fence_after();
-                            }
-                            if (j > 0 || hf) {
+                                const float next = fmaxf(ref, mx * cs);
+                                const float f = ref == -INFINITY ? 0.0f : kv4_exp2(ref - next);
+                                ref = next;
+                                l *= f;
+                                if (hf) {  // the first half's product has to be in O
+                                    KP_WAIT_WARP(bars.o_half[m], nt & 1);
+                                    tc::fence_after();
+                                }
+                                if (left < bars.item[warp].n || hf) {
 #pragma unroll 1
-                                for (int ch = 0; ch < HD; ch += 32) {
-                                    tc::ld32(to + ch, s0);
-                                    tc::wait_ld(s0);
+                                    for (int ch = 0; ch < HD; ch += 32) {
+                                        tc::ld32(to + ch, p);
+                                        tc::wait_ld(p);
 #pragma unroll
-                                    for (int i = 0; i < 32; i++) s0[i] = __float_as_uint(__uint_as_float(s0[i]) * f);
-                                    tc::st32(to + ch, s0);
+                                        for (int i = 0; i < 32; i++) p[i] = __float_as_uint(__uint_as_float(p[i]) * f);
+                                        tc::st32(to + ch, p);
+                                    }
                                 }
                             }
-                            tc::ld32(th, s0);
-                            tc::ld32(th + 32, s1);
-                            tc::wait_ld(s0);
-                            tc::wait_ld(s1);
+                            const float neg_ref = KP_BIAS - (ref == -INFINITY ? 0.0f : ref);
+                            const uint64_t c2 = tc::pair(cs, cs), r2 = tc::pair(neg_ref, neg_ref);
+                            uint64_t sums[2] = {0, 0};
+                            if (whole)
+                                exps(s0, p, c2, r2, sums, ~0u, KpNo{});
+                            else
+                                exps(s0, p, c2, r2, sums, sees32(k0), KpYes{});
+                            if (!hf) tc::ld32(ts + 64, s0);
+                            if (whole)
+                                exps(s1, p + 16, c2, r2, sums, ~0u, KpNo{});
+                            else
+                                exps(s1, p + 16, c2, r2, sums, sees32(k0 + 32), KpYes{});
+                            const float2 x = tc::unpair(tc::add2(sums[0], sums[1]));
+                            sum = x.x + x.y;
+                            if (raise) break;
+                            raise = __any_sync(0xffffffffu, sum > KP_MOST);
+                            if (!raise) break;
                         }
-                        const float neg_ref = KP_BIAS - (ref == -INFINITY ? 0.0f : ref);
-                        const uint64_t c2 = tc::pair(cs, cs), r2 = tc::pair(neg_ref, neg_ref);
-                        uint64_t sums[2] = {0, 0};
-                        if (whole)
-                            exps(s0, p, c2, r2, sums, k0, KpNo{});
-                        else
-                            exps(s0, p, c2, r2, sums, k0, KpYes{});
-                        if (!hf) tc::ld32(ts + 64, s0);
-                        if (whole)
-                            exps(s1, p + 16, c2, r2, sums, k0 + 32, KpNo{});
-                        else
-                            exps(s1, p + 16, c2, r2, sums, k0 + 32, KpYes{});
-                        const float2 x = tc::unpair(tc::add2(sums[0], sums[1]));
-                        sum = x.x + x.y;
-                        raise = __any_sync(0xffffffffu, sum > KP_MOST);
-                        if (!raise) break;
-                        tc::wait_ld(s0);
+                        l += sum;
+                        if (fresh) fresh = __any_sync(0xffffffffu, ref == -INFINITY);
                     }
-                    l += sum;
                     tc::st32(th, p);
                     tc::wait_st();
                     tc::fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.p_full[m][hf]);
                 }
+                k_tile = --sinks == 0 ? k_body : k_tile + KP_N;
             }
             // ---- the rows' results
-            float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            it = bars.item[warp];
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int row = row_lo + r;
             float *part = nullptr;
-            if (a.splits > 1) {  // O as it is, rows side by side
-                part = a.part + (int64_t)blockIdx.x * KP_ROWS * (HD + 2) + (m * KP_M + r) * 4;
-                float *stats = a.part + (int64_t)blockIdx.x * KP_ROWS * (HD + 2) + KP_ROWS * HD + m * KP_M + r;
-                stats[0] = ref, stats[KP_ROWS] = l;
+            if (!it.whole()) {  // O as it is, rows side by side
+                float *piece = a.part + (2 * (int64_t)blockIdx.x + (it.tile0 > 0 ? 0 : 1)) * Cfg::PART;
+                part = piece + (m * KP_M + r) * 4;
+                float *stats = piece + KP_ROWS * HD + m * KP_M + r;
+                if (row <= row_hi) stats[0] = ref, stats[KP_ROWS] = l;
             }
-            if (n > 0) {
-                KP_WAIT_WARP(bars.o_full[m], 0);
-                tc::fence_after();
-                T *out = reinterpret_cast<T *>(a.out) + (int64_t)(row / G) * a.out_ld + (int64_t)(g * G + row % G) * HD;
+            const int tok = a.token(row);
+            const unsigned long long out =
+                reinterpret_cast<unsigned long long>(reinterpret_cast<T *>(a.out) + (int64_t)tok * a.out_ld +
+                                                     (int64_t)(it.g * a.group + row - tok * a.group) * HD);
+            KP_WAIT_WARP(bars.o_full[m], items & 1);
+            items++;
+            tc::fence_after();
 #pragma unroll 1
-                for (int ch = 0; ch < HD; ch += 32) {
-                    uint32_t o[32];
-                    tc::ld32(to + ch, o);
-                    tc::wait_ld(o);
-                    if (part) {
+            for (int ch = 0; ch < HD; ch += 32) {
+                uint32_t o[32];
+                tc::ld32(to + ch, o);
+                tc::wait_ld(o);
+                if (part) {
+                    if (row <= row_hi) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
                             *reinterpret_cast<uint4 *>(part + (ch + i) * KP_ROWS) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                    } else if (row < rows) {
+                    }
+                } else {
+                    // Column 2e of 8 is value e, column 2e + 1 value 4 + e.  Four lanes exchange 16-byte pieces so that each
+                    // store of theirs fills 64 bytes of one row.
+                    uint32_t y[sizeof(T) == 2 ? 16 : 32];
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            // column 2e of a chunk is value e, column 2e + 1 value 4 + e
-                            float x[8];
+                    for (int i = 0; i < 32; i += 8) {
+                        float x[8];
 #pragma unroll
-                            for (int v = 0; v < 4; v++)
-                                x[v] = __uint_as_float(o[i + 2 * v]) * inv, x[4 + v] = __uint_as_float(o[i + 2 * v + 1]) * inv;
-                            kv4_store_row(out + ch + i, x);
+                        for (int v = 0; v < 4; v++)
+                            x[v] = __uint_as_float(o[i + 2 * v]) * inv, x[4 + v] = __uint_as_float(o[i + 2 * v + 1]) * inv;
+#pragma unroll
+                        for (int v = 0; v < 8; v++) {
+                            if constexpr (sizeof(T) == 2) {
+                                if (v & 1) y[(i + v) / 2] = kv4_pack_bf2(x[v - 1], x[v]);
+                            } else {
+                                y[i + v] = __float_as_uint(x[v]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < (sizeof(T) == 2 ? 16 : 32); q += 16) {
+                        uint32_t *z = y + q;  // pieces z[4 i ..] of this row, then piece lane & 3 of rows i
+#pragma unroll
+                        for (int bit = 1; bit < 4; bit <<= 1) {
+                            const bool up = lane & bit;
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                if (i & bit) continue;
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    uint32_t &lo = z[4 * i + e], &hi = z[4 * (i | bit) + e];
+                                    const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, bit);
+                                    (up ? lo : hi) = got;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            char *dst = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, out, (lane & ~3) | i)) +
+                                        ch * sizeof(T) + q * 4 + 16 * (lane & 3);
+                            if ((row & ~3) + i <= row_hi)
+                                *reinterpret_cast<uint4 *>(dst) = make_uint4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
                         }
                     }
                 }
             }
+            tc::fence_before();
         }
     } else if (warp < 16) {
         tc::fewer_registers<KP_REGS_DEQUANT>();
         // ------------------------------------------------------------ dequantise: a thread per position
         const int r = threadIdx.x & 127;
         const bool is_v = warp >= 12;
+        const uint32_t smem0 = smem_u32(smem);
         const __half2 cap = __float2half2_rn(KP_SCALE_MAX), ncap = __float2half2_rn(-KP_SCALE_MAX);
-        for (int j = 0; j < n; j++) {
-            const int i = 2 * j + is_v, slot = j & 1, rs = i % KP_RAW;
-            uint8_t *dst = smem + (is_v ? Cfg::V : Cfg::K) + slot * Cfg::TILE;
-            KP_WAIT_WARP(bars.raw_full[is_v][rs], (j / KP_RAW) & 1);
-            if (j >= 2) KP_WAIT_WARP(is_v ? bars.v_empty[slot] : bars.k_empty[slot], ((j >> 1) - 1) & 1);
-            const uint8_t *raw = smem + Cfg::R + rs * Cfg::RAW;
-            const int pos = seen.tile(tile0 + j) * KP_N + r;
-            uint32_t sc[NB / 2];
+        const int m = is_v;  // the Q tile that this group loads: before its first tile of all, later after a block's first tile
+        int nt = 0, items = 0;
+        for (; it.in_run_warp(a, len); it.next(a)) {
+            if (it.n == 0) continue;
+            const int q_at = nt ? 1 : 0;
+#pragma unroll 1
+            for (int j = 0; j < it.n || j <= q_at; j++) {
+                if (j == q_at && m < it.mt()) {
+                    if (items > 0) KP_WAIT_WARP(bars.q_empty[m], (items - 1) & 1);
+                    // The warp's 32 rows into the operand's layout, a thread per row: bf16 by asynchronous copies, all in flight,
+                    // and then in place; f32 read twice.  Loops stay rolled: their code is fetched anew by every CTA.
+                    uint8_t *q_tile = smem + Cfg::Q + m * Cfg::TILE;
+                    auto chunk = [&](int r, int ch) { return q_tile + (ch >> 3) * Cfg::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
+                    const int my_row = min(it.row0 + m * KP_M + r, it.row0 + it.n_rows - 1), tok = a.token(my_row);
+                    const T *my_q = reinterpret_cast<const T *>(a.q) + (int64_t)tok * a.q_ld + (int64_t)(it.g * a.group + my_row - tok * a.group) * HD;
+                    constexpr int CH = HD / 8;
+                    float top = 0.0f;
+                    if constexpr (sizeof(T) == 2) {
+#pragma unroll 4
+                        for (int i = 0; i < 32; i += 32 / CH) {
+                            const int src = i + lane / CH, ch = lane % CH;
+                            const T *p = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, (unsigned long long)my_q, src)) + 8 * ch;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(chunk((warp & 3) * 32 + src, ch))), "l"(p)
+                                         : "memory");
+                        }
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        asm volatile("cp.async.wait_group 0;" ::: "memory");
+                        __syncwarp();
+#pragma unroll 2
+                        for (int ch = 0; ch < CH; ch++) {
+                            const uint4 u = *reinterpret_cast<const uint4 *>(chunk(r, ch));
+                            // magnitudes of bf16 order as their bits
+                            const uint32_t h = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu),
+                                                        __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
+                            top = fmaxf(top, fmaxf(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)));
+                        }
+                    } else {
+#pragma unroll 2
+                        for (int ch = 0; ch < CH; ch++) {
+                            float x[8];
+                            kv4_load_row(my_q + 8 * ch, x);
 #pragma unroll
-            for (int b = 0; b < NB / 2; b++) {
-                sc[b] = *reinterpret_cast<const uint32_t *>(raw + Cfg::CODES + (r * NB + 2 * b) * 2);
-                __half2 h;
-                memcpy(&h, &sc[b], 4);
-                h = __hmax2(__hmin2(h, cap), ncap);  // also keeps a NaN out
-                memcpy(&sc[b], &h, 4);
-                if (!seen.sees(pos, a.n_sink)) sc[b] = 0;  // a row that no query sees may hold anything
-            }
+                            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
+                        }
+                    }
+                    // 2^e * top in [2^5, 2^6): exact for bf16 values down to 2^-22 of the largest
+                    const int e = top > 0.0f && top <= FLT_MAX ? 5 - ilogbf(top) : 0;
+                    const int e1 = e / 2, e2 = e - e1;
+                    const float up1 = kv4_pow2(e1), up2 = kv4_pow2(e2);
+#pragma unroll 2
+                    for (int ch = 0; ch < CH; ch++) {
+                        uint4 *dst = reinterpret_cast<uint4 *>(chunk(r, ch));
+                        float x[8];
+                        if constexpr (sizeof(T) == 2) {
+                            const uint4 u = *dst;
+                            kv4_bf2(u.x, x[0], x[1]), kv4_bf2(u.y, x[2], x[3]), kv4_bf2(u.z, x[4], x[5]), kv4_bf2(u.w, x[6], x[7]);
+                        } else {
+                            kv4_load_row(my_q + 8 * ch, x);
+                        }
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(raw + r * (HD / 2) + 16 * (b ^ kv4_turn<HD>(r)));
-                __half2 d;
-                const uint32_t dd = __byte_perm(sc[b / 2], 0, b & 1 ? 0x3232 : 0x1010);
-                memcpy(&d, &dd, 4);
-                uint8_t *half = dst + (b >> 1) * Cfg::HALF + r * 128;
-                const int c0 = (b & 1) * 4;
-                *reinterpret_cast<uint4 *>(half + (((c0 + 0) ^ (r & 7)) << 4)) = kp_word(w.x, d);
-                *reinterpret_cast<uint4 *>(half + (((c0 + 1) ^ (r & 7)) << 4)) = kp_word(w.y, d);
-                *reinterpret_cast<uint4 *>(half + (((c0 + 2) ^ (r & 7)) << 4)) = kp_word(w.z, d);
-                *reinterpret_cast<uint4 *>(half + (((c0 + 3) ^ (r & 7)) << 4)) = kp_word(w.w, d);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&bars.raw_empty[rs]);
-                mbar_arrive(is_v ? &bars.v_full[slot] : &bars.k_full[slot]);
+                        for (int v = 0; v < 8; v++) x[v] = x[v] * up1 * up2;
+                        *dst = make_uint4(kv4_half2(x[0], x[4]), kv4_half2(x[1], x[5]), kv4_half2(x[2], x[6]), kv4_half2(x[3], x[7]));
+                    }
+                    // log2 score of an accumulator's 1; never 0: masked scores are -inf times it
+                    const float cs = fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(-e1) * kv4_pow2(-e2), FLT_MIN);
+                    cs_smem[m * KP_M + r] = cs;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.q_full[m]);
+                    items++;
+                }
+                if (j < it.n) {
+                    const int i = 2 * nt + is_v, slot = nt & 1, rs = i % KP_RAW;
+                    // 16-byte chunk c of row r lies at chunk c ^ (r & 7), so at `dst` ^ 16 c
+                    const uint32_t dst = smem0 + (is_v ? Cfg::V : Cfg::K) + slot * Cfg::TILE + r * 128 + (r & 7) * 16;
+                    const uint32_t raw = smem0 + Cfg::R + rs * Cfg::RAW, codes = raw + r * (HD / 2) + 16 * kv4_turn<HD>(r);
+                    KP_WAIT_WARP(bars.raw_full[is_v][rs], (nt / KP_RAW) & 1);
+                    if (nt >= 2) KP_WAIT_WARP(is_v ? bars.v_empty[slot] : bars.k_empty[slot], ((nt >> 1) - 1) & 1);
+                    const int pos = it.seen.tile(it.tile0 + j) * KP_N + r;
+                    const bool seen = it.seen.sees(pos, a.n_sink);  // a row that no query sees may hold anything
+                    uint32_t sc[NB / 2];
+#pragma unroll
+                    for (int b = 0; b < NB / 2; b++) {
+                        sc[b] = tc::lds32(raw + Cfg::CODES + (r * NB + 2 * b) * 2);
+                        __half2 h;
+                        memcpy(&h, &sc[b], 4);
+                        h = __hmax2(__hmin2(h, cap), ncap);  // also keeps a NaN out
+                        memcpy(&sc[b], &h, 4);
+                        if (!seen) sc[b] = 0;
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const uint4 w = tc::lds128(codes ^ (16 * b));
+                        __half2 d;
+                        const uint32_t dd = __byte_perm(sc[b / 2], 0, b & 1 ? 0x3232 : 0x1010);
+                        memcpy(&d, &dd, 4);
+                        const uint32_t to = dst + (b >> 1) * Cfg::HALF;
+                        const int c0 = (b & 1) * 4;
+                        tc::sts128(to ^ (16 * (c0 + 0)), kp_word(w.x, d));
+                        tc::sts128(to ^ (16 * (c0 + 1)), kp_word(w.y, d));
+                        tc::sts128(to ^ (16 * (c0 + 2)), kp_word(w.z, d));
+                        tc::sts128(to ^ (16 * (c0 + 3)), kp_word(w.w, d));
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&bars.raw_empty[rs]);
+                        mbar_arrive(is_v ? &bars.v_full[slot] : &bars.k_full[slot]);
+                    }
+                    nt++;
+                }
             }
         }
     } else {
         tc::fewer_registers<KP_REGS_ISSUE>();
         if (warp == 16) {
             // -------------------------------------------------------- the MMAs
-            if (n > 0) {
-                constexpr uint32_t id_qk = tc::idesc(KP_M, KP_N, false), id_pv = tc::idesc(KP_M, HD, true);
-                const uint32_t q_lo = tc::desc_lo(smem_u32(smem + Cfg::Q), 16), k_lo = tc::desc_lo(smem_u32(smem + Cfg::K), 16),
-                               v_lo = tc::desc_lo(smem_u32(smem + Cfg::V), Cfg::HALF);
-                auto qk = [&](int m, int j) {
-                    const uint32_t a_lo = q_lo + m * (Cfg::TILE >> 4), b_lo = k_lo + (j & 1) * (Cfg::TILE >> 4);
-                    if (tc::elect()) {
+            constexpr uint32_t id_qk = tc::idesc(KP_M, KP_N, false), id_pv = tc::idesc(KP_M, HD, true);
+            const uint32_t q_lo = tc::desc_lo(smem_u32(smem + Cfg::Q), 16), k_lo = tc::desc_lo(smem_u32(smem + Cfg::K), 16),
+                           v_lo = tc::desc_lo(smem_u32(smem + Cfg::V), Cfg::HALF);
+            // S of tile nt, and with the last of m: K's slot is free, with a block's last: Q too
+            auto qk = [&](int m, int nt, bool k_free, bool q_free) {
+                const uint32_t a_lo = q_lo + m * (Cfg::TILE >> 4), b_lo = k_lo + (nt & 1) * (Cfg::TILE >> 4);
+                if (tc::elect()) {
 #pragma unroll
-                        for (int k = 0; k < HD / 16; k++) {
-                            const uint32_t off = ((k >> 2) * Cfg::HALF + (k & 3) * 32) >> 4;
-                            tc::mma_ss(tmem + m * KP_N, a_lo + off, tc::DESC_HI, b_lo + off, tc::DESC_HI, id_qk, k > 0);
-                        }
-                        tc::commit(&bars.s_full[m]);
+                    for (int k = 0; k < HD / 16; k++) {
+                        const uint32_t off = ((k >> 2) * Cfg::HALF + (k & 3) * 32) >> 4;
+                        tc::mma_ss(tmem + m * KP_N, a_lo + off, tc::DESC_HI, b_lo + off, tc::DESC_HI, id_qk, k > 0);
                     }
-                    __syncwarp();
-                };
-                auto pv = [&](int m, int j, int hf) {
-                    const uint32_t b_lo = v_lo + (j & 1) * (Cfg::TILE >> 4) + hf * (64 * 128 >> 4);
-                    if (tc::elect()) {
+                    tc::commit(&bars.s_full[m]);
+                    if (k_free) tc::commit(&bars.k_empty[nt & 1]);
+                    if (q_free) tc::commit(&bars.q_empty[m]);
+                }
+                __syncwarp();
+            };
+            auto pv = [&](int m, int nt, int hf, bool first, bool v_free, bool last) {
+                const uint32_t b_lo = v_lo + (nt & 1) * (Cfg::TILE >> 4) + hf * (64 * 128 >> 4);
+                if (tc::elect()) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            tc::mma_ts(tmem + 256 + m * HD, tmem + m * KP_N + 64 * hf + 8 * k, b_lo + k * (2048 >> 4), tc::DESC_HI,
-                                       id_pv, k > 0 ? 1 : j | hf);
-                        if (hf == 0) {
-                            tc::commit(&bars.o_half[m]);
-                        } else {
-                            if (m == mt - 1) tc::commit(&bars.v_empty[j & 1]);
-                            if (j + 1 == n) tc::commit(&bars.o_full[m]);
-                        }
-                    }
-                    __syncwarp();
-                };
-                KP_WAIT_WARP(bars.q_full, 0);
-                KP_WAIT_WARP(bars.k_full[0], 0);
-                tc::fence_after();
-                for (int m = 0; m < mt; m++) qk(m, 0);
-                if (tc::elect()) tc::commit(&bars.k_empty[0]);
-                for (int j = 0; j < n; j++) {
-                    KP_WAIT_WARP(bars.v_full[j & 1], (j >> 1) & 1);
-                    for (int m = 0; m < mt; m++) {
-                        for (int hf = 0; hf < 2; hf++) {
-                            KP_WAIT_WARP(bars.p_full[m][hf], j & 1);
-                            tc::fence_after();
-                            pv(m, j, hf);
-                        }
-                        if (j + 1 < n) {
-                            if (m == 0) KP_WAIT_WARP(bars.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
-                            tc::fence_after();
-                            qk(m, j + 1);
-                            if (m == mt - 1 && tc::elect()) tc::commit(&bars.k_empty[(j + 1) & 1]);
-                        }
+                    for (int k = 0; k < 4; k++)
+                        tc::mma_ts(tmem + 256 + m * HD, tmem + m * KP_N + 64 * hf + 8 * k, b_lo + k * (2048 >> 4), tc::DESC_HI,
+                                   id_pv, k > 0 || hf || !first);
+                    if (hf == 0) {
+                        tc::commit(&bars.o_half[m]);
+                    } else {
+                        if (v_free) tc::commit(&bars.v_empty[nt & 1]);
+                        if (last) tc::commit(&bars.o_full[m]);
                     }
                 }
+                __syncwarp();
+            };
+            // One step a tile: its products with V, and S of the tile after it, which may be the next block's
+            auto skip_empty = [&]() {  // to a block with tiles in the run, if there is one
+                while (it.in_run_warp(a, len)) {
+                    if (it.n > 0) return true;
+                    it.next(a);
+                }
+                return false;
+            };
+            bool more = skip_empty();
+            int j = -1, n = more ? it.n : 0, mt = 0;  // the tile of the products; -1: none yet
+            int nt = -1, pt[2] = {0, 0}, qt[2] = {0, 0};  // tiles; tiles and blocks of A and of B
+            while (more) {
+                // the tile after (j, n, mt)
+                int nj = j + 1, nn = n, nmt = mt;
+                if (j < 0) {
+                    nmt = it.mt();
+                } else if (nj == n) {
+                    it.next(a);
+                    more = skip_empty();
+                    if (more) nj = 0, nn = it.n, nmt = it.mt();
+                }
+                if (j >= 0) KP_WAIT_WARP(bars.v_full[nt & 1], (nt >> 1) & 1);
+                for (int m = 0; m < 2; m++) {
+                    if (j >= 0 && m < mt) {
+                        for (int hf = 0; hf < 2; hf++) {
+                            KP_WAIT_WARP(bars.p_full[m][hf], pt[m] & 1);
+                            tc::fence_after();
+                            pv(m, nt, hf, j == 0, m == mt - 1, j + 1 == n);
+                        }
+                        pt[m]++;
+                    }
+                    if (more && m < nmt) {
+                        if (m == 0) KP_WAIT_WARP(bars.k_full[(nt + 1) & 1], ((nt + 1) >> 1) & 1);
+                        if (nj == 0) {
+                            KP_WAIT_WARP(bars.q_full[m], qt[m] & 1);
+                            qt[m]++;
+                        }
+                        tc::fence_after();
+                        qk(m, nt + 1, m == nmt - 1, nj + 1 == nn);
+                    }
+                }
+                nt++;
+                j = nj, n = nn, mt = nmt;
             }
         } else if (warp == 17) {
         // ------------------------------------------------------------ raw tiles by bulk copies
         if (lane == 0) {
-            const int64_t head = ((int64_t)a.seq * c.n_kv + g) * c.n_ctx;
-            for (int i = 0; i < 2 * n; i++) {
-                const int rs = i % KP_RAW;
-                if (i >= KP_RAW) KP_WAIT(bars.raw_empty[rs], ((i / KP_RAW) - 1) & 1);
-                const int p0 = seen.tile(tile0 + (i >> 1)) * KP_N;
-                const int np = min(KP_N, c.n_ctx - p0);  // the cache may end inside the last tile (at 64)
-                uint8_t *dst = smem + Cfg::R + rs * Cfg::RAW;
-                uint64_t *full = &bars.raw_full[i & 1][rs];
-                mbar_arrive_expect_tx(full, (uint32_t)(np * (HD / 2 + NB * 2)));
-                bulk_g2s(dst, (i & 1 ? c.vc : c.kc) + (head + p0) * (HD / 2), (uint32_t)(np * (HD / 2)), full);
-                bulk_g2s(dst + Cfg::CODES, (i & 1 ? c.vs : c.ks) + (head + p0) * NB, (uint32_t)(np * NB * 2),
-                         full);
+            int i = 0;  // raw tiles before
+            for (; it.in_run(a, len); it.next(a)) {
+                const int64_t head = ((int64_t)a.seq * c.n_kv + it.g) * c.n_ctx;
+                for (int j = 0; j < 2 * it.n; j++, i++) {
+                    const int rs = i % KP_RAW;
+                    if (i >= KP_RAW) KP_WAIT(bars.raw_empty[rs], ((i / KP_RAW) - 1) & 1);
+                    const int p0 = it.seen.tile(it.tile0 + (j >> 1)) * KP_N;
+                    const int np = min(KP_N, c.n_ctx - p0);  // the cache may end inside the last tile (at 64)
+                    uint8_t *dst = smem + Cfg::R + rs * Cfg::RAW;
+                    uint64_t *full = &bars.raw_full[j & 1][rs];
+                    mbar_arrive_expect_tx(full, (uint32_t)(np * (HD / 2 + NB * 2)));
+                    bulk_g2s(dst, (j & 1 ? c.vc : c.kc) + (head + p0) * (HD / 2), (uint32_t)(np * (HD / 2)), full);
+                    bulk_g2s(dst + Cfg::CODES, (j & 1 ? c.vs : c.ks) + (head + p0) * NB, (uint32_t)(np * NB * 2), full);
+                }
             }
         }
         }
@@ -518,18 +722,21 @@ done:
     }
 }
 
-// The rows' parts, in order: a thread per row and 8 values, a block's rows side by side.
+// The pieces of a block that was cut, in order: a thread per row and 8 values, the block's rows side by side.  Of the
+// runs that share a block the second one's blocks here do it.
 template <int HD, typename T>
-__global__ void __launch_bounds__(KP_ROWS) kv4_join_kernel(const float *__restrict__ part, T *__restrict__ out, int64_t out_ld,
-                                                           int n_tok, int n_head, int n_kv, int splits) {
+__global__ void __launch_bounds__(KP_ROWS) kv4_join_kernel(const float *__restrict__ part, const KpCut *__restrict__ cuts,
+                                                           T *__restrict__ out, int64_t out_ld, int rows, int G) {
     pdl_wait();
     pdl_trigger();
-    const int G = n_head / n_kv, rows = n_tok * G, blocks = (rows + KP_ROWS - 1) / KP_ROWS;
-    const int g8 = blockIdx.x % (HD / 8), list = blockIdx.x / (HD / 8);  // of (block, KV head), as the CTAs were numbered
-    const int row = (blocks - 1 - list / n_kv) * KP_ROWS + (int)threadIdx.x, g = list % n_kv;
+    const int g8 = blockIdx.x % (HD / 8), run = blockIdx.x / (HD / 8) + 1;
+    const KpCut cut = cuts[run];
+    if (cut.first != run - 1) return;
+    const int row = cut.blk * KP_ROWS + (int)threadIdx.x, g = cut.g, splits = cut.last - cut.first + 1;
     if (row >= rows) return;
-    constexpr int64_t STEP = (int64_t)KP_ROWS * (HD + 2);
-    const float *p = part + (int64_t)list * splits * STEP;
+    constexpr int64_t STEP = 2 * Kv4PrefillCfg<HD>::PART;
+    // the first run's tail, then the others' heads
+    const float *p = part + cut.first * STEP;
     const float *stats = p + KP_ROWS * HD + threadIdx.x;
     const float4 *o = reinterpret_cast<const float4 *>(p) + 2 * g8 * KP_ROWS + threadIdx.x;
     float top = -INFINITY, L = 0.0f, x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -540,7 +747,7 @@ __global__ void __launch_bounds__(KP_ROWS) kv4_join_kernel(const float *__restri
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const bool in = s0 + u < splits;
-            const int64_t at = (s0 + u) * STEP;
+            const int64_t at = (s0 + u) * STEP + (s0 + u ? 0 : STEP / 2);
             r[u] = in ? __ldcg(stats + at) : -INFINITY, l[u] = in ? __ldcg(stats + at + KP_ROWS) : 0.0f;
             y[u][0] = in ? __ldcg(o + at / 4) : make_float4(0, 0, 0, 0);
             y[u][1] = in ? __ldcg(o + at / 4 + KP_ROWS) : make_float4(0, 0, 0, 0);
@@ -567,7 +774,9 @@ __global__ void __launch_bounds__(KP_ROWS) kv4_join_kernel(const float *__restri
 }
 
 // ------------------------------------------------------------------ launchers
-size_t kv4_prefill_part_bytes(int sm_count) { return (size_t)sm_count * KP_ROWS * (128 + 2) * 4; }
+size_t kv4_prefill_part_bytes(int sm_count) {
+    return (size_t)sm_count * (sizeof(KpCut) + 2 * Kv4PrefillCfg<128>::PART * 4);
+}
 
 template <int HD, typename T>
 static cudaError_t prefill_launch(const Kv4Attn &x, const Kv4Planes &c, float *part, int sm_count, int *err,
@@ -584,23 +793,30 @@ static cudaError_t prefill_launch(const Kv4Attn &x, const Kv4Planes &c, float *p
         set[dev] = 1;
     }
     const int G = x.n_head / c.n_kv;
-    const int64_t rows = (int64_t)x.n_tok * G, blocks = (rows + KP_ROWS - 1) / KP_ROWS, ctas = blocks * c.n_kv;
+    const int64_t rows = (int64_t)x.n_tok * G, blocks = (rows + KP_ROWS - 1) / KP_ROWS;
     if (rows > (1 << 30)) return cudaErrorInvalidValue;
-    // fewer CTAs than SMs: each block's positions over several, two tiles each at least
-    const int tiles = kp_seen(x.pos0, 0, x.n_tok - 1, x.window, x.n_sink).tiles;
-    int64_t splits = sm_count / ctas;
-    if (splits > tiles / 2) splits = tiles / 2;
-    if (splits < 1) splits = 1;
+    int64_t units = 0;  // of a KV head
+    for (int64_t row = 0; row < rows; row += KP_ROWS) {
+        const int64_t last = row + KP_ROWS < rows ? row + KP_ROWS - 1 : rows - 1;
+        units += (int64_t)kp_seen(x.pos0, (int)(row / G), (int)(last / G), x.window, x.n_sink).tiles *
+                     (last - row >= KP_M ? KP_UNITS : KP_UNITS1) +
+                 KP_UNITS_BLOCK;
+    }
+    // a CTA per SM, each with a block's cost and two tiles at least (so that every run has a tile)
+    const int64_t most = units * c.n_kv / (KP_UNITS_BLOCK + 2 * KP_UNITS);
+    const int ctas = most < 1 ? 1 : most < sm_count ? (int)most : sm_count;
+    if (units * c.n_kv / ctas > (1 << 30)) return cudaErrorInvalidValue;
     Kv4PrefillArgs a;
     a.q = x.q, a.out = x.out, a.q_ld = x.q_ld, a.out_ld = x.out_ld;
-    a.seq = x.seq0, a.pos0 = x.pos0, a.n_tok = x.n_tok, a.n_head = x.n_head;
-    a.window = x.window, a.n_sink = x.n_sink, a.splits = (int)splits, a.scale = x.scale;
-    a.part = part, a.err = err;
-    cudaError_t e = launch_k(kv4_prefill_kernel<HD, T>, dim3((unsigned)(ctas * splits)), dim3(KP_THREADS),
-                             (size_t)Cfg::SMEM, st, a, c);
-    if (e != cudaSuccess || splits == 1) return e;
-    return launch_k(kv4_join_kernel<HD, T>, dim3((unsigned)(ctas * (HD / 8))), dim3(KP_ROWS), 0, st,
-                    (const float *)part, (T *)x.out, x.out_ld, x.n_tok, x.n_head, c.n_kv, (int)splits);
+    a.seq = x.seq0, a.pos0 = x.pos0, a.n_tok = x.n_tok;
+    a.window = x.window, a.n_sink = x.n_sink, a.scale = x.scale;
+    a.group = G, a.group_inv = G > 1 ? ~0ull / G + 1 : 0, a.blocks = (int)blocks, a.head_units = units;
+    a.cuts = reinterpret_cast<KpCut *>(part), a.part = part + sm_count * (sizeof(KpCut) / 4);
+    a.err = err;
+    cudaError_t e = launch_k(kv4_prefill_kernel<HD, T>, dim3((unsigned)ctas), dim3(KP_THREADS), (size_t)Cfg::SMEM, st, a, c);
+    if (e != cudaSuccess || ctas == 1) return e;
+    return launch_k(kv4_join_kernel<HD, T>, dim3((unsigned)((ctas - 1) * (HD / 8))), dim3(KP_ROWS), 0, st,
+                    (const float *)a.part, (const KpCut *)a.cuts, (T *)x.out, x.out_ld, (int)rows, G);
 }
 
 cudaError_t launch_kv4_prefill(bool f32, int head_dim, const Kv4Attn &x, const Kv4Planes &c, void *scratch,
