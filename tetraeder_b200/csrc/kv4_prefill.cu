@@ -36,7 +36,7 @@ constexpr int KP_THREADS = 640;
 constexpr int KP_REGS_SOFTMAX = 144, KP_REGS_DEQUANT = 64, KP_REGS_ISSUE = 64;
 static_assert(2 * KP_REGS_SOFTMAX + 2 * KP_REGS_DEQUANT + KP_REGS_ISSUE <= 5 * 96, "the block's registers");
 constexpr int KP_RAW = 3;            // raw tiles (of K or of V) in flight
-constexpr int KP_UNITS = 8, KP_UNITS1 = 5, KP_UNITS_BLOCK = 20;  // work of a tile of positions, of a block (see KpItem)
+constexpr int KP_UNITS = 8, KP_UNITS1 = 5, KP_UNITS_BLOCK = 12;  // work of a tile of positions, of a block (see KpItem)
 constexpr float KP_BIAS = 6.0f;      // P is 2^KP_BIAS at the reference
 constexpr float KP_MOST = 16384.0f;  // a half tile's sum of P above which the row's reference moves
 constexpr float KP_SCALE_MAX = 8188.0f;  // 8 * this is f16's largest
@@ -53,9 +53,9 @@ __host__ __device__ __forceinline__ Kv4Seen kp_seen(int pos0, int t0, int t1, in
     return s;
 }
 
-// A run's first block, where the run begins inside it: its rows' place and the first and last of the runs that share it
+// A block that was cut, and the first and last of the runs that share it
 struct KpCut {
-    int blk, g, first, last;  // first < 0: no such block
+    int blk, g, first, last;  // first < 0: none
 };
 struct Kv4PrefillArgs {
     const void *q;
@@ -66,7 +66,8 @@ struct Kv4PrefillArgs {
     uint64_t group_inv;      // floor((2^64 - 1) / group) + 1, or 0 for a group of 1
     int64_t head_units;      // a KV head's work (see KpItem)
     float scale;
-    KpCut *cuts;  // [cta]
+    KpCut *cuts;  // of the second run of each block that was cut: [run - 1], or (by_item) [g * blocks + blk]
+    bool by_item;
     float *part;  // [cta][head, tail of its run] of O as [HD / 4][KP_ROWS][4], then the references and sums as [2][KP_ROWS]
     int *err;
     // row / group, exact for rows below 2^32
@@ -269,7 +270,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
     float *cs_smem = reinterpret_cast<float *>(smem + Cfg::CS);  // [KP_ROWS]
     pdl_wait();
     pdl_trigger();
-    if (threadIdx.x == 17 * 32) a.cuts[blockIdx.x] = bars.cut;
+    if (threadIdx.x == 17 * 32 && blockIdx.x > 0) {
+        KpCut cut = bars.cut;
+        const bool second = cut.first == (int)blockIdx.x - 1;
+        if (!second) cut.first = -1;
+        if (!a.by_item)
+            a.cuts[blockIdx.x - 1] = cut;
+        else if (second)
+            a.cuts[cut.g * a.blocks + cut.blk] = cut;
+    }
 
     if (warp < 8) {
         tc::more_registers<KP_REGS_SOFTMAX>();
@@ -697,6 +706,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
             int i = 0;  // raw tiles before
             for (; it.in_run(a, len); it.next(a)) {
                 const int64_t head = ((int64_t)a.seq * c.n_kv + it.g) * c.n_ctx;
+                if (a.by_item && it.whole()) a.cuts[it.g * a.blocks + it.blk] = KpCut{it.blk, it.g, -1, -1};
                 for (int j = 0; j < 2 * it.n; j++, i++) {
                     const int rs = i % KP_RAW;
                     if (i >= KP_RAW) KP_WAIT(bars.raw_empty[rs], ((i / KP_RAW) - 1) & 1);
@@ -722,17 +732,17 @@ done:
     }
 }
 
-// The pieces of a block that was cut, in order: a thread per row and 8 values, the block's rows side by side.  Of the
-// runs that share a block the second one's blocks here do it.
+// The pieces of a block that was cut, in order: a thread per row and 8 values, the block's rows side by side.
 template <int HD, typename T>
 __global__ void __launch_bounds__(KP_ROWS) kv4_join_kernel(const float *__restrict__ part, const KpCut *__restrict__ cuts,
                                                            T *__restrict__ out, int64_t out_ld, int rows, int G) {
+    constexpr int DEEP = 8;  // pieces in flight
     pdl_wait();
     pdl_trigger();
-    const int g8 = blockIdx.x % (HD / 8), run = blockIdx.x / (HD / 8) + 1;
-    const KpCut cut = cuts[run];
-    if (cut.first != run - 1) return;
-    const int row = cut.blk * KP_ROWS + (int)threadIdx.x, g = cut.g, splits = cut.last - cut.first + 1;
+    const int g8 = blockIdx.x % (HD / 8);
+    const KpCut cut = cuts[blockIdx.x / (HD / 8)];
+    if (cut.first < 0) return;
+    const int row = cut.blk * KP_ROWS + (int)threadIdx.x, g = cut.g, pieces = cut.last - cut.first + 1;
     if (row >= rows) return;
     constexpr int64_t STEP = 2 * Kv4PrefillCfg<HD>::PART;
     // the first run's tail, then the others' heads
@@ -741,26 +751,28 @@ __global__ void __launch_bounds__(KP_ROWS) kv4_join_kernel(const float *__restri
     const float4 *o = reinterpret_cast<const float4 *>(p) + 2 * g8 * KP_ROWS + threadIdx.x;
     float top = -INFINITY, L = 0.0f, x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
-    for (int s0 = 0; s0 < splits; s0 += 4) {
-        float r[4], l[4];
-        float4 y[4][2];
+    for (int s0 = 0; s0 < pieces; s0 += DEEP) {
+        float r[DEEP], l[DEEP];
+        float4 y[DEEP][2];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const bool in = s0 + u < splits;
-            const int64_t at = (s0 + u) * STEP + (s0 + u ? 0 : STEP / 2);
-            r[u] = in ? __ldcg(stats + at) : -INFINITY, l[u] = in ? __ldcg(stats + at + KP_ROWS) : 0.0f;
-            y[u][0] = in ? __ldcg(o + at / 4) : make_float4(0, 0, 0, 0);
-            y[u][1] = in ? __ldcg(o + at / 4 + KP_ROWS) : make_float4(0, 0, 0, 0);
+        for (int u = 0; u < DEEP; u++) {
+            r[u] = -INFINITY, l[u] = 0.0f, y[u][0] = y[u][1] = make_float4(0, 0, 0, 0);
+            if (s0 + u < pieces) {
+                const int64_t at = (s0 + u) * STEP + (s0 + u ? 0 : STEP / 2);
+                r[u] = __ldcg(stats + at), l[u] = __ldcg(stats + at + KP_ROWS);
+                y[u][0] = __ldcg(o + at / 4), y[u][1] = __ldcg(o + at / 4 + KP_ROWS);
+            }
         }
-        const float next = fmaxf(fmaxf(top, fmaxf(r[0], r[1])), fmaxf(r[2], r[3]));
+        float next = top;
+#pragma unroll
+        for (int u = 0; u < DEEP; u++) next = fmaxf(next, r[u]);
         const float f = top == -INFINITY ? 1.0f : kv4_exp2(top - next);
         top = next, L *= f;
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] *= f;
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            if (l[u] == 0.0f) continue;  // nothing seen there: its sums were not written
-            const float w = r[u] == -INFINITY ? 1.0f : kv4_exp2(r[u] - top);
+        for (int u = 0; u < DEEP; u++) {
+            const float w = r[u] == -INFINITY ? 0.0f : kv4_exp2(r[u] - top);  // without a reference nothing was seen
             L += w * l[u];
             // column 2e of a chunk is value e, column 2e + 1 value 4 + e
             x[0] += w * y[u][0].x, x[4] += w * y[u][0].y, x[1] += w * y[u][0].z, x[5] += w * y[u][0].w;
@@ -812,10 +824,12 @@ static cudaError_t prefill_launch(const Kv4Attn &x, const Kv4Planes &c, float *p
     a.window = x.window, a.n_sink = x.n_sink, a.scale = x.scale;
     a.group = G, a.group_inv = G > 1 ? ~0ull / G + 1 : 0, a.blocks = (int)blocks, a.head_units = units;
     a.cuts = reinterpret_cast<KpCut *>(part), a.part = part + sm_count * (sizeof(KpCut) / 4);
+    const int64_t items = blocks * c.n_kv;
+    a.by_item = items < ctas - 1;
     a.err = err;
     cudaError_t e = launch_k(kv4_prefill_kernel<HD, T>, dim3((unsigned)ctas), dim3(KP_THREADS), (size_t)Cfg::SMEM, st, a, c);
     if (e != cudaSuccess || ctas == 1) return e;
-    return launch_k(kv4_join_kernel<HD, T>, dim3((unsigned)((ctas - 1) * (HD / 8))), dim3(KP_ROWS), 0, st,
+    return launch_k(kv4_join_kernel<HD, T>, dim3((unsigned)((a.by_item ? items : ctas - 1) * (HD / 8))), dim3(KP_ROWS), 0, st,
                     (const float *)a.part, (const KpCut *)a.cuts, (T *)x.out, x.out_ld, (int)rows, G);
 }
 
