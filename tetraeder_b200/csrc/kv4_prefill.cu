@@ -37,6 +37,7 @@ constexpr int KP_REGS_SOFTMAX = 144, KP_REGS_DEQUANT = 64, KP_REGS_ISSUE = 64;
 static_assert(2 * KP_REGS_SOFTMAX + 2 * KP_REGS_DEQUANT + KP_REGS_ISSUE <= 5 * 96, "the block's registers");
 constexpr int KP_RAW = 3;            // raw tiles (of K or of V) in flight
 constexpr int KP_UNITS = 8, KP_UNITS1 = 5, KP_UNITS_BLOCK = 12;  // work of a tile of positions, of a block (see KpItem)
+constexpr int KP_UNITS_JOIN = 28, KP_MAX_CTAS = 512;
 constexpr float KP_BIAS = 6.0f;      // P is 2^KP_BIAS at the reference
 constexpr float KP_MOST = 16384.0f;  // a half tile's sum of P above which the row's reference moves
 constexpr float KP_SCALE_MAX = 8188.0f;  // 8 * this is f16's largest
@@ -62,7 +63,8 @@ struct Kv4PrefillArgs {
     void *out;
     int64_t q_ld, out_ld;
     int seq, pos0, n_tok, window, n_sink;
-    int group, blocks;       // query heads of a KV head; blocks of KP_ROWS rows of one
+    int group, blocks, n_kv;  // query heads of a KV head; blocks of KP_ROWS rows of one
+    bool whole;              // see KpItem
     uint64_t group_inv;      // floor((2^64 - 1) / group) + 1, or 0 for a group of 1
     int64_t head_units;      // a KV head's work (see KpItem)
     float scale;
@@ -79,13 +81,14 @@ __device__ __forceinline__ int kp_uniform(int x) { return __shfl_sync(0xffffffff
 
 // The work is one list: KV head by KV head, block by block, tile by tile.  A block costs KP_UNITS_BLOCK, then a tile
 // KP_UNITS (KP_UNITS1 where there are no rows in B).  Every CTA takes an even run of the list, so a block may be cut: its pieces
-// go to `part` and kv4_join_kernel adds them.
+// go to `part` and kv4_join_kernel adds them.  Where whole blocks share out as well (see prefill_launch) nothing is cut: the CTAs
+// take them in turn, the last (longest) ones first, to and fro.
 struct KpItem {
-    int g, blk, s;  // s: the block's first unit, from the run's first
+    int g, blk, s;  // s: the block's first unit, from the run's first (whole: the turn)
     int row0, n_rows, tiles, tile0, n;
     Kv4Seen seen;
     __device__ __forceinline__ int mt() const { return n_rows > KP_M ? 2 : 1; }
-    __device__ __forceinline__ bool whole() const { return n == tiles; }
+    __device__ __forceinline__ bool uncut() const { return n == tiles; }
     __device__ __forceinline__ int tiles_before(int units) const {  // tiles that begin before the block's first `units`
         const int u = units - KP_UNITS_BLOCK;
         return u <= 0 ? 0 : min(tiles, mt() == 2 ? (u + KP_UNITS - 1) / KP_UNITS : (u + KP_UNITS1 - 1) / KP_UNITS1);
@@ -93,11 +96,18 @@ struct KpItem {
     __device__ __forceinline__ int units() const { return KP_UNITS_BLOCK + tiles * (mt() == 2 ? KP_UNITS : KP_UNITS1); }
     // The part of this block in a run of `len` units: tiles tile0 .. tile0 + n - 1 of `tiles`; false: beyond the run
     __device__ __forceinline__ bool in_run(const Kv4PrefillArgs &a, int len) {
-        if (s >= len) return false;
+        if (a.whole) {
+            const int ctas = (int)gridDim.x, i = s * ctas + (s & 1 ? ctas - 1 - (int)blockIdx.x : (int)blockIdx.x);
+            if (i >= a.blocks * a.n_kv) return false;
+            blk = a.blocks - 1 - i / a.n_kv, g = i % a.n_kv;
+        } else if (s >= len) {
+            return false;
+        }
         row0 = blk * KP_ROWS, n_rows = min(KP_ROWS, a.n_tok * a.group - row0);
         seen = kp_seen(a.pos0, a.token(row0), a.token(row0 + n_rows - 1), a.window, a.n_sink);
         tiles = seen.tiles;
-        tile0 = tiles_before(-s), n = tiles_before(len - s) - tile0;
+        tile0 = 0, n = tiles;
+        if (!a.whole) tile0 = tiles_before(-s), n = tiles_before(len - s) - tile0;
         return true;
     }
     // The same by a whole warp, the results in uniform registers: what depends on them (branches, descriptors) is the
@@ -109,6 +119,10 @@ struct KpItem {
         return true;
     }
     __device__ __forceinline__ void next(const Kv4PrefillArgs &a) {
+        if (a.whole) {
+            s++;
+            return;
+        }
         s += units();
         if (++blk == a.blocks) blk = 0, g++;
     }
@@ -222,7 +236,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
         fence_barrier_init();
     }
     if (warp == 16) tc::alloc(&bars.tmem, 512);
-    if (warp == 17) {
+    if (a.whole) {
+        if (threadIdx.x == 0) bars.g = bars.blk = bars.s = bars.len = 0;
+    } else if (warp == 17) {
         // the run, by a scan over a head's blocks
         const int64_t total = a.head_units * c.n_kv, u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
         const int g = (int)(u0 / a.head_units);
@@ -270,7 +286,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
     float *cs_smem = reinterpret_cast<float *>(smem + Cfg::CS);  // [KP_ROWS]
     pdl_wait();
     pdl_trigger();
-    if (threadIdx.x == 17 * 32 && blockIdx.x > 0) {
+    if (!a.whole && threadIdx.x == 17 * 32 && blockIdx.x > 0) {
         KpCut cut = bars.cut;
         const bool second = cut.first == (int)blockIdx.x - 1;
         if (!second) cut.first = -1;
@@ -426,7 +442,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const int row = row_lo + r;
             float *part = nullptr;
-            if (!it.whole()) {  // O as it is, rows side by side
+            if (!it.uncut()) {  // O as it is, rows side by side
                 float *piece = a.part + (2 * (int64_t)blockIdx.x + (it.tile0 > 0 ? 0 : 1)) * Cfg::PART;
                 part = piece + (m * KP_M + r) * 4;
                 float *stats = piece + KP_ROWS * HD + m * KP_M + r;
@@ -512,69 +528,26 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
             const int q_at = nt ? 1 : 0;
 #pragma unroll 1
             for (int j = 0; j < it.n || j <= q_at; j++) {
-                if (j == q_at && m < it.mt()) {
+                const bool load_q = j == q_at && m < it.mt();
+                const uint32_t q_tile = smem0 + Cfg::Q + m * Cfg::TILE;  // chunk c of row r at c ^ (r & 7)
+                const int my_row = min(it.row0 + m * KP_M + r, it.row0 + it.n_rows - 1), tok = a.token(my_row);
+                const T *my_q = reinterpret_cast<const T *>(a.q) + (int64_t)tok * a.q_ld +
+                                (int64_t)(it.g * a.group + my_row - tok * a.group) * HD;
+                constexpr int CH = HD / 8;
+                if (load_q) {
                     if (items > 0) KP_WAIT_WARP(bars.q_empty[m], (items - 1) & 1);
-                    // The warp's 32 rows into the operand's layout, a thread per row: bf16 by asynchronous copies, all in flight,
-                    // and then in place; f32 read twice.  Loops stay rolled: their code is fetched anew by every CTA.
-                    uint8_t *q_tile = smem + Cfg::Q + m * Cfg::TILE;
-                    auto chunk = [&](int r, int ch) { return q_tile + (ch >> 3) * Cfg::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
-                    const int my_row = min(it.row0 + m * KP_M + r, it.row0 + it.n_rows - 1), tok = a.token(my_row);
-                    const T *my_q = reinterpret_cast<const T *>(a.q) + (int64_t)tok * a.q_ld + (int64_t)(it.g * a.group + my_row - tok * a.group) * HD;
-                    constexpr int CH = HD / 8;
-                    float top = 0.0f;
-                    if constexpr (sizeof(T) == 2) {
+                    if constexpr (sizeof(T) == 2) {  // the warp's 32 rows in flight, while a tile is dequantised
 #pragma unroll 4
                         for (int i = 0; i < 32; i += 32 / CH) {
-                            const int src = i + lane / CH, ch = lane % CH;
+                            const int src = i + lane / CH, ch = lane % CH, rr = (warp & 3) * 32 + src;
                             const T *p = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, (unsigned long long)my_q, src)) + 8 * ch;
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(chunk((warp & 3) * 32 + src, ch))), "l"(p)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                             q_tile + (ch >> 3) * Cfg::HALF + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)),
+                                         "l"(p)
                                          : "memory");
                         }
                         asm volatile("cp.async.commit_group;" ::: "memory");
-                        asm volatile("cp.async.wait_group 0;" ::: "memory");
-                        __syncwarp();
-#pragma unroll 2
-                        for (int ch = 0; ch < CH; ch++) {
-                            const uint4 u = *reinterpret_cast<const uint4 *>(chunk(r, ch));
-                            // magnitudes of bf16 order as their bits
-                            const uint32_t h = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu),
-                                                        __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
-                            top = fmaxf(top, fmaxf(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)));
-                        }
-                    } else {
-#pragma unroll 2
-                        for (int ch = 0; ch < CH; ch++) {
-                            float x[8];
-                            kv4_load_row(my_q + 8 * ch, x);
-#pragma unroll
-                            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
-                        }
                     }
-                    // 2^e * top in [2^5, 2^6): exact for bf16 values down to 2^-22 of the largest
-                    const int e = top > 0.0f && top <= FLT_MAX ? 5 - ilogbf(top) : 0;
-                    const int e1 = e / 2, e2 = e - e1;
-                    const float up1 = kv4_pow2(e1), up2 = kv4_pow2(e2);
-#pragma unroll 2
-                    for (int ch = 0; ch < CH; ch++) {
-                        uint4 *dst = reinterpret_cast<uint4 *>(chunk(r, ch));
-                        float x[8];
-                        if constexpr (sizeof(T) == 2) {
-                            const uint4 u = *dst;
-                            kv4_bf2(u.x, x[0], x[1]), kv4_bf2(u.y, x[2], x[3]), kv4_bf2(u.z, x[4], x[5]), kv4_bf2(u.w, x[6], x[7]);
-                        } else {
-                            kv4_load_row(my_q + 8 * ch, x);
-                        }
-#pragma unroll
-                        for (int v = 0; v < 8; v++) x[v] = x[v] * up1 * up2;
-                        *dst = make_uint4(kv4_half2(x[0], x[4]), kv4_half2(x[1], x[5]), kv4_half2(x[2], x[6]), kv4_half2(x[3], x[7]));
-                    }
-                    // log2 score of an accumulator's 1; never 0: masked scores are -inf times it
-                    const float cs = fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(-e1) * kv4_pow2(-e2), FLT_MIN);
-                    cs_smem[m * KP_M + r] = cs;
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars.q_full[m]);
-                    items++;
                 }
                 if (j < it.n) {
                     const int i = 2 * nt + is_v, slot = nt & 1, rs = i % KP_RAW;
@@ -615,6 +588,55 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                         mbar_arrive(is_v ? &bars.v_full[slot] : &bars.k_full[slot]);
                     }
                     nt++;
+                }
+                if (load_q) {
+                    // A thread per row, scaled in place (f32 rows are read twice)
+                    const uint32_t q_row = q_tile + r * 128 + (r & 7) * 16;
+                    auto chunk = [&](int ch) { return (q_row + (ch >> 3) * Cfg::HALF) ^ ((ch & 7) * 16); };
+                    float top = 0.0f;
+                    if constexpr (sizeof(T) == 2) {
+                        asm volatile("cp.async.wait_group 0;" ::: "memory");
+                        __syncwarp();
+#pragma unroll 4
+                        for (int ch = 0; ch < CH; ch++) {
+                            const uint4 u = tc::lds128(chunk(ch));
+                            // magnitudes of bf16 order as their bits
+                            const uint32_t h = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu),
+                                                        __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
+                            top = fmaxf(top, fmaxf(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)));
+                        }
+                    } else {
+#pragma unroll 4
+                        for (int ch = 0; ch < CH; ch++) {
+                            float x[8];
+                            kv4_load_row(my_q + 8 * ch, x);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
+                        }
+                    }
+                    // 2^e * top in [2^5, 2^6), or below where top < 2^-121: exact for bf16 values down to 2^-22 of the largest
+                    const int e = top > 0.0f && top <= FLT_MAX ? min(5 + 127 - (int)(__float_as_uint(top) >> 23), 126) : 0;
+                    const float up = kv4_pow2(e);
+#pragma unroll 4
+                    for (int ch = 0; ch < CH; ch++) {
+                        float x[8];
+                        if constexpr (sizeof(T) == 2) {
+                            const uint4 u = tc::lds128(chunk(ch));
+                            kv4_bf2(u.x, x[0], x[1]), kv4_bf2(u.y, x[2], x[3]), kv4_bf2(u.z, x[4], x[5]), kv4_bf2(u.w, x[6], x[7]);
+                        } else {
+                            kv4_load_row(my_q + 8 * ch, x);
+                        }
+#pragma unroll
+                        for (int v = 0; v < 8; v++) x[v] *= up;
+                        tc::sts128(chunk(ch), make_uint4(kv4_half2(x[0], x[4]), kv4_half2(x[1], x[5]), kv4_half2(x[2], x[6]),
+                                                         kv4_half2(x[3], x[7])));
+                    }
+                    // log2 score of an accumulator's 1; never 0: masked scores are -inf times it
+                    cs_smem[m * KP_M + r] = fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(-e), FLT_MIN);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.q_full[m]);
+                    items++;
                 }
             }
         }
@@ -706,7 +728,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
             int i = 0;  // raw tiles before
             for (; it.in_run(a, len); it.next(a)) {
                 const int64_t head = ((int64_t)a.seq * c.n_kv + it.g) * c.n_ctx;
-                if (a.by_item && it.whole()) a.cuts[it.g * a.blocks + it.blk] = KpCut{it.blk, it.g, -1, -1};
+                if (a.by_item && it.uncut()) a.cuts[it.g * a.blocks + it.blk] = KpCut{it.blk, it.g, -1, -1};
                 for (int j = 0; j < 2 * it.n; j++, i++) {
                     const int rs = i % KP_RAW;
                     if (i >= KP_RAW) KP_WAIT(bars.raw_empty[rs], ((i / KP_RAW) - 1) & 1);
@@ -732,33 +754,37 @@ done:
     }
 }
 
-// The pieces of a block that was cut, in order: a thread per row and 8 values, the block's rows side by side.
-template <int HD, typename T>
+// The pieces of a block that was cut: a thread per row and 8 values, and of those pieces every LISTS-th.  A block
+// here has KP_ROWS / LISTS rows.  Few blocks of many pieces take 4 lists (33 tokens at 20000: 18 pieces of 8 blocks), else all pieces
+// are one thread's, in two loads.
+template <int HD, typename T, int LISTS>
 __global__ void __launch_bounds__(KP_ROWS) kv4_join_kernel(const float *__restrict__ part, const KpCut *__restrict__ cuts,
                                                            T *__restrict__ out, int64_t out_ld, int rows, int G) {
-    constexpr int DEEP = 8;  // pieces in flight
+    constexpr int DEEP = LISTS > 1 ? 6 : 2, R = KP_ROWS / LISTS;  // pieces in flight; rows
+    __shared__ float sums[LISTS > 1 ? LISTS - 1 : 1][10][R];
     pdl_wait();
     pdl_trigger();
-    const int g8 = blockIdx.x % (HD / 8);
-    const KpCut cut = cuts[blockIdx.x / (HD / 8)];
+    const int g8 = blockIdx.x % (HD / 8), rb = blockIdx.x / (HD / 8) % LISTS;
+    const KpCut cut = cuts[blockIdx.x / (HD / 8 * LISTS)];
     if (cut.first < 0) return;
-    const int row = cut.blk * KP_ROWS + (int)threadIdx.x, g = cut.g, pieces = cut.last - cut.first + 1;
-    if (row >= rows) return;
+    const int mine = threadIdx.x % R, list = threadIdx.x / R, r_blk = rb * R + mine;
+    const int row = cut.blk * KP_ROWS + r_blk, g = cut.g, pieces = cut.last - cut.first + 1;
     constexpr int64_t STEP = 2 * Kv4PrefillCfg<HD>::PART;
     // the first run's tail, then the others' heads
     const float *p = part + cut.first * STEP;
-    const float *stats = p + KP_ROWS * HD + threadIdx.x;
-    const float4 *o = reinterpret_cast<const float4 *>(p) + 2 * g8 * KP_ROWS + threadIdx.x;
+    const float *stats = p + KP_ROWS * HD + r_blk;
+    const float4 *o = reinterpret_cast<const float4 *>(p) + 2 * g8 * KP_ROWS + r_blk;
     float top = -INFINITY, L = 0.0f, x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
-    for (int s0 = 0; s0 < pieces; s0 += DEEP) {
+    for (int s0 = list; s0 < pieces && row < rows; s0 += DEEP * LISTS) {
         float r[DEEP], l[DEEP];
         float4 y[DEEP][2];
 #pragma unroll
         for (int u = 0; u < DEEP; u++) {
+            const int s = s0 + u * LISTS;
             r[u] = -INFINITY, l[u] = 0.0f, y[u][0] = y[u][1] = make_float4(0, 0, 0, 0);
-            if (s0 + u < pieces) {
-                const int64_t at = (s0 + u) * STEP + (s0 + u ? 0 : STEP / 2);
+            if (s < pieces) {
+                const int64_t at = s * STEP + (s ? 0 : STEP / 2);
                 r[u] = __ldcg(stats + at), l[u] = __ldcg(stats + at + KP_ROWS);
                 y[u][0] = __ldcg(o + at / 4), y[u][1] = __ldcg(o + at / 4 + KP_ROWS);
             }
@@ -779,6 +805,31 @@ __global__ void __launch_bounds__(KP_ROWS) kv4_join_kernel(const float *__restri
             x[2] += w * y[u][1].x, x[6] += w * y[u][1].y, x[3] += w * y[u][1].z, x[7] += w * y[u][1].w;
         }
     }
+    if constexpr (LISTS > 1) {
+        if (list > 0) {
+            float (*z)[R] = sums[list - 1];
+            z[0][mine] = top, z[1][mine] = L;
+#pragma unroll
+            for (int e = 0; e < 8; e++) z[2 + e][mine] = x[e];
+        }
+        __syncthreads();
+        if (list > 0) return;
+        float next = top;
+#pragma unroll
+        for (int i = 0; i < LISTS - 1; i++) next = fmaxf(next, sums[i][0][mine]);
+        const float f = top == -INFINITY ? 0.0f : kv4_exp2(top - next);
+        L *= f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= f;
+#pragma unroll
+        for (int i = 0; i < LISTS - 1; i++) {
+            const float t = sums[i][0][mine], w = t == -INFINITY ? 0.0f : kv4_exp2(t - next);
+            L += w * sums[i][1][mine];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] += w * sums[i][2 + e][mine];
+        }
+    }
+    if (row >= rows) return;
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
     for (int e = 0; e < 8; e++) x[e] *= inv;
@@ -807,30 +858,43 @@ static cudaError_t prefill_launch(const Kv4Attn &x, const Kv4Planes &c, float *p
     const int G = x.n_head / c.n_kv;
     const int64_t rows = (int64_t)x.n_tok * G, blocks = (rows + KP_ROWS - 1) / KP_ROWS;
     if (rows > (1 << 30)) return cudaErrorInvalidValue;
-    int64_t units = 0;  // of a KV head
-    for (int64_t row = 0; row < rows; row += KP_ROWS) {
-        const int64_t last = row + KP_ROWS < rows ? row + KP_ROWS - 1 : rows - 1;
-        units += (int64_t)kp_seen(x.pos0, (int)(row / G), (int)(last / G), x.window, x.n_sink).tiles *
-                     (last - row >= KP_M ? KP_UNITS : KP_UNITS1) +
-                 KP_UNITS_BLOCK;
+    const int64_t items = blocks * c.n_kv;
+    // The work, and the most that a CTA gets if the blocks stay whole
+    int64_t units = 0, most = 0, load[KP_MAX_CTAS] = {};
+    const int turns = sm_count < items ? sm_count : (int)items;
+    if (turns > KP_MAX_CTAS) return cudaErrorInvalidValue;
+    for (int64_t i = 0, b = blocks - 1; b >= 0; b--) {
+        const int64_t row = b * KP_ROWS, last = row + KP_ROWS < rows ? row + KP_ROWS - 1 : rows - 1;
+        const int64_t cost = KP_UNITS_BLOCK + (int64_t)kp_seen(x.pos0, (int)(row / G), (int)(last / G), x.window, x.n_sink).tiles *
+                                                  (last - row >= KP_M ? KP_UNITS : KP_UNITS1);
+        units += cost;
+        for (int g = 0; g < c.n_kv; g++, i++) {
+            const int64_t turn = i / turns, at = i % turns;
+            int64_t &l = load[turn & 1 ? turns - 1 - at : at];
+            l += cost;
+            if (l > most) most = l;
+        }
     }
-    // a CTA per SM, each with a block's cost and two tiles at least (so that every run has a tile)
-    const int64_t most = units * c.n_kv / (KP_UNITS_BLOCK + 2 * KP_UNITS);
-    const int ctas = most < 1 ? 1 : most < sm_count ? (int)most : sm_count;
-    if (units * c.n_kv / ctas > (1 << 30)) return cudaErrorInvalidValue;
+    const int64_t total = units * c.n_kv;
+    // even runs: a CTA per SM, each with a block's cost and two tiles at least (so that every run has a tile)
+    int64_t ctas = total / (KP_UNITS_BLOCK + 2 * KP_UNITS);
+    ctas = ctas < 1 ? 1 : ctas < sm_count ? ctas : sm_count;
+    if (total / ctas > (1 << 30)) return cudaErrorInvalidValue;
     Kv4PrefillArgs a;
+    a.whole = most <= total / ctas + KP_UNITS_JOIN;
+    if (a.whole) ctas = turns;
     a.q = x.q, a.out = x.out, a.q_ld = x.q_ld, a.out_ld = x.out_ld;
     a.seq = x.seq0, a.pos0 = x.pos0, a.n_tok = x.n_tok;
     a.window = x.window, a.n_sink = x.n_sink, a.scale = x.scale;
-    a.group = G, a.group_inv = G > 1 ? ~0ull / G + 1 : 0, a.blocks = (int)blocks, a.head_units = units;
+    a.group = G, a.group_inv = G > 1 ? ~0ull / G + 1 : 0, a.blocks = (int)blocks, a.n_kv = c.n_kv, a.head_units = units;
     a.cuts = reinterpret_cast<KpCut *>(part), a.part = part + sm_count * (sizeof(KpCut) / 4);
-    const int64_t items = blocks * c.n_kv;
     a.by_item = items < ctas - 1;
     a.err = err;
-    cudaError_t e = launch_k(kv4_prefill_kernel<HD, T>, dim3((unsigned)ctas), dim3(KP_THREADS), (size_t)Cfg::SMEM, st, a, c);
-    if (e != cudaSuccess || ctas == 1) return e;
-    return launch_k(kv4_join_kernel<HD, T>, dim3((unsigned)((a.by_item ? items : ctas - 1) * (HD / 8))), dim3(KP_ROWS), 0, st,
-                    (const float *)a.part, (const KpCut *)a.cuts, (T *)x.out, x.out_ld, (int)rows, G);
+    const cudaError_t e = launch_k(kv4_prefill_kernel<HD, T>, dim3((unsigned)ctas), dim3(KP_THREADS), (size_t)Cfg::SMEM, st, a, c);
+    if (e != cudaSuccess || a.whole || ctas == 1) return e;
+    return launch_k(a.by_item ? kv4_join_kernel<HD, T, 4> : kv4_join_kernel<HD, T, 1>,
+                    dim3((unsigned)((a.by_item ? 4 * items : ctas - 1) * (HD / 8))), dim3(KP_ROWS), 0, st, (const float *)a.part,
+                    (const KpCut *)a.cuts, (T *)x.out, x.out_ld, (int)rows, G);
 }
 
 cudaError_t launch_kv4_prefill(bool f32, int head_dim, const Kv4Attn &x, const Kv4Planes &c, void *scratch,
