@@ -36,8 +36,8 @@ constexpr int KP_THREADS = 640;
 constexpr int KP_REGS_SOFTMAX = 144, KP_REGS_DEQUANT = 64, KP_REGS_ISSUE = 64;
 static_assert(2 * KP_REGS_SOFTMAX + 2 * KP_REGS_DEQUANT + KP_REGS_ISSUE <= 5 * 96, "the block's registers");
 constexpr int KP_RAW = 3;            // raw tiles (of K or of V) in flight
-constexpr int KP_UNITS = 8, KP_UNITS1 = 5, KP_UNITS_BLOCK = 12;  // work of a tile of positions, of a block (see KpItem)
-constexpr int KP_UNITS_JOIN = 28, KP_MAX_CTAS = 512;
+constexpr int KP_UNITS = 8, KP_UNITS1 = 6, KP_UNITS_BLOCK = 12;  // work of a tile of positions, of a block (see KpItem)
+constexpr int KP_UNITS_JOIN = 76, KP_MAX_CTAS = 512;
 constexpr float KP_BIAS = 6.0f;      // P is 2^KP_BIAS at the reference
 constexpr float KP_MOST = 16384.0f;  // a half tile's sum of P above which the row's reference moves
 constexpr float KP_SCALE_MAX = 8188.0f;  // 8 * this is f16's largest
