@@ -387,6 +387,32 @@ def test_prefill_long(hd, nh, nkv, S, pos0):
     run_prefill("bf16", hd, nh, nkv, S, pos0, rows=sorted({0, 1, S // 3, S // 2, S - 2, S - 1} | set(range(0, S, 37))))
 
 
+# More rows than the decode kernel is given: a block with rows in one tile only, a last block of a few rows, odd groups
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd,nh,nkv,S,pos0", [(128, 8, 1, 130, 0), (64, 16, 1, 140, 1), (128, 14, 2, 90, 129), (64, 6, 3, 50, 77),
+                                              (128, 5, 5, 27, 4000), (128, 1, 1, 257, 63), (64, 48, 2, 65, 191)])
+def test_prefill_blocks(dtype, hd, nh, nkv, S, pos0):
+    run_prefill(dtype, hd, nh, nkv, S, pos0, rows=sorted({0, 1, S // 2, S - 2, S - 1} | set(range(0, S, 13))))
+
+
+# How the blocks are shared out: few ones cut into many pieces, many ones cut where their number does not divide, all whole and
+# more of them than SMs, a cut inside a block with rows in one tile only, and the same under a window
+@pytest.mark.parametrize("hd,nh,nkv,S,pos0,window,n_sink", [
+    (128, 8, 1, 33, 12000, 0, 0), (64, 4, 1, 40, 30000, 0, 0), (128, 16, 2, 130, 9001, 0, 0), (128, 32, 8, 1240, 5000, 0, 0),
+    (128, 32, 4, 1300, 0, 0, 0), (64, 16, 8, 2900, 0, 0, 0), (128, 40, 8, 1200, 6000, 4096, 4), (64, 8, 8, 260, 20000, 9000, 200)])
+def test_prefill_shares(hd, nh, nkv, S, pos0, window, n_sink):
+    run_prefill("bf16", hd, nh, nkv, S, pos0, window=window, n_sink=n_sink, rows=sorted({0, 1, S // 3, S // 2, S - 2, S - 1} |
+                                                                                        set(range(0, S, S // 7))))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd,nh,nkv", [(128, 32, 4), (64, 16, 16), (128, 24, 2)])
+@pytest.mark.parametrize("S", [2, 3, 4, 5, 9])
+def test_prefill_few_tokens(dtype, hd, nh, nkv, S):
+    run_prefill(dtype, hd, nh, nkv, S, 3001)
+    run_prefill(dtype, hd, nh, nkv, S, 130, window=64, n_sink=3)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("window,n_sink,S,pos0", [(1, 0, 70, 0), (1, 1, 70, 200), (16, 4, 150, 300), (128, 0, 140, 128), (100, 130, 60, 400),
                                                   (129, 3, 300, 0), (5, 300, 40, 500), (1000, 2, 64, 64)])

@@ -34,7 +34,7 @@ __device__ __forceinline__ bool kv4_place(const Kv4RowArgs &a, int64_t i, int &s
 // Rows are independent and only moved once: HBM-bound, if the codes cost few instructions.  A thread takes 16
 // values (a block is two threads, its extremes one shuffle each), so that a warp reads whole 128-byte
 // lines; rows run fastest over the threads, so that a run of positions writes one contiguous piece of a
-// head's plane.
+// head's plane.  8191 bf16 rows of 8 heads of 128, K and V: 12.6 us (floor 9.2); with 8 values a thread and converted codes 20.6.
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowArgs a) {
     const Kv4Planes &c = a.c;
@@ -76,6 +76,8 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowArgs a) {
     if ((sub & 1) == 0) (is_v ? c.vs : c.ks)[row * NB + b] = d;
 }
 
+// A thread writes 8 values (16 bytes of bf16), so that a warp's stores are whole lines.  The same rows: 14.4 us (floor 9.2); two rows
+// a thread 16.5, four 19.7.
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
     const Kv4Planes &c = a.c;
@@ -105,8 +107,8 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
 // For each query token and KV head: softmax(q K^T) V over the seen positions, up to 8 of the head's query
 // heads together (more are further passes over the same rows, from L2).
 //
-// Bound: HBM (a cached position is read once, 4.5 bits a value).  At that rate an SM has about 195
-// clocks for a 32-position tile of 128-wide K and V, 780 issue slots, so the work per value has to be
+// Bound: HBM (a cached position is read once, 4.5 bits a value).  At that rate an SM has about 390
+// clocks for a 64-position tile of 128-wide K and V, 1560 issue slots, so the work per value has to be
 // small:
 //   - Codes meet the tensor cores as they are, as the 16-row operand of mma.sync m16n8k16 (f16 operands, f32
 //     sums); the 8 heads are the 8 columns.  S^T = K Q^T: a 4-bit code under a mask is the f16 subnormal
@@ -129,9 +131,13 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
 // lengths, few sequences or many all load every SM the same.  A segment (one token, KV head and pass)
 // costs a CTA about KA_PART tiles' time to begin and to join, so that a segment counts that much more in
 // the list; where the segments are few against the CTAs, each is instead padded to whole runs, and no
-// CTA has more than one (the cheaper of the two by its longest run).  A warp takes every 8th tile of a
+// CTA has more than one (the cheaper of the two by its longest run).  A warp takes every WARPS-th tile of a
 // run, fetched by bulk copies into its own ring.  Runs that hold less than a segment leave partial sums in
 // scratch; the CTA that arrives last there joins them, in run order (the same sums every call).
+//
+// Measured (32 heads, width 128, bf16): 64 sequences of up to 32768 positions, 4 KV heads, 150 us, 5.1 TB/s; one of 131071, 8 KV
+// heads, 40 us, 3.8 TB/s.  What is left there: the SMs get unequal shares of the bandwidth (their even runs end 138 .. 150 us), and a part's start
+// and join are about 5 us.
 constexpr int KA_HEADS = 8;
 constexpr int KA_PART = 32;
 constexpr float KA_ROOM = 8.0f;  // how far (log2) a score may exceed its head's reference
@@ -153,9 +159,14 @@ struct Kv4AttnArgs {
 template <int HD, bool PREC>
 struct Kv4AttnCfg {
     static constexpr int NB = HD / 32;
-    static constexpr int TILE = 64;  // positions
-    static constexpr int WARPS = HD == 128 ? (PREC ? 8 : 12) : (PREC ? 6 : 6), STAGES = HD == 128 ? (PREC ? 3 : 2) : (PREC ? 4 : 4);
-    static constexpr int CTAS = HD == 128 ? (PREC ? 1 : 1) : (PREC ? 2 : 2);  // per SM
+    static constexpr int TILE = 64;  // positions; in tiles of 32 all of the cases below took 5 to 25% longer
+    // Warps of a CTA, tiles in a warp's ring, CTAs of an SM.  Per SM about 200 KB of ring and as many warps as registers allow;
+    // which split is best was measured:
+    //   width 128, bf16, 64 x 32768 / 1 x 131071: 12 x 2, one CTA 149 / 39.8 us; 8 x 3, one 160 / 41.6; 6 x 2, two 157 / 42.4
+    //   width 128, f32, 4 x 4096: 8 x 3, one CTA 11.1 us; 12 x 2, one 13.3; 6 x 2, two 15.3
+    //   width 64, 16 heads over 16, 24 x 5003: 6 x 4, two CTAs 32.3 us; 12 x 4, one 37.2; 8 x 6, one 38.5
+    static constexpr int WARPS = HD == 64 ? 6 : PREC ? 8 : 12, STAGES = HD == 64 ? 4 : PREC ? 3 : 2;
+    static constexpr int CTAS = HD == 64 ? 2 : 1;
     static constexpr int THREADS = 32 * WARPS;
     static constexpr int CODES = TILE * HD / 2, SCALES = TILE * NB * 2;
     static constexpr int STAGE = 2 * (CODES + SCALES);  // K codes, V codes, K scales, V scales

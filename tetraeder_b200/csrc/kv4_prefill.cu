@@ -2,14 +2,16 @@
 // 5th-generation tensor cores.
 //
 // The query rows of a KV head are its tokens times the query heads that share it (row r: token r / G, head
-// r % G), so that one dequantised tile of K and V serves all of them.  A CTA takes 256 rows, as two
-// 128-row tiles A and B, and walks the 128-position tiles that its tokens see:
+// r % G), so that one dequantised tile of K and V serves all of them.  A block is 256 rows, as two
+// 128-row tiles A and B; a CTA, one per SM, takes its share of the blocks (see KpItem) and walks the 128-position tiles that
+// a block's tokens see:
 //   S = Q K^T   tcgen05, Q and K f16 in shared memory (128-byte swizzle), S f32 in TMEM (128 columns a tile)
 //   P           a thread per row: exp2(S c - ref) as f16, back into TMEM over S
 //   O += P V    tcgen05, P from TMEM, V f16 in shared memory as it lies (rows are positions: an N-major
 //               operand), O f32 in TMEM
-// Warps: 0-3 and 4-7 the softmax of A and B, 8-11 dequantise K and 12-15 V, 16 issues the MMAs, 17 the
-// bulk copies.  While the softmax of one tile runs, the tensor cores work on the other.
+// Warps: 0-3 and 4-7 the softmax of A and B, 8-11 dequantise K and load Q of A, 12-15 V and Q of B, 16 issues the MMAs, 17
+// the bulk copies.  While the softmax of one tile runs, the tensor cores work on the other; the roles run on from one block into
+// the next, so that a block's Q, first tiles and first S are ready when the last one's O is written.
 //
 // Bound: per 256 rows x 128 positions of 128-wide heads the MMAs take 2048 clocks and so do the exps (16 a
 // clock and SM); the dequantisation (13 instructions for 8 values, about 475 issue slots a scheduler)
@@ -21,7 +23,13 @@
 //     at the reference, so that no P leaves f16 before that): no maximum is taken, and O needs no rescaling.
 //     A tile is first tried with the old reference, S still whole in TMEM; the rare failure is redone.
 //   - Q is scaled per row by a power of two into f16's range.  Scales are held to what f16 can carry times 8.
-//   - Few query rows leave SMs idle, so their positions are split over CTAs, and kv4_join_kernel adds the parts.
+//   - What a warp has alike (its role, its block, the conditions of a tile) goes through a shuffle from lane 0, and
+//     shared memory is declared aligned: branches, addresses and descriptors then stay out of the lanes' registers (a tile
+//     pair 2.41 us, without either 2.79).
+// Measured (32 heads over 4, width 128, bf16): 8192 tokens 577 us, 952 TFLOP/s; 4097 tokens of 40 heads over 8 under a window of
+// 4096 419 us; 2048 tokens 50 us; 33 tokens at position 20000 37 us.  A tile pair takes about 4400 clocks, the softmax's chain of
+// S wait (1000), TMEM loads, exps and P (1700 a half) for A beside the same for B; at length the device is at its power limit
+// (1000 W, 1.83 GHz).
 #include "kernels.cuh"
 #include "kv4.cuh"
 #include "tcgen05.cuh"
@@ -29,15 +37,18 @@
 namespace tmoe {
 
 constexpr int KP_M = 128;            // rows of a tile
-constexpr int KP_ROWS = 2 * KP_M;    // of a CTA
+constexpr int KP_ROWS = 2 * KP_M;    // of a block
 constexpr int KP_N = 128;            // positions of a tile
 constexpr int KP_THREADS = 640;
 // Registers per thread: the softmax warps take what the others give back (5 * 96 at launch)
 constexpr int KP_REGS_SOFTMAX = 144, KP_REGS_DEQUANT = 64, KP_REGS_ISSUE = 64;
 static_assert(2 * KP_REGS_SOFTMAX + 2 * KP_REGS_DEQUANT + KP_REGS_ISSUE <= 5 * 96, "the block's registers");
 constexpr int KP_RAW = 3;            // raw tiles (of K or of V) in flight
-constexpr int KP_UNITS = 8, KP_UNITS1 = 6, KP_UNITS_BLOCK = 12;  // work of a tile of positions, of a block (see KpItem)
-constexpr int KP_UNITS_JOIN = 76, KP_MAX_CTAS = 512;
+// Work (see KpItem) of a tile of positions, of one of a block without rows in B (33 tokens at 20000: 5 40 us, 6 36, 7 37), of a block
+// itself (8192 tokens: 8 615 us, 12 597, 20 604), and how much longer a CTA may work to spare cuts and their join (1024
+// tokens: 28 41 us, cut, 76 27, whole; 2048 tokens at 4096 differ by 92: cut 177 us, whole 194).
+constexpr int KP_UNITS = 8, KP_UNITS1 = 6, KP_UNITS_BLOCK = 12, KP_UNITS_JOIN = 76;
+constexpr int KP_MAX_CTAS = 512;
 constexpr float KP_BIAS = 6.0f;      // P is 2^KP_BIAS at the reference
 constexpr float KP_MOST = 16384.0f;  // a half tile's sum of P above which the row's reference moves
 constexpr float KP_SCALE_MAX = 8188.0f;  // 8 * this is f16's largest
@@ -64,9 +75,9 @@ struct Kv4PrefillArgs {
     int64_t q_ld, out_ld;
     int seq, pos0, n_tok, window, n_sink;
     int group, blocks, n_kv;  // query heads of a KV head; blocks of KP_ROWS rows of one
-    bool whole;              // see KpItem
-    uint64_t group_inv;      // floor((2^64 - 1) / group) + 1, or 0 for a group of 1
-    int64_t head_units;      // a KV head's work (see KpItem)
+    bool whole;               // see KpItem
+    uint64_t group_inv;       // floor((2^64 - 1) / group) + 1, or 0 for a group of 1
+    int64_t head_units;       // a KV head's work (see KpItem)
     float scale;
     KpCut *cuts;  // of the second run of each block that was cut: [run - 1], or (by_item) [g * blocks + blk]
     bool by_item;
@@ -755,8 +766,8 @@ done:
 }
 
 // The pieces of a block that was cut: a thread per row and 8 values, and of those pieces every LISTS-th.  A block
-// here has KP_ROWS / LISTS rows.  Few blocks of many pieces take 4 lists (33 tokens at 20000: 18 pieces of 8 blocks), else all pieces
-// are one thread's, in two loads.
+// here has KP_ROWS / LISTS rows.  Few blocks of many pieces take 4 lists (33 tokens at 20000, 8 blocks in some 150 pieces: 7 us from HBM,
+// with one 16); else a block has two pieces, mostly, and they are one thread's.
 template <int HD, typename T, int LISTS>
 __global__ void __launch_bounds__(KP_ROWS) kv4_join_kernel(const float *__restrict__ part, const KpCut *__restrict__ cuts,
                                                            T *__restrict__ out, int64_t out_ld, int rows, int G) {
@@ -857,8 +868,8 @@ static cudaError_t prefill_launch(const Kv4Attn &x, const Kv4Planes &c, float *p
     }
     const int G = x.n_head / c.n_kv;
     const int64_t rows = (int64_t)x.n_tok * G, blocks = (rows + KP_ROWS - 1) / KP_ROWS;
-    if (rows > (1 << 30)) return cudaErrorInvalidValue;
     const int64_t items = blocks * c.n_kv;
+    if (rows > (1 << 30) || items > (1 << 30)) return cudaErrorInvalidValue;
     // The work, and the most that a CTA gets if the blocks stay whole
     int64_t units = 0, most = 0, load[KP_MAX_CTAS] = {};
     const int turns = sm_count < items ? sm_count : (int)items;

@@ -1542,6 +1542,16 @@ int tmoe_kv4_attn_decode(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cac
     return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "kv4 decode attention");
 }
 
+// Whether the decode kernel, a segment per token and KV head, beats the prefill kernel's 256-row blocks.  Measured (32 heads
+// over 4, bf16): 4 tokens at 300 / 20000 / 60000 9 / 18 / 34 us against 11 / 23 / 40; 16 at 300 / 2000 / 8000 8 / 12 / 25 against
+// 11 / 19 / 19.  40 heads over 8: 16 at 2000 18 against 19, 24 at 300 14 against 12.  f32, 3 / 4 at 60000: 37 / 47 against 40 / 41.
+static bool kv4_few(const tmoe::Kv4Attn &x, int n_kv, bool f32) {
+    const int64_t passes = (x.n_head / n_kv + 7) / 8, segments = x.n_tok * n_kv * passes;
+    int64_t seen = (int64_t)x.pos0 + x.n_tok;
+    if (x.window > 0 && seen > (int64_t)x.window + x.n_sink) seen = (int64_t)x.window + x.n_sink;
+    return x.n_tok * passes <= (f32 ? 3 : 4) || x.n_tok == 1 || (segments <= 128 && segments * seen <= 1 << 18);
+}
+
 int tmoe_kv4_attn_prefill(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cache, const tmoe_kv4_attn *attn,
                           int32_t seq, int32_t pos0, int32_t S) {
     if (!h) return TMOE_E_INVALID;
@@ -1559,16 +1569,15 @@ int tmoe_kv4_attn_prefill(tmoe_handle *h, void *stream, const tmoe_kv4_cache *ca
     DeviceGuard dg(h->cfg.device);
     tmoe::PdlScope pdl(!h->prof.on);  // overlap with the kernel before (programmatic launch)
     cudaError_t e = cudaSuccess;
-    if (S == 1) {
-        // a decode step of one sequence
-        e = tmoe::launch_kv4_attn(f32, cache->head_dim, x, planes, attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
-        return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "kv4 decode attention");
-    }
-    if (x.k) {
+    if (S > 1 && x.k) {
         e = tmoe::launch_kv4_rows(true, f32, cache->head_dim, (void *)x.k, (void *)x.v, x.kv_ld, nullptr, seq, nullptr,
                                   pos0, S, planes, h->err, (cudaStream_t)stream);
         if (e != cudaSuccess) return cuda_fail(h, e, "kv4 store");
         x.k = x.v = nullptr;
+    }
+    if (kv4_few(x, cache->n_kv, f32)) {
+        e = tmoe::launch_kv4_attn(f32, cache->head_dim, x, planes, attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
+        return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "kv4 decode attention");
     }
     e = tmoe::launch_kv4_prefill(f32, cache->head_dim, x, planes, attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
     return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "kv4 prefill attention");
