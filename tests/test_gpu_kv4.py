@@ -425,6 +425,27 @@ def test_prefill_flat_and_peaked(gain):
     run_prefill("bf16", 128, 8, 2, 100, 60, gain=gain)
 
 
+def test_prefill_nan_query_stays_in_its_row():
+    rng = np.random.default_rng(12)
+    S, nh, nkv, hd, pos0 = 200, 8, 1, 128, 500
+    cache = tb.Kv4Cache(1, nkv, hd, pos0 + S)
+    K, V = fill(cache, rng)
+    q = randn(rng, (S, nh, hd), torch.bfloat16)
+    poisoned = q.clone()
+    poisoned[77, 3, 5] = float("nan")
+    poisoned[150, 6] = float("inf")
+    got = cache.prefill(poisoned.cuda(), None, None, pos0=pos0)
+    cache.check()
+    assert bool(got[77, 3].isnan().any())
+    Kt, Vt = K[0].transpose(1, 0, 2), V[0].transpose(1, 0, 2)
+    for i in (0, 76, 77, 78, 150, 199):
+        want, *m = R.attend(q[i].double().numpy(), Kt, Vt, pos0 + i, 0, 0, hd ** -0.5)
+        tol = prefill_tol("bf16", want, *m)
+        for h in range(nh):
+            if (i, h) not in ((77, 3), (150, 6)):
+                close(got[i, h], want[h], tol[h] if np.ndim(tol) else tol, f"token {i} head {h}")
+
+
 def test_prefill_rows_stored_before():
     run_prefill("bf16", 128, 8, 2, 45, 10, given=False)
 

@@ -197,7 +197,7 @@ struct KpNo {
     static constexpr bool value = false;
 };
 
-// Bounded waits: by one thread, or by a whole warp.  One that runs out latches the error and ends the role.
+// Bounded waits by a whole warp.  One that runs out latches the error and ends the role.
 #define KP_WAIT_WARP(bar, phase)                                                            \
     do {                                                                                    \
         if (!__all_sync(0xffffffffu, mbar_wait_bounded(&(bar), (uint32_t)(phase)))) {       \
@@ -205,14 +205,6 @@ struct KpNo {
             goto done;                                                                      \
         }                                                                                   \
     } while (0)
-#define KP_WAIT(bar, phase)                                  \
-    do {                                                     \
-        if (!mbar_wait_bounded(&(bar), (uint32_t)(phase))) { \
-            latch_error(a.err, TMOE_DEV_ERR_TIMEOUT);        \
-            goto done;                                       \
-        }                                                    \
-    } while (0)
-
 template <int HD, typename T>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4PrefillArgs a, const Kv4Planes c) {
     using Cfg = Kv4PrefillCfg<HD>;
@@ -737,12 +729,17 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
         // ------------------------------------------------------------ raw tiles by bulk copies
         if (lane == 0) {
             int i = 0;  // raw tiles before
-            for (; it.in_run(a, len); it.next(a)) {
+            bool ok = true;
+            for (; ok && it.in_run(a, len); it.next(a)) {
                 const int64_t head = ((int64_t)a.seq * c.n_kv + it.g) * c.n_ctx;
                 if (a.by_item && it.uncut()) a.cuts[it.g * a.blocks + it.blk] = KpCut{it.blk, it.g, -1, -1};
                 for (int j = 0; j < 2 * it.n; j++, i++) {
                     const int rs = i % KP_RAW;
-                    if (i >= KP_RAW) KP_WAIT(bars.raw_empty[rs], ((i / KP_RAW) - 1) & 1);
+                    if (i >= KP_RAW && !mbar_wait_bounded(&bars.raw_empty[rs], ((i / KP_RAW) - 1) & 1)) {
+                        latch_error(a.err, TMOE_DEV_ERR_TIMEOUT);
+                        ok = false;
+                        break;
+                    }
                     const int p0 = it.seen.tile(it.tile0 + (j >> 1)) * KP_N;
                     const int np = min(KP_N, c.n_ctx - p0);  // the cache may end inside the last tile (at 64)
                     uint8_t *dst = smem + Cfg::R + rs * Cfg::RAW;
@@ -752,10 +749,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                     bulk_g2s(dst + Cfg::CODES, (j & 1 ? c.vs : c.ks) + (head + p0) * NB, (uint32_t)(np * NB * 2), full);
                 }
             }
+            // whatever became of their readers, the CTA does not end before its copies
+            for (int k = max(i - KP_RAW, 0); k < i; k++)
+                mbar_wait_bounded(&bars.raw_full[k & 1][k % KP_RAW], ((k >> 1) / KP_RAW) & 1);
         }
         }
     }
 done:
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
     tc::fence_before();
     __syncthreads();
