@@ -361,7 +361,7 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4>::THREADS), (Kv
         const int heads = min(G - h0, KA_HEADS);
         const int64_t row0 = ((int64_t)(a.seq0 >= 0 ? a.seq0 : t) * c.n_kv + g) * c.n_ctx;
 
-        // ---- this warp's tiles: first + warp, first + warp + 8, ...  Lanes 0..3 copy a plane's piece each
+        // ---- this warp's tiles: first + warp, first + warp + WARPS, ...  Lanes 0..3 copy a plane's piece each
         const int mine = n_part > warp ? (n_part - warp + WARPS - 1) / WARPS : 0;
         const uint8_t *src;
         uint32_t piece, dst;
