@@ -4,6 +4,8 @@
 //   kv4_load_kernel    the same rows back as values
 //   kv4_attn_kernel    one query token per sequence (a decode step), its K/V row quantised into the
 //                      cache on the way; or a few tokens of one sequence
+#include <algorithm>
+
 #include "kernels.cuh"
 #include "kv4.cuh"
 
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
 //
 // Work: the tiles of all (token, KV head, pass) are one list, cut into equal runs, one per CTA: ragged
 // lengths, few sequences or many all load every SM the same.  A segment (one token, KV head and pass)
-// costs a CTA about KA_PART tiles' time to begin and to join, so that a segment counts that much more in
+// costs a CTA about PART tiles' time to begin and to join, so that a segment counts that much more in
 // the list; where the segments are few against the CTAs, each is instead padded to whole runs, and no
 // CTA has more than one (the cheaper of the two by its longest run).  A warp takes every WARPS-th tile of a
 // run, fetched by bulk copies into its own ring.  Runs that hold less than a segment leave partial sums in
@@ -139,7 +141,6 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
 // heads, 40 us, 3.8 TB/s.  What is left there: the SMs get unequal shares of the bandwidth (their even runs end 138 .. 150 us), and a part's start
 // and join are about 5 us.
 constexpr int KA_HEADS = 8;
-constexpr int KA_PART = 32;
 constexpr float KA_ROOM = 8.0f;  // how far (log2) a score may exceed its head's reference
 constexpr float KA_BIAS = 6.0f;  // P times the V scale is held below 2^(KA_BIAS + KA_ROOM)
 
@@ -156,7 +157,7 @@ struct Kv4AttnArgs {
     int *err;
 };
 
-template <int HD, bool PREC>
+template <int HD, bool PREC, bool SHORT>
 struct Kv4AttnCfg {
     static constexpr int NB = HD / 32;
     static constexpr int TILE = 64;  // positions; in tiles of 32 all of the cases below took 5 to 25% longer
@@ -165,8 +166,15 @@ struct Kv4AttnCfg {
     //   width 128, bf16, 64 x 32768 / 1 x 131071: 12 x 2, one CTA 149 / 39.8 us; 8 x 3, one 160 / 41.6; 6 x 2, two 157 / 42.4
     //   width 128, f32, 4 x 4096: 8 x 3, one CTA 11.1 us; 12 x 2, one 13.3; 6 x 2, two 15.3
     //   width 64, 16 heads over 16, 24 x 5003: 6 x 4, two CTAs 32.3 us; 12 x 4, one 37.2; 8 x 6, one 38.5
-    static constexpr int WARPS = HD == 64 ? 6 : PREC ? 8 : 12, STAGES = HD == 64 ? 4 : PREC ? 3 : 2;
-    static constexpr int CTAS = HD == 64 ? 2 : 1;
+    // SHORT: more segments than SMs, of 128 tiles at most each.  A CTA's start and join then come often, and run beside a second
+    // CTA's tiles: width 128, bf16, 6 x 2, two CTAs against 12 x 2, one, in 64 sequences of 1024 / 4096 / 8192 / 16384 positions
+    // 19.3 / 38.5 / 61.9 / 98.7 us against 21.4 / 41.8 / 61.9 / 96.1; f32, 4 x 3, two against 8 x 3, one, 21.3 / 50.1 / 83.9 / 137.0
+    // against 22.7 / 53.7 / 84.2 / 137.9.
+    static constexpr int WARPS = HD == 64 ? 6 : SHORT ? (PREC ? 4 : 6) : PREC ? 8 : 12, STAGES = HD == 64 ? 4 : PREC ? 3 : 2;
+    static constexpr int CTAS = HD == 64 || SHORT ? 2 : 1;
+    // In tiles, what a segment costs besides its own (f32's take longer): f32, 16 / 20 / 32 in 64 sequences of 8192 77.7 / 78.9 / 83.7
+    // us, 16 of 2048 15.6 / 13.9 / 13.9; bf16, 12 / 20 / 32 / 48 in 32 of 4096 (window, 40 heads over 8) 44.3 / 44.0 / 42.4 / 43.4.
+    static constexpr int PART = PREC ? 20 : 32;
     static constexpr int THREADS = 32 * WARPS;
     static constexpr int CODES = TILE * HD / 2, SCALES = TILE * NB * 2;
     static constexpr int STAGE = 2 * (CODES + SCALES);  // K codes, V codes, K scales, V scales
@@ -227,11 +235,12 @@ __device__ __forceinline__ uint32_t ka_codes(uint32_t u, uint32_t mask, __half2 
     return ka_u(__hsub2(ka_h2(r), off));
 }
 
-template <int HD, typename T>
-__global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4>::THREADS), (Kv4AttnCfg<HD, sizeof(T) == 4>::CTAS))
+template <int HD, typename T, bool SHORT>
+__global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREADS), (Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::CTAS))
     kv4_attn_kernel(const Kv4AttnArgs a, const Kv4Planes c) {
     constexpr bool PREC = sizeof(T) == 4;
-    using Cfg = Kv4AttnCfg<HD, PREC>;
+    using Cfg = Kv4AttnCfg<HD, PREC, SHORT>;
+    constexpr int PART = Cfg::PART;
     constexpr int NB = Cfg::NB, ST = Cfg::STAGES, RW = HD + 2, TILE = Cfg::TILE, HB = TILE / 16, WARPS = Cfg::WARPS;
     constexpr uint32_t M1 = 0x000f000fu, M16 = 0x00f000f0u;
     extern __shared__ __align__(128) uint8_t ka_smem[];
@@ -272,10 +281,10 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4>::THREADS), (Kv
     const int grid = gridDim.x;
     // runs of whole segments' pieces, a tile a warp at least; or runs over the list as it comes
     const int alone = live < grid ? max((total + grid - live - 1) / (grid - live), WARPS) : 0x7fffffff;
-    const int across = (int)(((int64_t)total + (int64_t)live * KA_PART + grid - 1) / grid);
+    const int across = (int)(((int64_t)total + (int64_t)live * PART + grid - 1) / grid);
     const bool pad = alone <= across;
     const int per = max(pad ? alone : across, 1);
-    auto length = [&](int n) { return n == 0 ? 0 : pad ? (n + per - 1) / per * per : n + KA_PART; };
+    auto length = [&](int n) { return n == 0 ? 0 : pad ? (n + per - 1) / per * per : n + PART; };
     int entries = 0;  // of the lane's tokens
 #pragma unroll 1
     for (int t = lane_t0; t < lane_t1; t++) entries += H * length(tiles_of(t));
@@ -345,10 +354,10 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4>::THREADS), (Kv
             const int each = seen.tiles / parts, more = seen.tiles - each * parts;
             first = i * each + min(i, more), n_part = each + (i < more);
         } else {
-            // its tiles are the entries from seg0 + KA_PART on
-            first = max(at - seg0 - KA_PART, 0);
-            n_part = upto - seg0 - KA_PART - first;
-            first_run = (seg0 + KA_PART) / per, parts = (seg0 + len - 1) / per - first_run + 1;
+            // its tiles are the entries from seg0 + PART on
+            first = max(at - seg0 - PART, 0);
+            n_part = upto - seg0 - PART - first;
+            first_run = (seg0 + PART) / per, parts = (seg0 + len - 1) / per - first_run + 1;
         }
         at = upto;
         const int t = tok, p_tok = p_new;
@@ -827,25 +836,21 @@ size_t kv4_attn_scratch_bytes(int sm_count) {
     return kv4_counter_bytes(sm_count) + (decode > prefill ? decode : prefill);
 }
 
-template <int HD, typename T>
-static cudaError_t attn_launch(Kv4Attn &x, const Kv4Planes &c, void *scratch, int sm_count, int *err, cudaStream_t st) {
-    using Cfg = Kv4AttnCfg<HD, sizeof(T) == 4>;
+template <int HD, typename T, bool SHORT>
+static cudaError_t attn_launch(const Kv4Attn &x, const Kv4Planes &c, int64_t segments, int64_t tiles, void *scratch, int sm_count,
+                               int *err, cudaStream_t st) {
+    using Cfg = Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>;
     static int set[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!set[dev]) {
         const cudaError_t e =
-            cudaFuncSetAttribute(kv4_attn_kernel<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+            cudaFuncSetAttribute(kv4_attn_kernel<HD, T, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
         if (e != cudaSuccess) return e;
         set[dev] = 1;
     }
     // as many CTAs as the most tiles that the cache allows need, at a tile a warp, and at most what is resident
-    const int G = x.n_head / c.n_kv, passes = (G + KA_HEADS - 1) / KA_HEADS;
-    const int most = x.window > 0 && x.window < c.n_ctx ? x.window + 2 * Cfg::TILE + x.n_sink : c.n_ctx;
-    const int64_t segments = (int64_t)x.n_tok * c.n_kv * passes;
-    const int64_t tiles = segments * (((most < c.n_ctx ? most : c.n_ctx) + Cfg::TILE - 1) / Cfg::TILE);
-    if (tiles + KA_PART * segments > (1ll << 30)) return cudaErrorInvalidValue;  // list positions are 32-bit
     const int64_t want = segments + (tiles + Cfg::WARPS - 1) / Cfg::WARPS, cap = (int64_t)Cfg::CTAS * sm_count;
     Kv4AttnArgs a;
     a.q = x.q, a.k = x.k, a.v = x.v, a.out = x.out;
@@ -855,18 +860,26 @@ static cudaError_t attn_launch(Kv4Attn &x, const Kv4Planes &c, void *scratch, in
     a.arrived = (int *)scratch;
     a.part = kv4_scratch_parts(scratch, sm_count);
     a.err = err;
-    return launch_k(kv4_attn_kernel<HD, T>, dim3((unsigned)(want < cap ? want : cap)), dim3(Cfg::THREADS),
+    return launch_k(kv4_attn_kernel<HD, T, SHORT>, dim3((unsigned)(want < cap ? want : cap)), dim3(Cfg::THREADS),
                     (size_t)Cfg::SMEM, st, a, c);
 }
 
 cudaError_t launch_kv4_attn(bool f32, int head_dim, Kv4Attn &x, const Kv4Planes &c, void *scratch, int sm_count,
                             int *err, cudaStream_t st) {
     if (x.n_tok <= 0) return cudaSuccess;
-    if (head_dim == 128)
-        return f32 ? attn_launch<128, float>(x, c, scratch, sm_count, err, st)
-                   : attn_launch<128, __nv_bfloat16>(x, c, scratch, sm_count, err, st);
-    return f32 ? attn_launch<64, float>(x, c, scratch, sm_count, err, st)
-               : attn_launch<64, __nv_bfloat16>(x, c, scratch, sm_count, err, st);
+    // the most tiles that a token can see, as far as the host knows
+    constexpr int TILE = 64;
+    const int G = x.n_head / c.n_kv, passes = (G + KA_HEADS - 1) / KA_HEADS;
+    int64_t most = x.pos ? c.n_ctx : x.pos0 + x.n_tok;
+    if (x.window > 0) most = std::min(most, (int64_t)x.window + 2 * TILE + x.n_sink);
+    const int64_t each = (std::min(most, (int64_t)c.n_ctx) + TILE - 1) / TILE;
+    const int64_t segments = (int64_t)x.n_tok * c.n_kv * passes, tiles = segments * each;
+    if (tiles + 32 * segments > (1ll << 30)) return cudaErrorInvalidValue;  // list positions are 32-bit
+    const bool few_tiles = segments > sm_count && each <= 128;
+    auto launch = [&](auto kernel) { return kernel(x, c, segments, tiles, scratch, sm_count, err, st); };
+    if (head_dim == 64) return launch(f32 ? attn_launch<64, float, false> : attn_launch<64, __nv_bfloat16, false>);
+    if (few_tiles) return launch(f32 ? attn_launch<128, float, true> : attn_launch<128, __nv_bfloat16, true>);
+    return launch(f32 ? attn_launch<128, float, false> : attn_launch<128, __nv_bfloat16, false>);
 }
 
 }  // namespace tmoe
