@@ -1,0 +1,28 @@
+"""How calls of the 4-bit KV cache follow one another: a refused one between two good ones."""
+import numpy as np
+import pytest
+import torch
+
+import tetraeder_b200 as tb
+from tests.test_gpu_kv4 import fill, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("first,other", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)])
+def test_a_refused_call_leaves_the_next_one_as_it_was(first, other):
+    rng = np.random.default_rng(21)
+    cache = tb.Kv4Cache(2, 2, 128, 256)
+    fill(cache, rng)
+    q, k, v = (randn(rng, (2, n, 128), first).cuda() for n in (8, 2, 2))
+    pos = torch.tensor([200, 77], dtype=torch.int32, device="cuda")
+    calls = [lambda q, k, v: cache.decode(q, k, v, pos), lambda q, k, v: cache.prefill(q, k, v, seq=1, pos0=99)]
+    for call in calls:
+        want = call(q, k, v).clone()
+        x = q.to(other)
+        for bad in (x[:, :, :64], x.transpose(0, 1), x.cpu(), x[0]):
+            with pytest.raises(ValueError):
+                call(bad, k.to(other), v.to(other))
+        assert torch.equal(call(q, k, v), want)
+        assert call(x, k.to(other), v.to(other)).dtype == other  # and the other type is taken once it is right
+    cache.check()

@@ -1,0 +1,103 @@
+"""Kv4Cache's host side without a GPU: CPU tensors and a stand-in for the library that keeps what each call is given."""
+import ctypes as C
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from tetraeder_b200 import _lib
+from tetraeder_b200.kv4 import Kv4Cache
+
+STREAM = SimpleNamespace(cuda_stream=0)
+
+
+class Lib:
+    """The C entry points: each keeps its arguments (the attention's as a copy of the struct) and succeeds."""
+
+    def __init__(self):
+        self.calls = []
+
+    def tmoe_kv4_attn_scratch_bytes(self, h):
+        return 64
+
+    def _attn(self, h, stream, cache, attn, *rest):
+        self.calls.append((h, _lib.Kv4AttnStruct.from_buffer_copy(C.string_at(attn, C.sizeof(_lib.Kv4AttnStruct))), rest))
+        return 0
+
+    def _rows(self, h, stream, cache, ty, *rest):
+        self.calls.append((h, ty, rest))
+        return 0
+
+    tmoe_kv4_attn_decode = tmoe_kv4_attn_prefill = _attn
+    tmoe_kv4_store = tmoe_kv4_load = _rows
+
+
+class Plane:
+    """A CPU tensor that passes for a CUDA one where the planes are checked."""
+
+    def __init__(self, t):
+        self._t = t
+
+    is_cuda = True
+
+    def __getattr__(self, name):
+        return getattr(self._t, name)
+
+
+def make(n_seq=2, n_kv=2, hd=128, ctx=64, layer=None):
+    layer = layer or SimpleNamespace(lib=Lib(), h=1, device=torch.device("cpu"))
+    planes = []
+    for _ in range(2):
+        planes += [Plane(torch.zeros((n_seq, n_kv, ctx, hd // 2), dtype=torch.uint8)),
+                   Plane(torch.zeros((n_seq, n_kv, ctx, hd // 32), dtype=torch.float16))]
+    cache = Kv4Cache.from_planes(*planes, layer=layer)
+    cache._dev = -1  # what a CPU tensor's get_device() says
+    return cache
+
+
+def rows(n, heads, dtype, hd=128):
+    return torch.zeros((n, heads, hd), dtype=dtype)
+
+
+POS = torch.zeros(2, dtype=torch.int32)
+REFUSED = [
+    ("width", lambda dt: rows(2, 4, dt, 64)),
+    ("strides", lambda dt: rows(4, 2, dt).transpose(0, 1)),
+    ("dimensions", lambda dt: rows(2, 4, dt)[0]),
+    ("device", lambda dt: rows(2, 4, dt).to("meta")),
+]
+
+
+@pytest.mark.parametrize("call", ["decode", "prefill"])
+@pytest.mark.parametrize("first,other", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("what,bad", REFUSED, ids=[r[0] for r in REFUSED])
+def test_a_refused_call_leaves_the_next_one_as_it_was(call, first, other, what, bad):
+    cache = make()
+
+    def run(q, dt):
+        k = rows(2, 2, dt)
+        if call == "decode":
+            cache.decode(q, k, k, POS, out=torch.empty_like(q), stream=STREAM)
+        else:
+            cache.prefill(q, k, k, out=torch.empty_like(q), stream=STREAM)
+
+    q = rows(2, 4, first)
+    run(q, first)
+    with pytest.raises(ValueError):
+        run(bad(other), other)
+    run(q, first)
+    (_, a, _), (_, b, _) = cache.lib.calls
+    for f in ("type", "n_head", "q_ld", "kv_ld", "out_ld"):
+        assert getattr(a, f) == getattr(b, f), f
+    run(rows(2, 4, other), other)  # and what was refused is taken once it is right
+    assert cache.lib.calls[2][1].type == (_lib.TYPE_F32 if other == torch.float32 else _lib.TYPE_BF16)
+
+
+def test_a_refused_load_is_refused_again():
+    cache = make()
+    cache.load(0, n=4, seq=0, dtype=torch.bfloat16, stream=STREAM)
+    for _ in range(2):
+        with pytest.raises(RuntimeError):
+            cache.load(0, n=-1, seq=0, stream=STREAM)
+    k, v = cache.load(0, n=3, seq=0, stream=STREAM)
+    assert k.shape == v.shape == (3, 2, 128) and k.dtype == torch.float32 and len(cache.lib.calls) == 2

@@ -171,8 +171,8 @@ class Kv4Cache:
         s, s0, p, p0 = self._place(n, pos, seq)
         sig = (n, dtype)
         if sig != self._row_sig:  # a shape to allocate by: no memory of its own
-            self._row_sig = sig
             self._row_like = torch.empty(1, dtype=dtype, device=self.device).expand(n, self.n_kv, self.head_dim)
+            self._row_sig = sig
         k, v = torch.empty_like(self._row_like), torch.empty_like(self._row_like)
         rc = self.lib.tmoe_kv4_load(self.h, self._stream(stream), self._cp, ty, k.data_ptr(), v.data_ptr(),
                                     self.n_kv * self.head_dim, s, s0, p, p0, n)
@@ -185,8 +185,8 @@ class Kv4Cache:
         a, n, dt = self._a, q.shape[0], q.dtype
         sig = (dt, q.shape, q.stride(), q.get_device())
         if sig != self._q_sig:
-            a.type = self._type(q)
-            a.q_ld, a.n_head = self._heads("q", q, n, dt), q.shape[1]
+            ty, ld = self._type(q), self._heads("q", q, n, dt)  # a refused q changes nothing
+            a.type, a.q_ld, a.n_head = ty, ld, q.shape[1]
             self._q_sig = sig
         if out is None:
             out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=self.device)
