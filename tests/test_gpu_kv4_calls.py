@@ -1,4 +1,4 @@
-"""How calls of the 4-bit KV cache follow one another: a refused one between two good ones."""
+"""How calls of the 4-bit KV cache follow one another: a refused one between two good ones, two caches on two streams."""
 import numpy as np
 import pytest
 import torch
@@ -26,3 +26,27 @@ def test_a_refused_call_leaves_the_next_one_as_it_was(first, other):
         assert torch.equal(call(q, k, v), want)
         assert call(x, k.to(other), v.to(other)).dtype == other  # and the other type is taken once it is right
     cache.check()
+
+
+def test_two_caches_on_two_unordered_streams():
+    """Each call splits its segments over many CTAs, whose parts meet in the scratch."""
+    rng = np.random.default_rng(30)
+    n = 9000
+    pos = torch.tensor([n - 1], dtype=torch.int32, device="cuda")
+    caches, q = [tb.Kv4Cache(1, 1, 128, n) for _ in range(2)], []
+    for c in caches:
+        fill(c, rng)
+        q.append(randn(rng, (1, 8, 128), torch.bfloat16).cuda())
+    p = randn(rng, (40, 8, 128), torch.bfloat16).cuda()
+    want = [(c.decode(x, None, None, pos).clone(), c.prefill(p, None, None, pos0=n - 40).clone()) for c, x in zip(caches, q)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in caches]
+    got = [[], []]
+    for _ in range(50):
+        for i, (c, x) in enumerate(zip(caches, q)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append((c.decode(x, None, None, pos), c.prefill(p, None, None, pos0=n - 40)))
+    torch.cuda.synchronize()
+    for i, c in enumerate(caches):
+        assert all(torch.equal(a, b) for pair in got[i] for a, b in zip(pair, want[i]))
+        c.check()

@@ -1,11 +1,12 @@
 """Kv4Cache's host side without a GPU: CPU tensors and a stand-in for the library that keeps what each call is given."""
 import ctypes as C
+import threading
 from types import SimpleNamespace
 
 import pytest
 import torch
 
-from tetraeder_b200 import _lib
+from tetraeder_b200 import _lib, kv4, moe
 from tetraeder_b200.kv4 import Kv4Cache
 
 STREAM = SimpleNamespace(cuda_stream=0)
@@ -44,8 +45,12 @@ class Plane:
         return getattr(self._t, name)
 
 
-def make(n_seq=2, n_kv=2, hd=128, ctx=64, layer=None):
-    layer = layer or SimpleNamespace(lib=Lib(), h=1, device=torch.device("cpu"))
+def a_layer(*args, **kw):
+    return SimpleNamespace(lib=Lib(), h=1, device=torch.device("cpu"))
+
+
+def make(n_seq=2, n_kv=2, hd=128, ctx=64, **kw):
+    layer = kw["layer"] if "layer" in kw else a_layer()
     planes = []
     for _ in range(2):
         planes += [Plane(torch.zeros((n_seq, n_kv, ctx, hd // 2), dtype=torch.uint8)),
@@ -101,3 +106,29 @@ def test_a_refused_load_is_refused_again():
             cache.load(0, n=-1, seq=0, stream=STREAM)
     k, v = cache.load(0, n=3, seq=0, stream=STREAM)
     assert k.shape == v.shape == (3, 2, 128) and k.dtype == torch.float32 and len(cache.lib.calls) == 2
+
+
+def test_caches_without_a_layer_have_a_scratch_each(monkeypatch):
+    monkeypatch.setattr(kv4, "_thread_layer", lambda device, layer=a_layer(): layer)
+    a, b = make(layer=None), make(layer=None)
+    assert a.layer is b.layer
+    assert a._scratch.data_ptr() != b._scratch.data_ptr()
+    q = rows(2, 4, torch.float32)
+    for cache in (a, b):
+        cache.decode(q, None, None, POS, out=q, stream=STREAM)
+    assert [c[1].scratch for c in a.lib.calls] == [a._scratch.data_ptr(), b._scratch.data_ptr()]
+    layer = a_layer()
+    c, d = make(layer=layer), make(layer=layer)  # a model's: one after the other anyway
+    assert c._scratch.data_ptr() == d._scratch.data_ptr()
+
+
+def test_each_thread_has_its_own_handle(monkeypatch):
+    monkeypatch.setattr(moe, "MoeLayer", a_layer)
+    monkeypatch.setattr(kv4, "_own", threading.local())
+    here = kv4._thread_layer(0)
+    assert kv4._thread_layer(0) is here and kv4._thread_layer(1) is not here
+    there = []
+    t = threading.Thread(target=lambda: there.append(kv4._thread_layer(0)))
+    t.start()
+    t.join()
+    assert there[0] is not here

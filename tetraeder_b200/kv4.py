@@ -11,6 +11,7 @@ Activations are float32 or bfloat16 CUDA tensors; a token's heads are contiguous
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -20,23 +21,25 @@ _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16}
 # the current stream's handle by device ordinal, without the Stream object where torch has the call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
-_layers: dict = {}  # device ordinal -> a small handle, for caches made without one
+_own = threading.local()  # .layers: device ordinal -> a small handle, for the caches that this thread makes without one
 
 
-def _default_layer(device: int):
+def _thread_layer(device: int):
     from .moe import MoeLayer
-    if device not in _layers:
-        _layers[device] = MoeLayer(512, 256, 8, 2, gate_type=_lib.TYPE_Q4_K, up_type=_lib.TYPE_Q4_K,
-                                   down_type=_lib.TYPE_Q4_K, max_tokens=4, device=device)
-    return _layers[device]
+    layers = _own.__dict__.setdefault("layers", {})
+    if device not in layers:
+        layers[device] = MoeLayer(512, 256, 8, 2, gate_type=_lib.TYPE_Q4_K, up_type=_lib.TYPE_Q4_K,
+                                  down_type=_lib.TYPE_Q4_K, max_tokens=4, device=device)
+    return layers[device]
 
 
 class Kv4Cache:
     """Planes k_codes, v_codes uint8 [n_seq, n_kv, capacity, head_dim / 2] and k_scales, v_scales float16
     [n_seq, n_kv, capacity, head_dim / 32]; capacity is n_ctx rounded up to a multiple of 64.  `layer` (a
-    MoeLayer) gives the handle whose device error flag the calls use; without one, caches of a device
-    share a small handle.  The caches of a handle share its attention scratch: like a handle's other calls,
-    theirs run on one stream, or on ordered ones."""
+    MoeLayer) gives the handle whose device error flag the calls use.  The caches of a layer share its attention
+    scratch (40 MB): like a handle's other calls, theirs come from one thread and run on one stream, or on
+    ordered ones.  A cache made without a layer has a scratch of its own, so that only its own calls have to be
+    ordered, and a small handle that it shares with such caches made by the same thread on the same device."""
 
     def __init__(self, n_seq: int, n_kv: int, head_dim: int, n_ctx: int, device: int | None = None, layer=None):
         if not torch.cuda.is_available():
@@ -75,17 +78,19 @@ class Kv4Cache:
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = planes
         self.n_seq, self.n_kv, self.head_dim, self.n_ctx = n_seq, n_kv, 2 * half, cap
         self.device = codes.device
-        self.layer = _default_layer(codes.device.index) if layer is None else layer
+        self.layer = _thread_layer(codes.device.index) if layer is None else layer
         if self.layer.device != self.device:
             raise ValueError("the layer's handle is of another device")
         self.lib, self.h = self.layer.lib, self.layer.h
         self._c = _lib.Kv4CacheStruct(*(t.data_ptr() for t in planes), n_seq, n_kv, self.head_dim, cap)
         self._cp = C.addressof(self._c)
-        self._scratch = getattr(self.layer, "_kv4_scratch", None)
+        self._scratch = getattr(layer, "_kv4_scratch", None)
         if self._scratch is None:
             n = self.lib.tmoe_kv4_attn_scratch_bytes(self.h)
             _lib.check(n if n < 0 else 0, self.h)
-            self._scratch = self.layer._kv4_scratch = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            self._scratch = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            if layer is not None:
+                layer._kv4_scratch = self._scratch
         self._a = _lib.Kv4AttnStruct()
         self._a.scratch = self._scratch.data_ptr()
         self._ap = C.addressof(self._a)
