@@ -1,4 +1,5 @@
-"""How calls of the 4-bit KV cache follow one another: a refused one between two good ones, two caches on two streams."""
+"""How calls of the 4-bit KV cache follow one another: a refused one between two good ones, two caches on two streams, a new
+cache on another stream than the one that made it."""
 import numpy as np
 import pytest
 import torch
@@ -50,3 +51,26 @@ def test_two_caches_on_two_unordered_streams():
     for i, c in enumerate(caches):
         assert all(torch.equal(a, b) for pair in got[i] for a, b in zip(pair, want[i]))
         c.check()
+
+
+def test_a_new_cache_may_be_used_on_another_stream_at_once():
+    """Its planes and its scratch are zero by then, although the stream that zeroes them is busy."""
+    hd, n = 128, 5000
+    x = torch.ones((1, 1, hd), device="cuda")
+    q = torch.ones((1, 8, hd), device="cuda")
+    pos = torch.tensor([n - 1], dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    junk = [torch.full((64 << 20,), 255, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    del junk  # what the allocator hands out next holds ones
+    torch.cuda._sleep(100_000_000)
+    cache = tb.Kv4Cache(1, 1, hd, n)
+    with torch.cuda.stream(side):
+        cache.decode(q, x, x, pos, out=out)
+    side.synchronize()
+    first = out.clone()
+    assert int(cache.k_scales.count_nonzero()) == hd // 32  # the new row's alone
+    for _ in range(3):
+        assert torch.equal(cache.decode(q, x, x, pos), first)
+    cache.check()

@@ -33,6 +33,14 @@ class Lib:
     tmoe_kv4_store = tmoe_kv4_load = _rows
 
 
+@pytest.fixture(autouse=True)
+def settled(monkeypatch):
+    """The devices whose stream a constructor waited for."""
+    seen = []
+    monkeypatch.setattr(kv4, "_settle", seen.append)
+    return seen
+
+
 class Plane:
     """A CPU tensor that passes for a CUDA one where the planes are checked."""
 
@@ -132,3 +140,11 @@ def test_each_thread_has_its_own_handle(monkeypatch):
     t.start()
     t.join()
     assert there[0] is not here
+
+
+def test_a_new_scratch_is_zero_before_a_call_on_any_stream(settled):
+    layer = a_layer()
+    cache = make(layer=layer)
+    assert settled == [cache.device]
+    make(layer=layer)
+    assert len(settled) == 1  # that scratch was waited for

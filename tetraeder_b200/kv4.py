@@ -33,6 +33,13 @@ def _thread_layer(device: int):
     return layers[device]
 
 
+def _settle(device):
+    """Waits for memory just zeroed on the current stream: a call may be on any other one."""
+    with torch.cuda.device(device):
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream().synchronize()
+
+
 class Kv4Cache:
     """Planes k_codes, v_codes uint8 [n_seq, n_kv, capacity, head_dim / 2] and k_scales, v_scales float16
     [n_seq, n_kv, capacity, head_dim / 32]; capacity is n_ctx rounded up to a multiple of 64.  `layer` (a
@@ -56,6 +63,7 @@ class Kv4Cache:
             planes.append(torch.zeros((n_seq, n_kv, cap, head_dim // 2), dtype=torch.uint8, device=dev))
             planes.append(torch.zeros((n_seq, n_kv, cap, head_dim // 32), dtype=torch.float16, device=dev))
         self._set(planes, layer)
+        _settle(dev)
 
     @classmethod
     def from_planes(cls, k_codes, k_scales, v_codes, v_scales, layer=None) -> "Kv4Cache":
@@ -91,6 +99,7 @@ class Kv4Cache:
             self._scratch = torch.zeros(n, dtype=torch.uint8, device=self.device)
             if layer is not None:
                 layer._kv4_scratch = self._scratch
+            _settle(self.device)
         self._a = _lib.Kv4AttnStruct()
         self._a.scratch = self._scratch.data_ptr()
         self._ap = C.addressof(self._a)
