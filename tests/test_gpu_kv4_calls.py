@@ -1,5 +1,5 @@
 """How calls of the 4-bit KV cache follow one another: a refused one between two good ones, two caches on two streams, a new
-cache on another stream than the one that made it."""
+cache on another stream than the one that made it, outputs written on another stream than the current one."""
 import numpy as np
 import pytest
 import torch
@@ -73,4 +73,30 @@ def test_a_new_cache_may_be_used_on_another_stream_at_once():
     assert int(cache.k_scales.count_nonzero()) == hd // 32  # the new row's alone
     for _ in range(3):
         assert torch.equal(cache.decode(q, x, x, pos), first)
+    cache.check()
+
+
+def test_an_output_does_not_take_memory_that_the_current_stream_still_reads():
+    rng = np.random.default_rng(40)
+    B, hd, n = 16, 128, 128
+    cache = tb.Kv4Cache(B, 1, hd, n)
+    fill(cache, rng)
+    q = randn(rng, (B, 64, hd), torch.float32).cuda()
+    pos = torch.full((B,), n - 1, dtype=torch.int32, device="cuda")
+    want = cache.decode(q, None, None, pos).clone()
+    wk, _ = cache.load(0, n=100, seq=0)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for call, shape in ((lambda: cache.decode(q, None, None, pos, stream=side), q.shape),
+                        (lambda: cache.load(0, n=100, seq=0, stream=side)[0], wk.shape)):
+        x = torch.full(shape, 7.0, device="cuda")
+        torch.cuda.synchronize()
+        torch.cuda._sleep(100_000_000)
+        y = x.clone()  # runs after the sleep
+        del x          # the next block of this size on the current stream is x's
+        got = call()
+        side.synchronize()
+        torch.cuda.synchronize()
+        assert bool((y == 7.0).all())
+        assert torch.equal(got, want if got.shape == want.shape else wk)
     cache.check()

@@ -38,6 +38,7 @@ def settled(monkeypatch):
     """The devices whose stream a constructor waited for."""
     seen = []
     monkeypatch.setattr(kv4, "_settle", seen.append)
+    monkeypatch.setattr(kv4, "_raw_stream", lambda device: 0)
     return seen
 
 
@@ -108,11 +109,11 @@ def test_a_refused_call_leaves_the_next_one_as_it_was(call, first, other, what, 
 
 def test_a_refused_load_is_refused_again():
     cache = make()
-    cache.load(0, n=4, seq=0, dtype=torch.bfloat16, stream=STREAM)
+    cache.load(0, n=4, seq=0, dtype=torch.bfloat16)
     for _ in range(2):
         with pytest.raises(RuntimeError):
-            cache.load(0, n=-1, seq=0, stream=STREAM)
-    k, v = cache.load(0, n=3, seq=0, stream=STREAM)
+            cache.load(0, n=-1, seq=0)
+    k, v = cache.load(0, n=3, seq=0)
     assert k.shape == v.shape == (3, 2, 128) and k.dtype == torch.float32 and len(cache.lib.calls) == 2
 
 
@@ -148,3 +149,44 @@ def test_a_new_scratch_is_zero_before_a_call_on_any_stream(settled):
     assert settled == [cache.device]
     make(layer=layer)
     assert len(settled) == 1  # that scratch was waited for
+
+
+def test_outputs_belong_to_the_stream_that_writes_them(monkeypatch):
+    cache, q = make(), rows(2, 4, torch.float32)
+    within, noted = [], []
+
+    class On:
+        def __init__(self, stream):
+            self.stream = stream
+
+        def __enter__(self):
+            within.append(self.stream)
+
+        def __exit__(self, *exc):
+            within.append(None)
+
+    empty_like = torch.empty_like
+
+    class Out:
+        def __init__(self, t, stream):
+            self.t, self.stream = t, stream
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+        def record_stream(self, stream):
+            noted.append(stream)
+
+    made = []
+
+    def new(t, **kw):
+        made.append(within[-1] if within else None)
+        return Out(empty_like(t, **kw), made[-1])
+
+    monkeypatch.setattr(torch.cuda, "stream", On)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: "current")
+    monkeypatch.setattr(torch, "empty_like", new)
+    cache.decode(q, None, None, POS, stream=STREAM)
+    cache.prefill(q, None, None, stream=STREAM)
+    cache.load(POS, stream=STREAM)
+    assert made == [STREAM] * 4 and noted == ["current"] * 4

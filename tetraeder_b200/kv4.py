@@ -145,6 +145,16 @@ class Kv4Cache:
     def _stream(self, stream):
         return _raw_stream(self._dev) if stream is None else stream.cuda_stream
 
+    def _new(self, like, stream):
+        """A tensor of that shape for a call's output.  Its memory is the stream's that writes it: a block that the current
+        stream has just freed may still be in use there.  The current stream, whose caller reads it, is noted too."""
+        if stream is None:
+            return torch.empty_like(like, memory_format=torch.contiguous_format)
+        with torch.cuda.stream(stream):
+            out = torch.empty_like(like, memory_format=torch.contiguous_format)
+        out.record_stream(torch.cuda.current_stream(self.device))
+        return out
+
     @staticmethod
     def _type(t):
         if t.dtype not in _TYPES:
@@ -187,7 +197,7 @@ class Kv4Cache:
         if sig != self._row_sig:  # a shape to allocate by: no memory of its own
             self._row_like = torch.empty(1, dtype=dtype, device=self.device).expand(n, self.n_kv, self.head_dim)
             self._row_sig = sig
-        k, v = torch.empty_like(self._row_like), torch.empty_like(self._row_like)
+        k, v = self._new(self._row_like, stream), self._new(self._row_like, stream)
         rc = self.lib.tmoe_kv4_load(self.h, self._stream(stream), self._cp, ty, k.data_ptr(), v.data_ptr(),
                                     self.n_kv * self.head_dim, s, s0, p, p0, n)
         if rc:
@@ -195,7 +205,7 @@ class Kv4Cache:
         return k, v
 
     # -- attention -------------------------------------------------------------------------
-    def _attn(self, q, k, v, window, n_sink, scale, out):
+    def _attn(self, q, k, v, window, n_sink, scale, out, stream):
         a, n, dt = self._a, q.shape[0], q.dtype
         sig = (dt, q.shape, q.stride(), q.get_device())
         if sig != self._q_sig:
@@ -203,7 +213,7 @@ class Kv4Cache:
             a.type, a.q_ld, a.n_head = ty, ld, q.shape[1]
             self._q_sig = sig
         if out is None:
-            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=self.device)
+            out = self._new(q, stream)
             a.out_ld = q.shape[1] * self.head_dim
         else:
             a.out_ld = self._heads("out", out, n, dt, q.shape[1])
@@ -224,7 +234,7 @@ class Kv4Cache:
         (None: stored already) at pos[b] (int32 CUDA [B]; negative: no token, zeros come out).  Each query
         attends to positions 0..pos[b] of its sequence, with window > 0 to the last `window` of them and the
         first n_sink.  Returns out [B, n_head, head_dim]."""
-        out = self._attn(q, k, v, window, n_sink, scale, out)
+        out = self._attn(q, k, v, window, n_sink, scale, out, stream)
         B = q.shape[0]
         rc = self.lib.tmoe_kv4_attn_decode(self.h, self._stream(stream), self._cp, self._ap, self._index("pos", pos, B), B)
         if rc:
@@ -236,7 +246,7 @@ class Kv4Cache:
         """S new tokens of sequence `seq` at positions pos0 .. pos0 + S - 1: rows k, v [S, n_kv, head_dim] are stored
         (None: stored already), then query i of q [S, n_head, head_dim] attends to positions 0 .. pos0 + i (or
         its window and sinks).  Returns out [S, n_head, head_dim]."""
-        out = self._attn(q, k, v, window, n_sink, scale, out)
+        out = self._attn(q, k, v, window, n_sink, scale, out, stream)
         rc = self.lib.tmoe_kv4_attn_prefill(self.h, self._stream(stream), self._cp, self._ap, seq, pos0, q.shape[0])
         if rc:
             _lib.check(rc, self.h)
