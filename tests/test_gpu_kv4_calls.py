@@ -1,5 +1,6 @@
 """How calls of the 4-bit KV cache follow one another: a refused one between two good ones, two caches on two streams, a new
-cache on another stream than the one that made it, outputs written on another stream than the current one."""
+cache on another stream than the one that made it, outputs written on another stream than the current one, calls after the
+layer was closed."""
 import numpy as np
 import pytest
 import torch
@@ -100,3 +101,16 @@ def test_an_output_does_not_take_memory_that_the_current_stream_still_reads():
         assert bool((y == 7.0).all())
         assert torch.equal(got, want if got.shape == want.shape else wk)
     cache.check()
+
+
+def test_calls_after_the_layer_was_closed_are_refused():
+    layer = tb.MoeLayer(512, 256, 8, 2, max_tokens=4)
+    cache = tb.Kv4Cache(2, 2, 128, 64, layer=layer)
+    q, k = torch.zeros((2, 4, 128), device="cuda"), torch.zeros((2, 2, 128), device="cuda")
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    cache.decode(q, k, k, pos)
+    layer.close()
+    for call in (lambda: cache.decode(q, k, k, pos), lambda: cache.prefill(q, k, k), lambda: cache.store(k, k, pos),
+                 lambda: cache.load(pos), cache.check):
+        with pytest.raises(tb.TmoeError, match="TMOE_E_INVALID"):
+            call()

@@ -190,3 +190,16 @@ def test_outputs_belong_to_the_stream_that_writes_them(monkeypatch):
     cache.prefill(q, None, None, stream=STREAM)
     cache.load(POS, stream=STREAM)
     assert made == [STREAM] * 4 and noted == ["current"] * 4
+
+
+def test_a_closed_layer_gives_its_caches_no_handle():
+    layer = a_layer()
+    cache, q = make(layer=layer), rows(2, 4, torch.float32)
+    calls = [lambda: cache.decode(q, None, None, POS, out=q), lambda: cache.prefill(q, None, None, out=q),
+             lambda: cache.store(rows(2, 2, torch.float32), rows(2, 2, torch.float32), POS), lambda: cache.load(POS)]
+    for call in calls:
+        call()
+    layer.h = None  # as MoeLayer.close leaves it
+    for call in calls:
+        call()
+    assert [c[0] for c in cache.lib.calls] == [1] * 4 + [None] * 4

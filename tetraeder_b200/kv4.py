@@ -89,7 +89,7 @@ class Kv4Cache:
         self.layer = _thread_layer(codes.device.index) if layer is None else layer
         if self.layer.device != self.device:
             raise ValueError("the layer's handle is of another device")
-        self.lib, self.h = self.layer.lib, self.layer.h
+        self.lib = self.layer.lib
         self._c = _lib.Kv4CacheStruct(*(t.data_ptr() for t in planes), n_seq, n_kv, self.head_dim, cap)
         self._cp = C.addressof(self._c)
         self._scratch = getattr(layer, "_kv4_scratch", None)
@@ -106,6 +106,11 @@ class Kv4Cache:
         self._dev, self._scale = self.device.index, self.head_dim ** -0.5
         self._q_sig = self._kv_sig = self._row_sig = None
         self._kv_ld = 0
+
+    @property
+    def h(self):
+        """The layer's handle: none once the layer is closed, which the library refuses."""
+        return self.layer.h
 
     @property
     def nbytes(self) -> int:
