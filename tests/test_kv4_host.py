@@ -203,3 +203,16 @@ def test_a_closed_layer_gives_its_caches_no_handle():
     for call in calls:
         call()
     assert [c[0] for c in cache.lib.calls] == [1] * 4 + [None] * 4
+
+
+@pytest.mark.parametrize("x", [1 << 32, (1 << 32) + 5, 1 << 31, -(1 << 31) - 1, -(1 << 32)])
+def test_numbers_past_32_bits_are_refused(x):
+    cache, q, k = make(), rows(2, 4, torch.float32), rows(2, 2, torch.float32)
+    for call in (lambda: cache.decode(q, None, None, POS, out=q, window=x), lambda: cache.decode(q, None, None, POS, out=q, n_sink=x),
+                 lambda: cache.decode(q, None, None, POS, out=q, window=8, n_sink=x),
+                 lambda: cache.prefill(q, None, None, out=q, seq=x), lambda: cache.prefill(q, None, None, out=q, pos0=x),
+                 lambda: cache.prefill(q, None, None, out=q, window=x), lambda: cache.store(k, k, x, seq=0),
+                 lambda: cache.store(k, k, 0, seq=x), lambda: cache.load(x, n=1, seq=0)):
+        with pytest.raises(ValueError):
+            call()
+    assert not cache.lib.calls

@@ -40,6 +40,13 @@ def _settle(device):
             torch.cuda.current_stream().synchronize()
 
 
+def _int32(**values):
+    """Numbers that the C calls take in 32 bits: ctypes would pass on the low ones of any other."""
+    for name, x in values.items():
+        if not -1 << 31 <= x < 1 << 31:
+            raise ValueError(f"{name} is {x}")
+
+
 class Kv4Cache:
     """Planes k_codes, v_codes uint8 [n_seq, n_kv, capacity, head_dim / 2] and k_scales, v_scales float16
     [n_seq, n_kv, capacity, head_dim / 32]; capacity is n_ctx rounded up to a multiple of 64.  `layer` (a
@@ -139,6 +146,8 @@ class Kv4Cache:
     def _place(self, n, pos, seq):
         """(seq, seq0, pos, pos0) of the C calls."""
         p, pos0 = (self._index("pos", pos, n), 0) if torch.is_tensor(pos) else (None, int(pos))
+        if p is None:
+            _int32(pos=pos0)
         if torch.is_tensor(seq):
             return self._index("seq", seq, n), 0, p, pos0
         if seq is None and p is None:
@@ -230,6 +239,8 @@ class Kv4Cache:
         else:
             raise ValueError("k and v come together")
         a.q, a.out = q.data_ptr(), out.data_ptr()
+        if window or n_sink:
+            _int32(window=window, n_sink=n_sink)
         a.window, a.n_sink = window, n_sink
         a.scale = self._scale if scale is None else scale
         return out
@@ -251,6 +262,7 @@ class Kv4Cache:
         """S new tokens of sequence `seq` at positions pos0 .. pos0 + S - 1: rows k, v [S, n_kv, head_dim] are stored
         (None: stored already), then query i of q [S, n_head, head_dim] attends to positions 0 .. pos0 + i (or
         its window and sinks).  Returns out [S, n_head, head_dim]."""
+        _int32(seq=seq, pos0=pos0)
         out = self._attn(q, k, v, window, n_sink, scale, out, stream)
         rc = self.lib.tmoe_kv4_attn_prefill(self.h, self._stream(stream), self._cp, self._ap, seq, pos0, q.shape[0])
         if rc:
