@@ -126,8 +126,9 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
 //     reduction over the warp.
 // Precision: Q is scaled by a power of two per head into f16's upper range; bf16 queries then are exact.
 // f32 queries, and P with them, are split into high + low f16 parts, in two products.  P times the V scale is
-// held relative to the reference and to the largest V scale seen, so that small scales do not end in
-// f16's subnormals; for bf16 it is f16 (2^-12 relative, below the output's own 2^-9).
+// held relative to the reference and to the largest V scale seen in the same block of 32 dimensions, so that neither small
+// scales nor another block's large ones leave it in f16's subnormals.  For bf16 P is rounded to f16, and its product with the
+// scale again (2^-11 relative each, below the output's own 2^-8).  A scale below 2^-14 of its block's largest loses last bits there.
 //
 // Work: the tiles of all (token, KV head, pass) are one list, cut into equal runs, one per CTA: ragged
 // lengths, few sequences or many all load every SM the same.  A segment (one token, KV head and pass)
@@ -467,8 +468,15 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
             for (int i = 0; i < 2; i++) o[b][i][0] = o[b][i][1] = o[b][i][2] = o[b][i][3] = 0.0f;
         // of heads 2 t4 + {0, 1}: the reference, the sum over this thread's positions
         float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-        uint32_t v_top = 0;  // the largest V scale seen, as f16 bits; V scales are below 2^v_exp
-        int v_exp = 0;
+        // Of each block of 32 values, a pair of them a word: the f16 power of two that takes every V scale seen below 1.
+        // O is held times it
+        uint32_t room[NB / 2];
+#pragma unroll
+        for (int b = 0; b < NB / 2; b++) room[b] = 0x74007400u;  // 2^14
+        auto room_of = [&](int b) {
+            const float2 r = ka_float2(room[b / 2]);
+            return b & 1 ? r.y : r.x;
+        };
         bool dead = false;
 
         for (int j = 0; j < filled; j++) {
@@ -596,18 +604,34 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
                     for (int hb = 1; hb < HB; hb++) mx[i] = fmaxf(mx[i], fmaxf(s[hb][i], s[hb][2 + i]));
                     mx[i] *= to_log2[i];
                 }
-                uint32_t dm = 0;  // the largest of this lane's share of V scales
+                // this lane's share of the V scales, each times its block's factor: the largest
+                uint32_t dm = 0;
 #pragma unroll
                 for (int i = 0; i < Cfg::SCALES; i += 256) {
                     const uint2 u = *reinterpret_cast<const uint2 *>(stage_p + Cfg::VSCALES + i + lane * 8);
-                    dm = __vmaxu2(dm, __vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu));
+                    dm = __vmaxu2(dm, ka_u(__hmul2(ka_h2(u.x & 0x7fff7fffu), ka_h2(room[0]))));
+                    dm = __vmaxu2(dm, ka_u(__hmul2(ka_h2(u.y & 0x7fff7fffu), ka_h2(room[NB / 2 - 1]))));
                 }
-                dm = max(dm & 0xffffu, dm >> 16);
-                if (__any_sync(0xffffffffu, mx[0] > ref[0] + KA_ROOM || mx[1] > ref[1] + KA_ROOM || dm > v_top)) {
-                    float f[2];
-                    v_top = max(v_top, __reduce_max_sync(0xffffffffu, dm));
-                    const int v_old = v_exp;
-                    v_exp = (int)(v_top >> 10) - 14;  // f16 bits e, m: the value is below 2^(e - 14)
+                const bool v_more = (dm + 0x04000400u) & 0xc000c000u;  // 1 (0x3c00) and more
+                if (__any_sync(0xffffffffu, mx[0] > ref[0] + KA_ROOM || mx[1] > ref[1] + KA_ROOM || v_more)) {
+                    float f[2], fv[NB];
+#pragma unroll
+                    for (int b = 0; b < NB / 2; b++) {
+                        uint32_t d = 0;
+#pragma unroll
+                        for (int i = 0; i < Cfg::SCALES; i += 256) {
+                            const uint2 u = *reinterpret_cast<const uint2 *>(stage_p + Cfg::VSCALES + i + lane * 8);
+                            d = __vmaxu2(d, (b ? u.y : u.x) & 0x7fff7fffu);
+                            if (NB == 2) d = __vmaxu2(d, u.y & 0x7fff7fffu);
+                        }
+                        // f16 bits e, m: below 2^(e - 14)
+                        const int e0 = (int)(__reduce_max_sync(0xffffffffu, d & 0xffffu) >> 10);
+                        const int e1 = (int)(__reduce_max_sync(0xffffffffu, d >> 16) >> 10);
+                        const float2 r = ka_float2(room[b]);
+                        const float r0 = fminf(r.x, kv4_pow2(14 - e0)), r1 = fminf(r.y, kv4_pow2(14 - e1));
+                        room[b] = kv4_half2(r0, r1);
+                        fv[2 * b] = r0 * kv4_inv_pow2(r.x), fv[2 * b + 1] = r1 * kv4_inv_pow2(r.y);
+                    }
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
 #pragma unroll
@@ -616,14 +640,13 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
                         f[i] = ref[i] == -INFINITY ? 0.0f : kv4_exp2(ref[i] - next);
                         ref[i] = next;
                         l[i] *= f[i];
-                        f[i] *= kv4_pow2(v_old - v_exp);  // O is held times 2^-v_exp
                     }
 #pragma unroll
                     for (int b = 0; b < NB; b++)
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            o[b][i][0] *= f[0], o[b][i][1] *= f[1];
-                            o[b][i][2] *= f[0], o[b][i][3] *= f[1];
+                            o[b][i][0] *= f[0] * fv[b], o[b][i][1] *= f[1] * fv[b];
+                            o[b][i][2] *= f[0] * fv[b], o[b][i][3] *= f[1] * fv[b];
                         }
                 }
                 // ---- P (rows positions, columns heads); f32: exact exponents, else 2^KA_BIAS at the reference
@@ -638,8 +661,9 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
                         l[i & 1] += s[hb][i];
                     }
                 // ---- O^T += (V^T - 8) (P d): 16 positions a step
-                const float room = kv4_pow2(-v_exp);
-                const __half2 room2 = __float2half2_rn(room);
+                float rf[NB];
+#pragma unroll
+                for (int b = 0; b < NB; b++) rf[b] = 64.0f * room_of(b);
 #pragma unroll
                 for (int hb = 0; hb < HB; hb++) {
                     uint32_t ph[NB][2], pl[PREC ? NB : 1][2];  // positions 2 t4 + {0, 1} and + 8, column head gr
@@ -647,10 +671,11 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
                         const uint8_t *vs = stage_p + Cfg::VSCALES + (16 * hb + gr) * NB * 2;
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            const float x = s[hb][2 * i] * (room * 64.0f), y = s[hb][2 * i + 1] * (room * 64.0f);
+                            const float x = s[hb][2 * i], y = s[hb][2 * i + 1];
 #pragma unroll
                             for (int b = 0; b < NB; b += 2) {
-                                const float2 d = ka_float2(*reinterpret_cast<const uint32_t *>(vs + (8 * i * NB + b) * 2));
+                                float2 d = ka_float2(*reinterpret_cast<const uint32_t *>(vs + (8 * i * NB + b) * 2));
+                                d.x *= rf[b], d.y *= rf[b + 1];
                                 uint32_t u, v;
                                 ka_split(x * d.x, y * d.x, u, v);
                                 ph[b][i] = ka_transpose(u), pl[b][i] = ka_transpose(v);
@@ -672,9 +697,11 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
                                 d[0] = u.x, d[1] = u.y;
                             }
 #pragma unroll
+                            for (int b = 0; b < NB; b++) d[b] = ka_u(__hmul2(ka_h2(d[b]), ka_h2(room[b % (NB / 2)])));
+#pragma unroll
                             for (int b = 0; b < NB; b++) {
                                 const uint32_t dd = __byte_perm(d[b / 2], d[NB / 2 + b / 2], b & 1 ? 0x7632 : 0x5410);
-                                ph[b][i] = ka_u(__hmul2(p, __hmul2(ka_h2(dd), room2)));
+                                ph[b][i] = ka_u(__hmul2(p, ka_h2(dd)));
                             }
                         }
                     }
@@ -714,15 +741,15 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             float *r = sums + (warp * KA_HEADS + 2 * t4 + i) * RW;
-            const float f = (PREC ? 0.015625f : 1.0f) * kv4_pow2(v_exp);
             if (gr == 0) r[0] = ref[i], r[1] = l[i];
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+            for (int b = 0; b < NB; b++) {
+                const float f = (PREC ? 0.015625f : 1.0f) * kv4_inv_pow2(room_of(b));
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
+                for (int e = 0; e < 2; e++)
                     *reinterpret_cast<float2 *>(r + 2 + 32 * b + 4 * gr + 2 * e) =
                         make_float2(o[b][e][i] * f, o[b][e][2 + i] * (f * 0.0625f));
-                }
+            }
         }
         __syncthreads();
         const bool split = parts > 1;

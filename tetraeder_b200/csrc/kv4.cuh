@@ -119,6 +119,8 @@ __device__ __forceinline__ uint32_t kv4_half2(float lo, float hi) {
 }
 // 2^e, e in [-126, 127]
 __device__ __forceinline__ float kv4_pow2(int e) { return __int_as_float((127 + e) << 23); }
+// 1 / p, p = 2^e for e in [-126, 126]
+__device__ __forceinline__ float kv4_inv_pow2(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
 __device__ __forceinline__ float kv4_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
