@@ -36,6 +36,44 @@ def prefill_block_tol(dtype, want, smax, sabs, vblock):
     return tol if dtype == "f32" else tol + 2.0 ** -8 * np.abs(want)
 
 
+# ------------------------------------------------------------------ scores far from 1
+def run_far(dtype, hd, tokens, gain, gain2=1.0):
+    """The softmax takes the one position of the largest score alone, where the next one is further away than the scores' own
+    relative error (2^-8 is allowed for it, Q and K in f16 the coarsest).  The output is that position's V, with the roundings of
+    P and V (prefill, past 128 tokens here) or of P and its product (bf16 decode) to f16, 2^-11 each, and of the output to bf16,
+    2^-8; f32 decode holds both to 22 bits, and 2^-20 covers its few roundings."""
+    rng = np.random.default_rng(hd + tokens)
+    nh, n = 8, 400
+    cache = tb.Kv4Cache(1, 1, hd, n)
+    K, V = (x[0, 0] for x in fill(cache, rng))
+    q = (randn(rng, (tokens, nh, hd), torch.float32) * gain * gain2).to(DT[dtype])
+    first = n - tokens
+    if tokens == 1:
+        got = cache.decode(q.cuda(), None, None, torch.tensor([n - 1], dtype=torch.int32, device="cuda"))
+    else:
+        got = cache.prefill(q.cuda(), None, None, pos0=first)
+    cache.check()
+    rel = 2.0 ** -20 if dtype == "f32" and tokens <= 128 else 2 * 2.0 ** -11 + (2.0 ** -8 if dtype == "bf16" else 0.0)
+    checked = 0
+    for t in range(tokens):
+        s = q[t].double().numpy() @ K[:first + t + 1].T
+        best = s.argmax(1)
+        top2 = np.sort(s, axis=1)[:, -2:]
+        for h in np.flatnonzero(top2[:, 1] - top2[:, 0] > 2.0 ** -8 * np.abs(q[t].double().numpy()).max(1) * np.abs(K).max()):
+            close(got[t, h], V[best[h]], rel * np.abs(V[best[h]]), f"token {t} head {h}")
+            checked += 1
+    assert checked > tokens * nh // 2
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("tokens", [1, 70, 200])
+@pytest.mark.parametrize("log2", [26, 32, 60, 100])
+def test_scores_past_24_bits(dtype, hd, tokens, log2):
+    """A score's last bit counts 1 and more."""
+    run_far(dtype, hd, tokens, 2.0 ** log2)
+
+
 # ------------------------------------------------------------------ V blocks of very different scales
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("hd,nh,nkv", [(128, 8, 1), (64, 6, 2), (128, 20, 2)])

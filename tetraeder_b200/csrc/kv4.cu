@@ -247,6 +247,7 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
     extern __shared__ __align__(128) uint8_t ka_smem[];
     uint64_t *bars = reinterpret_cast<uint64_t *>(ka_smem + Cfg::RING);
     __shared__ int sh_last;
+    __shared__ float sh_up[Cfg::WARPS][KA_HEADS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t4 = lane & 3;
     const int G = a.n_head / c.n_kv, passes = (G + KA_HEADS - 1) / KA_HEADS, H = c.n_kv * passes;
     uint64_t *bar = bars + warp * ST;
@@ -393,9 +394,12 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
                     : "memory");
             st_fill = st_fill + 1 == ST ? 0 : st_fill + 1;
         };
-        int filled = 0;
+        int filled;
+        auto fill_first = [&]() {
 #pragma unroll 1
-        for (; filled < mine && filled < ST; filled++) fill(filled);
+            for (filled = 0; filled < mine && filled < ST; filled++) fill(filled);
+        };
+        fill_first();
 
         // ---- Q operand: column gr is head gr of the pass; of block b the thread has dims 32 b + 8 t4 + 0..7, as
         // pairs (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16, matching the codes' order in a word
@@ -461,6 +465,8 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
             }
             q_sums = t4 < 2 ? sums[0] : sums[1];
         }
+        bool dead = false, held = false;  // held: the second time, for references past 2^24 (kv4_far)
+    tiles:
         float o[NB][2][4];  // [block][values 0, 1 or 2, 3 of 4 gr ..]: rows (value, head 2 t4 + {0, 1})
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -477,7 +483,6 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
             const float2 r = ka_float2(room[b / 2]);
             return b & 1 ? r.y : r.x;
         };
-        bool dead = false;
 
         for (int j = 0; j < filled; j++) {
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bar[st_read], phase))) {
@@ -731,6 +736,18 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
             }
         }
 
+        if (__builtin_expect(!held && !dead && __any_sync(0xffffffffu, kv4_far(ref[0]) || kv4_far(ref[1])), 0)) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int far = kv4_far(ref[i]);
+                to_log2[i] *= kv4_pow2(-far);
+                if (gr == 0) sh_up[warp][2 * t4 + i] = kv4_pow2(far);
+            }
+            held = true;
+            fill_first();
+            goto tiles;
+        }
+
         // ---- join the warps: [warp][head][ref, l, o...]
 #pragma unroll
         for (int i = 0; i < 2; i++)
@@ -741,7 +758,7 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             float *r = sums + (warp * KA_HEADS + 2 * t4 + i) * RW;
-            if (gr == 0) r[0] = ref[i], r[1] = l[i];
+            if (gr == 0) r[0] = held ? ref[i] * sh_up[warp][2 * t4 + i] : ref[i], r[1] = l[i];
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const float f = (PREC ? 0.015625f : 1.0f) * kv4_inv_pow2(room_of(b));

@@ -127,6 +127,15 @@ __device__ __forceinline__ float kv4_exp2(float x) {
     return y;
 }
 
+// An exponent is s c - ref in one multiply-add, ref the rounded s c of a row's largest score s.  From |ref| = 2^24 on, what that
+// rounding left would be an exponent of its own, past a float's in the end.  There c and ref are held below, times
+// 2^-kv4_far(ref): scores whose difference a float can tell at all still differ by more than a weight's bits, or by less than
+// the scores' own error.
+__device__ __forceinline__ int kv4_far(float ref) {
+    const int e = (int)((__float_as_uint(ref) >> 23) & 255u) - 127;
+    return e >= 24 && e < 128 ? e - 23 : 0;
+}
+
 // The attention calls' scratch: counters (zero between calls), then the parts of split work.
 inline size_t kv4_counter_bytes(int sm_count) { return ((size_t)sm_count * 8 + 15) / 16 * 16; }
 inline float *kv4_scratch_parts(void *scratch, int sm_count) {

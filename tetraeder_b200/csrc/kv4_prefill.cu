@@ -149,7 +149,8 @@ struct Kv4PrefillCfg {
     static constexpr int HALF = KP_N * 128;               // bytes of a half tile
     static constexpr int TILE = HALVES * HALF;
     static constexpr int CODES = KP_N * HD / 2, SCALES = KP_N * NB * 2, RAW = CODES + SCALES;
-    static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, R = V + 2 * TILE, CS = R + KP_RAW * RAW, BARS = CS + KP_ROWS * 4;
+    static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, R = V + 2 * TILE, CS = R + KP_RAW * RAW, UP = CS + KP_ROWS * 4,
+                         BARS = UP + KP_ROWS * 4;
     static constexpr int SMEM = BARS + 1024;
     static constexpr int64_t PART = KP_ROWS * (HD + 2);  // floats of a piece
 };
@@ -309,7 +310,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
         for (; it.in_run_warp(a, len); it.next(a)) {
             if (it.n == 0 || m >= it.mt()) continue;
             KP_WAIT_WARP(bars.q_full[m], items & 1);
-            const float cs = cs_smem[m * KP_M + r];
+            float cs = cs_smem[m * KP_M + r];
+            float &up = reinterpret_cast<float *>(smem + Cfg::UP)[m * KP_M + r];  // 2^kv4_far: cs and ref are the row's own over it
+            up = 1.0f;
             const int t = a.pos0 + a.token(min(it.row0 + m * KP_M + r, it.row0 + it.n_rows - 1));  // the row's position
             const int row_lo = it.row0 + m * KP_M, row_hi = min(row_lo + KP_M, it.row0 + it.n_rows) - 1;
             // the tile's first and last position, and the last positions before their windows
@@ -392,8 +395,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                                     mx = fmaxf(mx, see0 & (1u << i) ? __uint_as_float(s0[i]) : -INFINITY);
                                     mx = fmaxf(mx, see1 & (1u << i) ? __uint_as_float(s1[i]) : -INFINITY);
                                 }
-                                const float next = fmaxf(ref, mx * cs);
-                                const float f = ref == -INFINITY ? 0.0f : kv4_exp2(ref - next);
+                                cs *= up, ref *= up;
+                                float next = fmaxf(ref, mx * cs);
+                                const int far = kv4_far(next);
+                                const float down = kv4_pow2(-far);
+                                cs *= down, next *= down, up = kv4_pow2(far);
+                                const float f = ref == -INFINITY ? 0.0f : kv4_exp2(ref * down - next);
                                 ref = next;
                                 l *= f;
                                 if (hf) {  // the first half's product has to be in O
@@ -449,7 +456,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 float *piece = a.part + (2 * (int64_t)blockIdx.x + (it.tile0 > 0 ? 0 : 1)) * Cfg::PART;
                 part = piece + (m * KP_M + r) * 4;
                 float *stats = piece + KP_ROWS * HD + m * KP_M + r;
-                if (row <= row_hi) stats[0] = ref, stats[KP_ROWS] = l;
+                if (row <= row_hi) stats[0] = ref * up, stats[KP_ROWS] = l;
             }
             const int tok = a.token(row);
             const unsigned long long out =
