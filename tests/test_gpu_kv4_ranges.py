@@ -74,6 +74,14 @@ def test_scores_past_24_bits(dtype, hd, tokens, log2):
     run_far(dtype, hd, tokens, 2.0 ** log2)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("tokens", [1, 70, 200])
+def test_queries_near_the_largest_float(dtype, hd, tokens):
+    """Scores beyond 2^100 but within a float's range."""
+    run_far(dtype, hd, tokens, 2.0 ** 60, 2.0 ** 61)
+
+
 # ------------------------------------------------------------------ V blocks of very different scales
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("hd,nh,nkv", [(128, 8, 1), (64, 6, 2), (128, 20, 2)])

@@ -425,10 +425,8 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
             const int e = top > 0.0f && top <= FLT_MAX ? 13 - ilogbf(top) : 0;
             const int e1 = e / 2, e2 = e - e1;
             const float up1 = kv4_pow2(e1), up2 = kv4_pow2(e2);
-            // never 0: masked scores are -inf times it
             constexpr int HALF_UNIT = PREC ? 0 : 12;  // codes count 1 with f32, 2^-24 with bf16
-            const float c_gr =
-                fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(HALF_UNIT - e1) * kv4_pow2(HALF_UNIT - e2), FLT_MIN);
+            const float c_gr = kv4_factor(a.scale * 1.4426950408889634f * kv4_pow2(HALF_UNIT - e1) * kv4_pow2(HALF_UNIT - e2));
             to_log2[0] = __shfl_sync(0xffffffffu, c_gr, 8 * t4);
             to_log2[1] = __shfl_sync(0xffffffffu, c_gr, 8 * t4 + 4);
             uint32_t sums[2] = {0, 0};  // [low]: of this lane's two blocks

@@ -127,6 +127,10 @@ __device__ __forceinline__ float kv4_exp2(float x) {
     return y;
 }
 
+// A row's factor from S to log2 scores, within a float's range: not 0, as masked scores are -inf times it, and not infinite, as
+// a score of 0 is 0 times it.  Queries so small have equal scores either way, and ones so large the largest score alone.
+__device__ __forceinline__ float kv4_factor(float c) { return fminf(fmaxf(c, FLT_MIN), FLT_MAX); }
+
 // An exponent is s c - ref in one multiply-add, ref the rounded s c of a row's largest score s.  From |ref| = 2^24 on, what that
 // rounding left would be an exponent of its own, past a float's in the end.  There c and ref are held below, times
 // 2^-kv4_far(ref): scores whose difference a float can tell at all still differ by more than a weight's bits, or by less than

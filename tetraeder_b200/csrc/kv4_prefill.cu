@@ -641,8 +641,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                         tc::sts128(chunk(ch), make_uint4(kv4_half2(x[0], x[4]), kv4_half2(x[1], x[5]), kv4_half2(x[2], x[6]),
                                                          kv4_half2(x[3], x[7])));
                     }
-                    // log2 score of an accumulator's 1; never 0: masked scores are -inf times it
-                    cs_smem[m * KP_M + r] = fmaxf(a.scale * 1.4426950408889634f * kv4_pow2(-e), FLT_MIN);
+                    // log2 score of an accumulator's 1
+                    cs_smem[m * KP_M + r] = kv4_factor(a.scale * 1.4426950408889634f * kv4_pow2(-e));
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.q_full[m]);
