@@ -100,3 +100,67 @@ def test_a_huge_value_block_leaves_the_others_alone(dtype, hd, nh, nkv, at, bloc
     K, V = rowvals(k), rowvals(v)
     want, smax, sabs, _ = R.attend(q[0].double().numpy(), K, V, n - 1, 0, 0, hd ** -0.5)
     close(got[0], want, decode_block_tol(dtype, want, smax, sabs, block_max(V, slice(None), nh // nkv)))
+
+
+# ------------------------------------------------------------------ values beyond f16's range
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd,nh,nkv,S,pos0,window,n_sink", [(128, 8, 1, 70, 300, 0, 0), (64, 8, 2, 150, 129, 0, 0), (128, 16, 2, 300, 500, 200, 3)])
+@pytest.mark.parametrize("what", ["k", "v", "kv"])
+def test_prefill_of_values_beyond_f16(dtype, hd, nh, nkv, S, pos0, window, n_sink, what):
+    """Rows of up to 5e5 among ordinary ones, in one block (V) or in all (K, whose queries are then small): what the scale can hold,
+    8 times f16's range, in some tiles and not in others."""
+    rng = np.random.default_rng(hd + S + pos0)
+    n = pos0 + S
+    cache = tb.Kv4Cache(2, nkv, hd, n)
+    q = randn(rng, (S, nh, hd), DT[dtype], 1e-5 if "k" in what else 1.0)
+    k, v = randn(rng, (n, nkv, hd), DT[dtype]), randn(rng, (n, nkv, hd), DT[dtype])
+    some = np.r_[0:n:97, pos0 + S // 2]
+    if "k" in what:
+        k[some] *= 1e5
+    if "v" in what:
+        v[some, :, 32:64] *= 1.3e5
+    cache.store(k[:pos0].cuda(), v[:pos0].cuda(), 0, seq=1)
+    got = cache.prefill(q.cuda(), k[pos0:].cuda(), v[pos0:].cuda(), seq=1, pos0=pos0, window=window, n_sink=n_sink)
+    cache.check()
+    K, V = rowvals(k), rowvals(v)
+    assert max(np.abs(K).max(), np.abs(V).max()) > 2e5
+    for i in sorted({0, 1, S // 2, S - 1} | set(range(0, S, 17))):
+        want, smax, sabs, _ = R.attend(q[i].double().numpy(), K, V, pos0 + i, window, n_sink, hd ** -0.5)
+        tol = prefill_block_tol(dtype, want, smax, sabs, block_max(V, seen(n, pos0 + i, window, n_sink), nh // nkv))
+        close(got[i], want, tol, f"token {i}")
+
+
+@pytest.mark.parametrize("hd,nh,nkv,S,pos0", [(128, 8, 1, 33, 12000), (64, 16, 2, 300, 9000), (128, 32, 8, 1240, 0)])
+def test_prefill_of_a_few_values_beyond_f16(hd, nh, nkv, S, pos0):
+    """One row of K and one of V, which few of the CTAs that share the work meet; the parts of a cut block are joined."""
+    rng = np.random.default_rng(hd + S)
+    n = pos0 + S
+    cache = tb.Kv4Cache(1, nkv, hd, n)
+    q = randn(rng, (S, nh, hd), torch.bfloat16)
+    k, v = randn(rng, (n, nkv, hd), torch.bfloat16), randn(rng, (n, nkv, hd), torch.bfloat16)
+    v[n // 3, :, :32] *= 1.3e5
+    k[n // 2, :, 5] = 3e5
+    q[:, :, 5] = 1e-5
+    cache.store(k.cuda(), v.cuda(), 0, seq=0)
+    got = cache.prefill(q.cuda(), None, None, pos0=pos0)
+    assert torch.equal(cache.prefill(q.cuda(), None, None, pos0=pos0), got)
+    cache.check()
+    K, V = rowvals(k), rowvals(v)
+    for i in sorted({0, 1, S // 2, S - 1, min(S - 1, n // 3), min(S - 1, n // 2)}):
+        want, smax, sabs, _ = R.attend(q[i].double().numpy(), K, V, pos0 + i, 0, 0, hd ** -0.5)
+        close(got[i], want, prefill_block_tol("bf16", want, smax, sabs, block_max(V, slice(0, pos0 + i + 1), nh // nkv)), f"token {i}")
+
+
+@pytest.mark.parametrize("junk", [float("inf"), float("nan"), 65504.0])
+def test_prefill_is_the_same_whatever_unseen_rows_hold(junk):
+    rng = np.random.default_rng(4)
+    S, nh, nkv, hd, pos0, window = 150, 8, 1, 128, 700, 100
+    cache = tb.Kv4Cache(1, nkv, hd, pos0 + S + 50)
+    fill(cache, rng)
+    q = randn(rng, (S, nh, hd), torch.bfloat16).cuda()
+    want = cache.prefill(q, None, None, pos0=pos0, window=window, n_sink=2).clone()
+    for scales in (cache.k_scales, cache.v_scales):
+        scales[0, :, 2:pos0 + 1 - window] = junk
+        scales[0, :, pos0 + S:] = junk
+    assert torch.equal(cache.prefill(q, None, None, pos0=pos0, window=window, n_sink=2), want)
+    cache.check()

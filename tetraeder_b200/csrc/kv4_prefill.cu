@@ -22,7 +22,9 @@
 //   - The running reference of a row moves only when P against it adds up to more than 2^14 in half a tile (P is 2^6
 //     at the reference, so that no P leaves f16 before that): no maximum is taken, and O needs no rescaling.
 //     A tile is first tried with the old reference, S still whole in TMEM; the rare failure is redone.
-//   - Q is scaled per row by a power of two into f16's range.  Scales are held to what f16 can carry times 8.
+//   - Q is scaled per row by a power of two into f16's range.
+//   - A scale of 2^13 and more takes its values (up to 8 times f16's largest) out of f16.  The first pass over a CTA's run only notes
+//     that it met one; the CTA then does its run again with K and V over 8.  Without one this costs a test of bits per scale.
 //   - What a warp has alike (its role, its block, the conditions of a tile) goes through a shuffle from lane 0, and
 //     shared memory is declared aligned: branches, addresses and descriptors then stay out of the lanes' registers (a tile
 //     pair 2.41 us, without either 2.79).
@@ -51,7 +53,7 @@ constexpr int KP_UNITS = 8, KP_UNITS1 = 6, KP_UNITS_BLOCK = 12, KP_UNITS_JOIN = 
 constexpr int KP_MAX_CTAS = 512;
 constexpr float KP_BIAS = 6.0f;      // P is 2^KP_BIAS at the reference
 constexpr float KP_MOST = 16384.0f;  // a half tile's sum of P above which the row's reference moves
-constexpr float KP_SCALE_MAX = 8188.0f;  // 8 * this is f16's largest
+constexpr float KP_BIG = 8.0f, KP_BIG_LOG2 = 3.0f;  // K and V are held over this where they leave f16 (see KpBars::big)
 
 // Which positions the tokens t0 .. t1 see between them, as tiles of KP_N (see Kv4Seen).
 __host__ __device__ __forceinline__ Kv4Seen kp_seen(int pos0, int t0, int t1, int window, int n_sink) {
@@ -161,6 +163,9 @@ struct KpBars {
     // a slot holds K and V by turns; each of the two has its own barrier of it, so that its readers see every phase
     uint64_t raw_full[2][KP_RAW];
     uint32_t tmem;
+    // A scale of 2^13 and more, 8 of which leave f16, was met: the CTA does its run a second time, K and V over KP_BIG
+    int big;
+    int failed;  // a wait ran out
     int g, blk, s, len;  // the run: its first block, that one's first unit from the run's first, its units
     KpCut cut;
     KpItem item[8];  // the softmax warps'
@@ -198,11 +203,20 @@ struct KpNo {
     static constexpr bool value = false;
 };
 
+// The roles meet at the end of the first pass over the run (barrier 1)
+__device__ __forceinline__ void kp_meet(bool wait) {
+    if (wait)
+        asm volatile("barrier.cta.sync 1, %0;" ::"n"(KP_THREADS) : "memory");
+    else
+        asm volatile("barrier.cta.arrive 1, %0;" ::"n"(KP_THREADS) : "memory");
+}
 // Bounded waits by a whole warp.  One that runs out latches the error and ends the role.
 #define KP_WAIT_WARP(bar, phase)                                                            \
     do {                                                                                    \
         if (!__all_sync(0xffffffffu, mbar_wait_bounded(&(bar), (uint32_t)(phase)))) {       \
-            if (lane == 0) latch_error(a.err, TMOE_DEV_ERR_TIMEOUT);                        \
+            if (lane == 0) latch_error(a.err, TMOE_DEV_ERR_TIMEOUT), bars.failed = 1;       \
+            __syncwarp();                                                                   \
+            if (!second) kp_meet(false);                                                    \
             goto done;                                                                      \
         }                                                                                   \
     } while (0)
@@ -219,6 +233,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
     const int warp = kp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
+        bars.big = bars.failed = 0;
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.q_full[i], 4);
             mbar_init(&bars.q_empty[i], 1 + 4);
@@ -287,6 +302,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
     KpItem it;
     it.g = bars.g, it.blk = bars.blk, it.s = bars.s;
     const int len = bars.len;
+    // Every role runs through the items, and through them again if the first pass met a big scale: barriers and counters go on
+    // as if these were further items, and all that was written is written anew
+    bool second = false;
+    auto again = [&]() {
+        if (second) return false;
+        kp_meet(true);
+        second = bars.big && !bars.failed;
+        it.g = bars.g, it.blk = bars.blk, it.s = bars.s;
+        return second;
+    };
     float *cs_smem = reinterpret_cast<float *>(smem + Cfg::CS);  // [KP_ROWS]
     pdl_wait();
     pdl_trigger();
@@ -307,6 +332,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + m * KP_N + lanes, to = tmem + 256 + m * HD + lanes;
         int nt = 0, items = 0;  // tiles and blocks before
+        do {  // the passes
         for (; it.in_run_warp(a, len); it.next(a)) {
             if (it.n == 0 || m >= it.mt()) continue;
             KP_WAIT_WARP(bars.q_full[m], items & 1);
@@ -449,14 +475,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
             }
             // ---- the rows' results
             it = bars.item[warp];
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float inv = l == 0.0f ? 0.0f : (second ? KP_BIG : 1.0f) / l;
             const int row = row_lo + r;
             float *part = nullptr;
             if (!it.uncut()) {  // O as it is, rows side by side
                 float *piece = a.part + (2 * (int64_t)blockIdx.x + (it.tile0 > 0 ? 0 : 1)) * Cfg::PART;
                 part = piece + (m * KP_M + r) * 4;
                 float *stats = piece + KP_ROWS * HD + m * KP_M + r;
-                if (row <= row_hi) stats[0] = ref * up, stats[KP_ROWS] = l;
+                // times KP_BIG, by its weight
+                if (row <= row_hi) stats[0] = ref * up + (second ? KP_BIG_LOG2 : 0.0f), stats[KP_ROWS] = second ? l / KP_BIG : l;
             }
             const int tok = a.token(row);
             const unsigned long long out =
@@ -524,15 +551,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
             }
             tc::fence_before();
         }
+        } while (again());
     } else if (warp < 16) {
         tc::fewer_registers<KP_REGS_DEQUANT>();
         // ------------------------------------------------------------ dequantise: a thread per position
         const int r = threadIdx.x & 127;
         const bool is_v = warp >= 12;
         const uint32_t smem0 = smem_u32(smem);
-        const __half2 cap = __float2half2_rn(KP_SCALE_MAX), ncap = __float2half2_rn(-KP_SCALE_MAX);
         const int m = is_v;  // the Q tile that this group loads: before its first tile of all, later after a block's first tile
         int nt = 0, items = 0;
+        do {
         for (; it.in_run_warp(a, len); it.next(a)) {
             if (it.n == 0) continue;
             const int q_at = nt ? 1 : 0;
@@ -568,15 +596,25 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                     if (nt >= 2) KP_WAIT_WARP(is_v ? bars.v_empty[slot] : bars.k_empty[slot], ((nt >> 1) - 1) & 1);
                     const int pos = it.seen.tile(it.tile0 + j) * KP_N + r;
                     const bool seen = it.seen.sees(pos, a.n_sink);  // a row that no query sees may hold anything
-                    uint32_t sc[NB / 2];
+                    uint32_t sc[NB / 2], top = 0;
 #pragma unroll
                     for (int b = 0; b < NB / 2; b++) {
                         sc[b] = tc::lds32(raw + Cfg::CODES + (r * NB + 2 * b) * 2);
-                        __half2 h;
-                        memcpy(&h, &sc[b], 4);
-                        h = __hmax2(__hmin2(h, cap), ncap);  // also keeps a NaN out
-                        memcpy(&sc[b], &h, 4);
                         if (!seen) sc[b] = 0;
+                        top |= (sc[b] & 0x70007000u) + 0x10001000u;
+                    }
+                    if (second) {
+#pragma unroll
+                        for (int b = 0; b < NB / 2; b++) {
+                            const __half2 most = __float2half2_rn(65504.0f);
+                            __half2 h;
+                            memcpy(&h, &sc[b], 4);
+                            h = __hmax2(__hmin2(h, most), __hneg2(most));  // also keeps a NaN out
+                            h = __hmul2(h, __float2half2_rn(1.0f / KP_BIG));
+                            memcpy(&sc[b], &h, 4);
+                        }
+                    } else if (top & 0x80008000u) {  // 2^13 (bits 0x7000) and more
+                        bars.big = 1;
                     }
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
@@ -642,7 +680,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                                                          kv4_half2(x[3], x[7])));
                     }
                     // log2 score of an accumulator's 1
-                    cs_smem[m * KP_M + r] = kv4_factor(a.scale * 1.4426950408889634f * kv4_pow2(-e));
+                    cs_smem[m * KP_M + r] = kv4_factor(a.scale * 1.4426950408889634f * kv4_pow2(-e) * (second ? KP_BIG : 1.0f));
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.q_full[m]);
@@ -650,6 +688,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 }
             }
         }
+        } while (again());
     } else {
         tc::fewer_registers<KP_REGS_ISSUE>();
         if (warp == 16) {
@@ -696,9 +735,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 }
                 return false;
             };
+            int nt = -1, pt[2] = {0, 0}, qt[2] = {0, 0};  // tiles; tiles and blocks of A and of B
+            do {
             bool more = skip_empty();
             int j = -1, n = more ? it.n : 0, mt = 0;  // the tile of the products; -1: none yet
-            int nt = -1, pt[2] = {0, 0}, qt[2] = {0, 0};  // tiles; tiles and blocks of A and of B
             while (more) {
                 // the tile after (j, n, mt)
                 int nj = j + 1, nn = n, nmt = mt;
@@ -732,10 +772,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                 nt++;
                 j = nj, n = nn, mt = nmt;
             }
+            if (nt >= 0) nt--;  // the last tile again
+            } while (again());
         } else if (warp == 17) {
         // ------------------------------------------------------------ raw tiles by bulk copies
+        int i = 0;  // raw tiles before
+        do {
         if (lane == 0) {
-            int i = 0;  // raw tiles before
             bool ok = true;
             for (; ok && it.in_run(a, len); it.next(a)) {
                 const int64_t head = ((int64_t)a.seq * c.n_kv + it.g) * c.n_ctx;
@@ -744,7 +787,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
                     const int rs = i % KP_RAW;
                     if (i >= KP_RAW && !mbar_wait_bounded(&bars.raw_empty[rs], ((i / KP_RAW) - 1) & 1)) {
                         latch_error(a.err, TMOE_DEV_ERR_TIMEOUT);
-                        ok = false;
+                        ok = false, bars.failed = 1;
                         break;
                     }
                     const int p0 = it.seen.tile(it.tile0 + (j >> 1)) * KP_N;
@@ -760,6 +803,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prefill_kernel(const Kv4Pre
             for (int k = max(i - KP_RAW, 0); k < i; k++)
                 mbar_wait_bounded(&bars.raw_full[k & 1][k % KP_RAW], ((k >> 1) / KP_RAW) & 1);
         }
+        __syncwarp();
+        } while (again());
+        } else {
+            kp_meet(false);
         }
     }
 done:
