@@ -114,3 +114,17 @@ def test_calls_after_the_layer_was_closed_are_refused():
                  lambda: cache.load(pos), cache.check):
         with pytest.raises(tb.TmoeError, match="TMOE_E_INVALID"):
             call()
+
+
+def test_an_error_on_a_side_stream_is_found_there():
+    cache = tb.Kv4Cache(1, 1, 64, 64)
+    x = torch.ones((1, 1, 64), device="cuda")
+    bad = torch.tensor([64], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+    cache.store(x, x, bad, seq=0, stream=side)
+    with pytest.raises(tb.TmoeError, match="outside the 4-bit cache"):
+        cache.check(stream=side)
+    cache.check()

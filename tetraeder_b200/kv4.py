@@ -269,6 +269,6 @@ class Kv4Cache:
             _lib.check(rc, self.h)
         return out
 
-    def check(self):
-        """Synchronises the current stream and raises if a kernel latched an error."""
-        _lib.check(self.lib.tmoe_check(self.h, self._stream(None)), self.h)
+    def check(self, stream=None):
+        """Synchronises the stream (the current one) and raises if a kernel latched an error."""
+        _lib.check(self.lib.tmoe_check(self.h, self._stream(stream)), self.h)
