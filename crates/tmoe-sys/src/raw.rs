@@ -88,6 +88,7 @@ pub struct tmoe_kv4_attn {
     pub window: i32,
     pub n_sink: i32,
     pub scale: f32,
+    pub f16_products: i32,
 }
 
 /// Stacked or slot expert tensors: device pointers into caller-owned ggml buffers.

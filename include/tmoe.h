@@ -391,9 +391,11 @@ TMOE_API int tmoe_argmax(tmoe_handle *h, void *stream, const float *x, int64_t r
  * A query at position t sees position p if p <= t and (window is 0, or t - p < window, or p < n_sink):
  * full causal attention, or a sliding window with the first n_sink positions always in sight.
  * Out = softmax(scale * q . K) V per head; query head h reads KV head h / (n_head / n_kv).  Statistics and
- * sums are f32.  Decoding with f32 activations computes to f32 precision; with bf16, P is rounded to 16
- * bits once.  The prefill takes Q, K, P and V to the tensor cores as F16 with either type, as
- * tmoe_attn_prefill does.
+ * sums are f32.  With f32 activations both calls compute to f32 precision, for any number of tokens, unless
+ * f16_products lets the prefill take Q, K, P and V to the tensor cores as F16, as tmoe_attn_prefill does
+ * (an error of 4e-4 of the largest output against 3e-7, in an eighth of the time).  With bf16 the decode
+ * rounds P, and its product with V's scale, to F16 (2^-11 each), and the prefill K, P and V: below the
+ * output's own rounding.
  * scratch: tmoe_kv4_attn_scratch_bytes bytes, 16-byte aligned, zeroed once before its first use; every
  * call leaves it ready for the next.  Calls that may run at the same time need a scratch each.
  * A sequence or position outside the cache is skipped (its output zero) and latches the device error
@@ -422,6 +424,7 @@ typedef struct {
     int32_t window;  /* 0: none */
     int32_t n_sink;
     float scale;
+    int32_t f16_products; /* prefill of f32 rows: 1 allows F16 operands (bf16 rows: no difference) */
 } tmoe_kv4_attn;
 TMOE_API int tmoe_kv4_store(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cache, int32_t type, const void *k,
                             const void *v, int64_t ld, const int32_t *seq, int32_t seq0, const int32_t *pos,

@@ -216,3 +216,11 @@ def test_numbers_past_32_bits_are_refused(x):
         with pytest.raises(ValueError):
             call()
     assert not cache.lib.calls
+
+
+def test_f16_products_are_asked_for():
+    cache, q = make(), rows(2, 4, torch.float32)
+    cache.prefill(q, None, None, out=q)
+    cache.prefill(q, None, None, out=q, f16_products=True)
+    cache.prefill(q, None, None, out=q)
+    assert [c[1].f16_products for c in cache.lib.calls] == [0, 1, 0]

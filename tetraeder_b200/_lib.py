@@ -50,7 +50,7 @@ class Kv4AttnStruct(C.Structure):
     _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
                 ("scratch", C.c_void_p), ("q_ld", C.c_int64), ("kv_ld", C.c_int64), ("out_ld", C.c_int64),
                 ("type", C.c_int32), ("n_head", C.c_int32), ("window", C.c_int32), ("n_sink", C.c_int32),
-                ("scale", C.c_float)]
+                ("scale", C.c_float), ("f16_products", C.c_int32)]
 
 
 P = C.c_void_p

@@ -3,6 +3,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
@@ -1476,6 +1477,8 @@ int check_kv4_attn(tmoe_handle *h, const tmoe_kv4_cache *c, const tmoe_kv4_attn 
     if (a->n_head <= 0 || a->n_head % c->n_kv || a->n_head > 65535)
         return fail(h, TMOE_E_INVALID, "%d heads over %d KV heads", a->n_head, c->n_kv);
     if (a->window < 0 || a->n_sink < 0) return fail(h, TMOE_E_INVALID, "window %d, %d sinks", a->window, a->n_sink);
+    if (a->f16_products != 0 && a->f16_products != 1)
+        return fail(h, TMOE_E_INVALID, "f16_products is %d, not 0 or 1", a->f16_products);
     if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return fail(h, TMOE_E_INVALID, "scale %g", (double)a->scale);
     return TMOE_OK;
 }
@@ -1546,7 +1549,7 @@ int tmoe_kv4_attn_decode(tmoe_handle *h, void *stream, const tmoe_kv4_cache *cac
 // over 4, bf16): 4 tokens at 300 / 20000 / 60000 9 / 18 / 34 us against 11 / 23 / 40; 16 at 300 / 2000 / 8000 8 / 12 / 25 against
 // 11 / 19 / 19.  40 heads over 8: 16 at 2000 18 against 19, 24 at 300 14 against 12.  f32, 3 / 4 at 60000: 37 / 47 against 40 / 41.
 static bool kv4_few(const tmoe::Kv4Attn &x, int n_kv, bool f32) {
-    const int64_t passes = (x.n_head / n_kv + 7) / 8, segments = x.n_tok * n_kv * passes;
+    const int64_t passes = (x.n_head / n_kv + 7) / 8, segments = (int64_t)x.n_tok * n_kv * passes;
     int64_t seen = (int64_t)x.pos0 + x.n_tok;
     if (x.window > 0 && seen > (int64_t)x.window + x.n_sink) seen = (int64_t)x.window + x.n_sink;
     return x.n_tok * passes <= (f32 ? 3 : 4) || x.n_tok == 1 || (segments <= 128 && segments * seen <= 1 << 18);
@@ -1575,9 +1578,19 @@ int tmoe_kv4_attn_prefill(tmoe_handle *h, void *stream, const tmoe_kv4_cache *ca
         if (e != cudaSuccess) return cuda_fail(h, e, "kv4 store");
         x.k = x.v = nullptr;
     }
-    if (kv4_few(x, cache->n_kv, f32)) {
-        e = tmoe::launch_kv4_attn(f32, cache->head_dim, x, planes, attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
-        return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "kv4 decode attention");
+    // f32 precision is the decode kernel's: a segment per token and KV head, in calls of up to 2^29 tiles of 64 positions.
+    // 32 heads over 4 of 128: 33 tokens at 20000 / 2048 / 8192 take 114 / 511 / 5620 us, with f16_products 43 / 68 / 690
+    if ((f32 && !attn->f16_products) || kv4_few(x, cache->n_kv, f32)) {
+        const int64_t segments = (int64_t)cache->n_kv * ((x.n_head / cache->n_kv + 7) / 8), tiles = (pos0 + (int64_t)S) / 64 + 64;
+        const int64_t most = std::max<int64_t>(1, (1ll << 29) / (segments * tiles));
+        for (int64_t t = 0; t < S; t += most) {
+            tmoe::Kv4Attn y = x;
+            y.n_tok = (int)std::min<int64_t>(most, S - t), y.pos0 = pos0 + (int)t;
+            y.q = (const char *)x.q + t * x.q_ld * (f32 ? 4 : 2), y.out = (char *)x.out + t * x.out_ld * (f32 ? 4 : 2);
+            e = tmoe::launch_kv4_attn(f32, cache->head_dim, y, planes, attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
+            if (e != cudaSuccess) return cuda_fail(h, e, "kv4 decode attention");
+        }
+        return TMOE_OK;
     }
     e = tmoe::launch_kv4_prefill(f32, cache->head_dim, x, planes, attn->scratch, h->sm_count, h->err, (cudaStream_t)stream);
     return e == cudaSuccess ? TMOE_OK : cuda_fail(h, e, "kv4 prefill attention");

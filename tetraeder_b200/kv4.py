@@ -258,12 +258,14 @@ class Kv4Cache:
         return out
 
     def prefill(self, q, k, v, seq: int = 0, pos0: int = 0, window: int = 0, n_sink: int = 0,
-                scale: float | None = None, out=None, stream=None):
+                scale: float | None = None, out=None, stream=None, f16_products: bool = False):
         """S new tokens of sequence `seq` at positions pos0 .. pos0 + S - 1: rows k, v [S, n_kv, head_dim] are stored
         (None: stored already), then query i of q [S, n_head, head_dim] attends to positions 0 .. pos0 + i (or
-        its window and sinks).  Returns out [S, n_head, head_dim]."""
+        its window and sinks).  float32 queries are computed to their own precision, or, with f16_products, with
+        Q, K, P and V as 16-bit operands of the tensor cores, up to eight times faster.  Returns out [S, n_head, head_dim]."""
         _int32(seq=seq, pos0=pos0)
         out = self._attn(q, k, v, window, n_sink, scale, out, stream)
+        self._a.f16_products = bool(f16_products)
         rc = self.lib.tmoe_kv4_attn_prefill(self.h, self._stream(stream), self._cp, self._ap, seq, pos0, q.shape[0])
         if rc:
             _lib.check(rc, self.h)

@@ -295,7 +295,8 @@ class Qwen3MoeModel:
                                     hp.rope_freq_base, hp.rms_eps))
             if self.kv4:
                 self.kv4[il].prefill(b["q"].view(S, nh, d), b["k"].view(S, nkv, d), b["v"].view(S, nkv, d), seq=seq, pos0=pos0,
-                                     window=self.window, n_sink=self.n_sink, out=b["att"].view(S, nh, d), stream=stream)
+                                     window=self.window, n_sink=self.n_sink, out=b["att"].view(S, nh, d), stream=stream,
+                                     f16_products=True)  # as over F16 caches
             else:
                 chk(L.tmoe_attn_prefill(h, st, _ptr(b["q"]), _ptr(b["k"]), _ptr(b["v"]), _ptr(self.kc[il]),
                                         _ptr(self.vc[il]), seq, self.max_batch, pos0, S, nh, nkv, d, self.n_ctx,
