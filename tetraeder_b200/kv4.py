@@ -40,11 +40,13 @@ def _settle(device):
             torch.cuda.current_stream().synchronize()
 
 
-def _int32(**values):
-    """Numbers that the C calls take in 32 bits: ctypes would pass on the low ones of any other."""
-    for name, x in values.items():
-        if not -1 << 31 <= x < 1 << 31:
-            raise ValueError(f"{name} is {x}")
+_INT_MIN, _INT_MAX = -1 << 31, (1 << 31) - 1
+
+
+def _int32(names, x, y):
+    """Two numbers that the C calls take in 32 bits: ctypes would pass on the low ones of any other."""
+    if not (_INT_MIN <= x <= _INT_MAX and _INT_MIN <= y <= _INT_MAX):
+        raise ValueError(f"{names} are {x}, {y}")
 
 
 class Kv4Cache:
@@ -147,7 +149,7 @@ class Kv4Cache:
         """(seq, seq0, pos, pos0) of the C calls."""
         p, pos0 = (self._index("pos", pos, n), 0) if torch.is_tensor(pos) else (None, int(pos))
         if p is None:
-            _int32(pos=pos0)
+            _int32("pos and n", pos0, n)
         if torch.is_tensor(seq):
             return self._index("seq", seq, n), 0, p, pos0
         if seq is None and p is None:
@@ -211,7 +213,8 @@ class Kv4Cache:
         if sig != self._row_sig:  # a shape to allocate by: no memory of its own
             self._row_like = torch.empty(1, dtype=dtype, device=self.device).expand(n, self.n_kv, self.head_dim)
             self._row_sig = sig
-        k, v = self._new(self._row_like, stream), self._new(self._row_like, stream)
+        like = self._row_like
+        k, v = (torch.empty_like(like), torch.empty_like(like)) if stream is None else (self._new(like, stream), self._new(like, stream))
         rc = self.lib.tmoe_kv4_load(self.h, self._stream(stream), self._cp, ty, k.data_ptr(), v.data_ptr(),
                                     self.n_kv * self.head_dim, s, s0, p, p0, n)
         if rc:
@@ -227,7 +230,7 @@ class Kv4Cache:
             a.type, a.q_ld, a.n_head = ty, ld, q.shape[1]
             self._q_sig = sig
         if out is None:
-            out = self._new(q, stream)
+            out = torch.empty_like(q) if stream is None and q.is_contiguous() else self._new(q, stream)
             a.out_ld = q.shape[1] * self.head_dim
         else:
             a.out_ld = self._heads("out", out, n, dt, q.shape[1])
@@ -240,7 +243,7 @@ class Kv4Cache:
             raise ValueError("k and v come together")
         a.q, a.out = q.data_ptr(), out.data_ptr()
         if window or n_sink:
-            _int32(window=window, n_sink=n_sink)
+            _int32("window and n_sink", window, n_sink)
         a.window, a.n_sink = window, n_sink
         a.scale = self._scale if scale is None else scale
         return out
@@ -263,9 +266,9 @@ class Kv4Cache:
         (None: stored already), then query i of q [S, n_head, head_dim] attends to positions 0 .. pos0 + i (or
         its window and sinks).  float32 queries are computed to their own precision, or, with f16_products, with
         Q, K, P and V as 16-bit operands of the tensor cores, up to eight times faster.  Returns out [S, n_head, head_dim]."""
-        _int32(seq=seq, pos0=pos0)
+        _int32("seq and pos0", seq, pos0)
         out = self._attn(q, k, v, window, n_sink, scale, out, stream)
-        self._a.f16_products = bool(f16_products)
+        self._a.f16_products = f16_products
         rc = self.lib.tmoe_kv4_attn_prefill(self.h, self._stream(stream), self._cp, self._ap, seq, pos0, q.shape[0])
         if rc:
             _lib.check(rc, self.h)
