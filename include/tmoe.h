@@ -381,7 +381,7 @@ TMOE_API int tmoe_argmax(tmoe_handle *h, void *stream, const float *x, int64_t r
  *                         elements apart, into the cache: row i at position pos[i] (pos NULL: pos0 + i)
  *                         of sequence seq[i] (seq NULL: seq0, or sequence i where seq0 is negative).
  *                         A negative position: no row.  The places of a call's rows are distinct
- *   tmoe_kv4_load         the same rows back as values (zeros where there is no row)
+ *   tmoe_kv4_load         the same rows back as values (zeros where there is no row), rounded to `type`
  *   tmoe_kv4_attn_decode  one new token for each of B sequences: its row k, v is stored at pos[b] of
  *                         sequence b (k and v NULL: it is there already) and its query attends to the
  *                         positions that it sees, the new one included, as the cache holds them.

@@ -33,10 +33,11 @@ __device__ __forceinline__ bool kv4_place(const Kv4RowArgs &a, int64_t i, int &s
     return true;
 }
 
-// Rows are independent and only moved once: HBM-bound, if the codes cost few instructions.  A thread takes 16
-// values (a block is two threads, its extremes one shuffle each), so that a warp reads whole 128-byte
-// lines; rows run fastest over the threads, so that a run of positions writes one contiguous piece of a
-// head's plane.  8191 bf16 rows of 8 heads of 128, K and V: 12.6 us (floor 9.2); with 8 values a thread and converted codes 20.6.
+// Rows are independent and only moved once, so that what bounds it is the codes' instructions: 79% of the issue slots in a
+// capture, 13% of DRAM.  A thread takes 16 values (a block is two threads, its extremes one shuffle each), so that a warp reads
+// whole 128-byte lines; rows run fastest over the threads, so that a run of positions writes one contiguous piece of a
+// head's plane.  8191 bf16 rows of 8 heads of 128, K and V: 12.5 us (43 MB, floor 6.6), f32 rows 13.0 (77 MB, 11.7); with 8
+// values a thread and converted codes 20.6.
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowArgs a) {
     const Kv4Planes &c = a.c;
@@ -78,8 +79,8 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowArgs a) {
     if ((sub & 1) == 0) (is_v ? c.vs : c.ks)[row * NB + b] = d;
 }
 
-// A thread writes 8 values (16 bytes of bf16), so that a warp's stores are whole lines.  The same rows: 14.4 us (floor 9.2); two rows
-// a thread 16.5, four 19.7.
+// A thread writes 8 values (16 bytes of bf16), so that a warp's stores are whole lines.  HBM-bound.  The same rows as f32: 14.4 us
+// (77 MB, floor 11.7); two rows a thread 16.5, four 19.7.
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
     const Kv4Planes &c = a.c;
@@ -138,9 +139,9 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowArgs a) {
 // run, fetched by bulk copies into its own ring.  Runs that hold less than a segment leave partial sums in
 // scratch; the CTA that arrives last there joins them, in run order (the same sums every call).
 //
-// Measured (32 heads, width 128, bf16): 64 sequences of up to 32768 positions, 4 KV heads, 150 us, 5.1 TB/s; one of 131071, 8 KV
-// heads, 40 us, 3.8 TB/s.  What is left there: the SMs get unequal shares of the bandwidth (their even runs end 138 .. 150 us), and a part's start
-// and join are about 5 us.
+// Measured (32 heads, width 128, bf16; graph replay): 64 sequences of up to 32768 positions, 4 KV heads, 150 to 160 us by device,
+// 4.8 to 5.1 TB/s; one of 131071, 8 KV heads, 40 us, 3.8 TB/s.  What is left there: the SMs get unequal shares of the bandwidth
+// (their even runs end 138 .. 150 us), and a part's start and join are about 5 us.
 constexpr int KA_HEADS = 8;
 constexpr float KA_ROOM = 8.0f;  // how far (log2) a score may exceed its head's reference
 constexpr float KA_BIAS = 6.0f;  // P times the V scale is held below 2^(KA_BIAS + KA_ROOM)
@@ -167,6 +168,7 @@ struct Kv4AttnCfg {
     //   width 128, bf16, 64 x 32768 / 1 x 131071: 12 x 2, one CTA 149 / 39.8 us; 8 x 3, one 160 / 41.6; 6 x 2, two 157 / 42.4
     //   width 128, f32, 4 x 4096: 8 x 3, one CTA 11.1 us; 12 x 2, one 13.3; 6 x 2, two 15.3
     //   width 64, 16 heads over 16, 24 x 5003: 6 x 4, two CTAs 32.3 us; 12 x 4, one 37.2; 8 x 6, one 38.5
+    // (sequences here and below: of up to that many positions, the mean 0.62 of it)
     // SHORT: more segments than SMs, of 128 tiles at most each.  A CTA's start and join then come often, and run beside a second
     // CTA's tiles: width 128, bf16, 6 x 2, two CTAs against 12 x 2, one, in 64 sequences of 1024 / 4096 / 8192 / 16384 positions
     // 19.3 / 38.5 / 61.9 / 98.7 us against 21.4 / 41.8 / 61.9 / 96.1; f32, 4 x 3, two against 8 x 3, one, 21.3 / 50.1 / 83.9 / 137.0
@@ -909,7 +911,9 @@ static cudaError_t attn_launch(const Kv4Attn &x, const Kv4Planes &c, int64_t seg
 cudaError_t launch_kv4_attn(bool f32, int head_dim, Kv4Attn &x, const Kv4Planes &c, void *scratch, int sm_count,
                             int *err, cudaStream_t st) {
     if (x.n_tok <= 0) return cudaSuccess;
-    // the most tiles that a token can see, as far as the host knows
+    // The most tiles that a token can see, as far as the host knows: decode positions are on the device, so that without a window
+    // it is the cache's capacity.  Sequences well below it then take the other form: 128 of 2048 positions 48 us in a cache of
+    // 2048, 58 in one of 32768; 64 of 4096 44 and 48.
     constexpr int TILE = 64;
     const int G = x.n_head / c.n_kv, passes = (G + KA_HEADS - 1) / KA_HEADS;
     int64_t most = x.pos ? c.n_ctx : x.pos0 + x.n_tok;

@@ -28,8 +28,11 @@
 //   - What a warp has alike (its role, its block, the conditions of a tile) goes through a shuffle from lane 0, and
 //     shared memory is declared aligned: branches, addresses and descriptors then stay out of the lanes' registers (a tile
 //     pair 2.41 us, without either 2.79).
-// Measured (32 heads over 4, width 128, bf16): 8192 tokens 577 us, 952 TFLOP/s; 4097 tokens of 40 heads over 8 under a window of
-// 4096 419 us; 2048 tokens 50 us; 33 tokens at position 20000 37 us.  A tile pair takes about 4400 clocks, the softmax's chain of
+//   - With f32 rows (f16_products) the operands are the same f16: 11 bits of Q, K, P and V, 4e-4 of the largest output off, where a
+//     4-bit value is itself off by 1/16 of its block's largest.  Callers who want f32's precision get the decode kernel.
+// Measured (32 heads over 4, width 128, bf16; graph replay): 8192 tokens 600 to 620 us by device, 890 to 915 TFLOP/s; 4097 tokens
+// of 40 heads over 8 under a window of 4096 430 us; 2048 tokens 50 us (64-wide heads 43, f32 rows 69); 33 tokens at position
+// 20000 36 us.  A tile pair takes about 4400 clocks, the softmax's chain of
 // S wait (1000), TMEM loads, exps and P (1700 a half) for A beside the same for B; at length the device is at its power limit
 // (1000 W, 1.83 GHz).
 #include "kernels.cuh"
