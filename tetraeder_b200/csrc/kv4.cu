@@ -342,6 +342,7 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
         p_new = __shfl_sync(0xffffffffu, p_new, src);
     }
     int at = start;
+    bool dead = false;  // a wait ran out: the warp fetches nothing more, as its barriers' phases may be open
     while (at < end) {
         if (p_new < 0) {
             p_new = pos_of(++tok);
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
         const int64_t row0 = ((int64_t)(a.seq0 >= 0 ? a.seq0 : t) * c.n_kv + g) * c.n_ctx;
 
         // ---- this warp's tiles: first + warp, first + warp + WARPS, ...  Lanes 0..3 copy a plane's piece each
-        const int mine = n_part > warp ? (n_part - warp + WARPS - 1) / WARPS : 0;
+        const int mine = n_part > warp && !dead ? (n_part - warp + WARPS - 1) / WARPS : 0;
         const uint8_t *src;
         uint32_t piece, dst;
         {
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__((Kv4AttnCfg<HD, sizeof(T) == 4, SHORT>::THREAD
             }
             q_sums = t4 < 2 ? sums[0] : sums[1];
         }
-        bool dead = false, held = false;  // held: the second time, for references past 2^24 (kv4_far)
+        bool held = false;  // the second time, for references past 2^24 (kv4_far)
     tiles:
         float o[NB][2][4];  // [block][values 0, 1 or 2, 3 of 4 gr ..]: rows (value, head 2 t4 + {0, 1})
 #pragma unroll
